@@ -363,6 +363,262 @@ int dot_run(const DotGeom& g, DotProblem& p, int32_t algorithm, void* ws, size_t
   return dot_simt(p, s);
 }
 
+// ---- linear recurrence and products grouped by expert ----------------------
+
+// Elements of a buffer, or -1 when the count passes 2^60.
+int64_t total_checked(const ds_buffer* b) {
+  int64_t n = 1;
+  for (int64_t i = 0; i < b->rank; ++i)
+    if (b->dims[i] == 0) return 0;
+  for (int64_t i = 0; i < b->rank; ++i) {
+    if (b->dims[i] > (1LL << 60) / n) return -1;
+    n *= b->dims[i];
+  }
+  return n;
+}
+
+// A named buffer with the bytes its data is read in (and aligned to) and its
+// elements' size.
+struct Named {
+  const ds_buffer* b;
+  const char* name;
+  int elem;   // bytes per element
+  int align;  // bytes the kernels load at a time
+};
+
+int check_named(const std::string& op, std::initializer_list<Named> all) {
+  for (const Named& x : all) {
+    if (!valid_buffer(x.b) || bad_dims(x.b)) return invalid(op + ": invalid buffer descriptor");
+    const int64_t n = total_checked(x.b);
+    if (n < 0) return invalid(op + ": " + x.name + " is too large");
+    if (n > 0 && x.b->data == nullptr) return invalid(op + ": null data pointer");
+    if (n > 0 && !aligned(x.b->data, x.align))
+      return invalid(op + ": " + x.name + " must be " + std::to_string(x.align) + "-byte aligned");
+  }
+  return DS_OK;
+}
+
+// Outputs must not share memory with operands or with one another.
+int check_overlap(const std::string& op, std::initializer_list<Named> ins,
+                  std::initializer_list<Named> outs) {
+  auto range = [](const Named& x, uintptr_t& lo, uintptr_t& hi) {
+    lo = reinterpret_cast<uintptr_t>(x.b->data);
+    hi = lo + static_cast<uintptr_t>(total(x.b)) * x.elem;
+  };
+  auto overlap = [&](const Named& x, const Named& y) {
+    uintptr_t xl, xh, yl, yh;
+    range(x, xl, xh);
+    range(y, yl, yh);
+    return xl < yh && yl < xh && xl < xh && yl < yh;
+  };
+  for (auto o = outs.begin(); o != outs.end(); ++o) {
+    for (const Named& i : ins)
+      if (overlap(*o, i)) return invalid(op + ": " + o->name + " overlaps " + i.name);
+    for (auto q = outs.begin(); q != o; ++q)
+      if (overlap(*o, *q)) return invalid(op + ": " + o->name + " overlaps " + q->name);
+  }
+  return DS_OK;
+}
+
+bool same_dims(const ds_buffer* x, const ds_buffer* y) {
+  if (x->rank != y->rank) return false;
+  for (int64_t i = 0; i < x->rank; ++i)
+    if (x->dims[i] != y->dims[i]) return false;
+  return true;
+}
+
+// [..., T, D] (packed: [..., T, D, 2]) as B, T, D.
+int scan_geometry(const std::string& op, const ds_buffer* a, int type, ScanArgs& s) {
+  const int64_t r = a->rank - (type == DS_FUSED_PACKED ? 1 : 0);
+  if (type == DS_FUSED_PACKED && (a->rank < 1 || a->dims[a->rank - 1] != 2))
+    return invalid(op + " expects last dim == 2");
+  if (r < 2) return invalid(op + ": a must be [..., T, D]");
+  s.type = type;
+  s.B = 1;
+  for (int64_t i = 0; i < r - 2; ++i) s.B *= a->dims[i];
+  s.T = a->dims[r - 2];
+  s.D = a->dims[r - 1];
+  return DS_OK;
+}
+
+// A state [..., D] beside a = [..., T, D].
+bool state_dims(const ds_buffer* a, int type, const ds_buffer* h0) {
+  const int64_t r = a->rank - (type == DS_FUSED_PACKED ? 1 : 0);
+  if (h0->rank != a->rank - 1) return false;
+  for (int64_t i = 0, o = 0; i < a->rank; ++i) {
+    if (i == r - 2) continue;
+    if (h0->dims[o++] != a->dims[i]) return false;
+  }
+  return true;
+}
+
+int scan_elem(int type) { return type == DS_FUSED_F64 ? 8 : 4; }
+int scan_align(int type) { return type == DS_FUSED_F32 ? 4 : 8; }
+
+int scan_workspace(const std::string& op, const ScanArgs& s) {
+  const size_t need = scan_workspace_bytes(s.type, s.B, s.T, s.D);
+  if (need > s.workspace_bytes || (need && !aligned(s.workspace, 256)))
+    return invalid(op + ": workspace too small (need " + std::to_string(need) +
+                   " bytes, 256-byte aligned)");
+  if (need && s.workspace == nullptr) return invalid(op + ": null workspace");
+  return DS_OK;
+}
+
+int linear_recurrence(const char* name, int type, const ds_buffer* a, const ds_buffer* b,
+                      const ds_buffer* h0, const ds_buffer* h, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  const std::string op(name);
+  const int e = scan_elem(type), al = scan_align(type);
+  const Named A{a, "a", e, al}, B{b, "b", e, al}, H{h, "h", e, al};
+  if (int st = check_named(op, {A, B, H})) return st;
+  ScanArgs s;
+  if (int st = scan_geometry(op, a, type, s)) return st;
+  if (!same_dims(a, b)) return invalid(op + ": a and b must have the same shape");
+  if (!same_dims(a, h)) return invalid(op + ": output shape mismatch");
+  if (int st = check_overlap(op, {A, B}, {H})) return st;
+  if (h0) {
+    const Named H0{h0, "h0", e, al};
+    if (int st = check_named(op, {H0})) return st;
+    if (!state_dims(a, type, h0)) return invalid(op + ": h0 must be [..., D]");
+    if (int st = check_overlap(op, {H0}, {H})) return st;
+    s.h0 = h0->data;
+  }
+  s.a = a->data;
+  s.x = b->data;
+  s.out = h->data;
+  s.workspace = workspace;
+  s.workspace_bytes = workspace_bytes;
+  if (int st = scan_workspace(op, s)) return st;
+  return scan_launch(s, false, as_stream(stream));
+}
+
+int linear_recurrence_vjp(const char* name, int type, const ds_buffer* a, const ds_buffer* h,
+                          const ds_buffer* grad_h, const ds_buffer* h0, const ds_buffer* grad_a,
+                          const ds_buffer* grad_b, const ds_buffer* grad_h0, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  const std::string op(name);
+  const int e = scan_elem(type), al = scan_align(type);
+  const Named A{a, "a", e, al}, H{h, "h", e, al}, G{grad_h, "grad_h", e, al},
+      GA{grad_a, "grad_a", e, al}, GB{grad_b, "grad_b", e, al}, GH{grad_h0, "grad_h0", e, al};
+  if (int st = check_named(op, {A, H, G, GA, GB, GH})) return st;
+  ScanArgs s;
+  if (int st = scan_geometry(op, a, type, s)) return st;
+  if (!same_dims(a, h) || !same_dims(a, grad_h))
+    return invalid(op + ": a, h and grad_h must have the same shape");
+  if (!same_dims(a, grad_a) || !same_dims(a, grad_b) || !state_dims(a, type, grad_h0))
+    return invalid(op + ": output shape mismatch");
+  if (int st = check_overlap(op, {A, H, G}, {GA, GB, GH})) return st;
+  if (h0) {
+    const Named H0{h0, "h0", e, al};
+    if (int st = check_named(op, {H0})) return st;
+    if (!state_dims(a, type, h0)) return invalid(op + ": h0 must be [..., D]");
+    if (int st = check_overlap(op, {H0}, {GA, GB, GH})) return st;
+    s.h0 = h0->data;
+  }
+  s.a = a->data;
+  s.x = grad_h->data;
+  s.h = h->data;
+  s.out = grad_b->data;
+  s.grad_a = grad_a->data;
+  s.grad_h0 = grad_h0->data;
+  s.workspace = workspace;
+  s.workspace_bytes = workspace_bytes;
+  if (int st = scan_workspace(op, s)) return st;
+  return scan_launch(s, true, as_stream(stream));
+}
+
+// Largest rows, columns and contraction of a grouped product, and number of
+// groups: tile counts and packed indices stay inside 31 bits.
+constexpr int64_t kRaggedMax = (1LL << 31) - 1024;
+constexpr int64_t kRaggedMaxGroups = 65535;
+
+int ragged_geometry(const std::string& op, const ds_buffer* lhs, const ds_buffer* rhs,
+                    int32_t rhs_contracting, RaggedProblem& p) {
+  if (rhs_contracting != 1 && rhs_contracting != 2)
+    return invalid(op + ": rhs_contracting must be 1 or 2");
+  if (lhs->rank != 2) return invalid(op + ": lhs must be [M, K]");
+  if (rhs->rank != 3) return invalid(op + ": rhs must be [G, K, N] or [G, N, K]");
+  p.M = lhs->dims[0];
+  p.K = lhs->dims[1];
+  p.G = rhs->dims[0];
+  p.rhs_t = rhs_contracting == 2;
+  p.N = rhs->dims[p.rhs_t ? 1 : 2];
+  if (rhs->dims[rhs_contracting] != p.K)
+    return invalid(op + ": contracting dimensions must match");
+  if (p.M > kRaggedMax || p.K > kRaggedMax || p.N > kRaggedMax)
+    return invalid(op + ": dimensions must be below 2^31 - 1024");
+  if (p.G > kRaggedMaxGroups) return invalid(op + ": at most 65535 groups");
+  p.lhs.s_r = p.K;
+  p.lhs.s_k = 1;
+  p.rhs.s_b = p.K * p.N;
+  p.rhs.s_r = p.rhs_t ? p.K : 1;
+  p.rhs.s_k = p.rhs_t ? 1 : p.N;
+  return DS_OK;
+}
+
+int contract_geometry(const std::string& op, const ds_buffer* lhs, const ds_buffer* rhs,
+                      const ds_buffer* group_sizes, RaggedProblem& p) {
+  if (lhs->rank != 2 || rhs->rank != 2) return invalid(op + ": lhs must be [M, K] and rhs [M, N]");
+  if (group_sizes->rank != 1) return invalid(op + ": group_sizes must be [G]");
+  if (lhs->dims[0] != rhs->dims[0]) return invalid(op + ": contracting dimensions must match");
+  p.M = lhs->dims[0];
+  p.K = lhs->dims[1];
+  p.N = rhs->dims[1];
+  p.G = group_sizes->dims[0];
+  if (p.M > kRaggedMax || p.K > kRaggedMax || p.N > kRaggedMax)
+    return invalid(op + ": dimensions must be below 2^31 - 1024");
+  if (p.G > kRaggedMaxGroups) return invalid(op + ": at most 65535 groups");
+  if (p.K > 0 && p.N > 0 && p.G > (1LL << 60) / p.K / p.N) return invalid(op + ": too large");
+  p.lhs.s_r = 1;
+  p.lhs.s_k = p.K;
+  p.rhs.s_r = 1;
+  p.rhs.s_k = p.N;
+  return DS_OK;
+}
+
+int ragged_workspace(const std::string& op, size_t need, void* workspace, size_t bytes) {
+  if (need > bytes || (need && (workspace == nullptr || !aligned(workspace, 256))))
+    return invalid(op + ": workspace too small (need " + std::to_string(need) +
+                   " bytes, 256-byte aligned)");
+  return DS_OK;
+}
+
+int ragged_dot_checked(const std::string& op, RaggedProblem& p, std::initializer_list<Named> ins,
+                       std::initializer_list<Named> outs, const ds_buffer* group_sizes,
+                       int32_t rhs_contracting, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  const ds_buffer* lhs = ins.begin()->b;
+  const ds_buffer* rhs = (ins.end() - 2)->b;  // group_sizes is last
+  if (int st = ragged_geometry(op, lhs, rhs, rhs_contracting, p)) return st;
+  if (group_sizes->rank != 1 || group_sizes->dims[0] != p.G)
+    return invalid(op + ": group_sizes must be [G]");
+  for (const Named& o : outs)
+    if (o.b->rank != 2 || o.b->dims[0] != p.M || o.b->dims[1] != p.N)
+      return invalid(op + ": output shape mismatch");
+  if (int st = check_overlap(op, ins, outs)) return st;
+  p.group_sizes = static_cast<const int32_t*>(group_sizes->data);
+  const size_t need = ragged_dot_workspace_bytes(p.M, p.K, p.N, p.G, p.rhs_t);
+  if (int st = ragged_workspace(op, need, workspace, workspace_bytes)) return st;
+  return ragged_dot(p, workspace, workspace_bytes, as_stream(stream));
+}
+
+int ragged_contract_checked(const std::string& op, RaggedProblem& p,
+                            std::initializer_list<Named> ins, std::initializer_list<Named> outs,
+                            const ds_buffer* group_sizes, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  const ds_buffer* lhs = ins.begin()->b;
+  const ds_buffer* rhs = (ins.end() - 2)->b;
+  if (int st = contract_geometry(op, lhs, rhs, group_sizes, p)) return st;
+  for (const Named& o : outs)
+    if (o.b->rank != 3 || o.b->dims[0] != p.G || o.b->dims[1] != p.K || o.b->dims[2] != p.N)
+      return invalid(op + ": output shape mismatch");
+  if (int st = check_overlap(op, ins, outs)) return st;
+  p.group_sizes = static_cast<const int32_t*>(group_sizes->data);
+  const size_t need = ragged_contract_workspace_bytes(p.M, p.K, p.N, p.G);
+  if (int st = ragged_workspace(op, need, workspace, workspace_bytes)) return st;
+  return ragged_contract(p, workspace, workspace_bytes, as_stream(stream));
+}
+
 }  // namespace
 }  // namespace dsb
 
@@ -755,6 +1011,162 @@ int ds_dot_general_f64(const ds_buffer* lhs, const ds_buffer* rhs, const ds_dot_
   p.b.f64 = f64p(rhs);
   p.c.f64 = static_cast<double*>(out->data);
   return dot_run(g, p, algorithm, workspace, workspace_bytes, as_stream(stream));
+}
+
+size_t ds_linear_recurrence_workspace_size(const ds_buffer* a, int32_t type) {
+  if (!valid_buffer(a) || bad_dims(a) || total_checked(a) < 0) return 0;
+  if (type != DS_FUSED_F64 && type != DS_FUSED_F32 && type != DS_FUSED_PACKED) return 0;
+  const std::string saved = g_last_error;
+  ScanArgs s;
+  const int st = scan_geometry("ds_linear_recurrence", a, type, s);
+  g_last_error = saved;
+  return st == DS_OK ? scan_workspace_bytes(type, s.B, s.T, s.D) : 0;
+}
+
+int ds_linear_recurrence_f64(const ds_buffer* a, const ds_buffer* b, const ds_buffer* h0,
+                             const ds_buffer* h, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  return linear_recurrence("ds_linear_recurrence_f64", DS_FUSED_F64, a, b, h0, h, workspace,
+                           workspace_bytes, stream);
+}
+
+int ds_linear_recurrence_f32(const ds_buffer* a, const ds_buffer* b, const ds_buffer* h0,
+                             const ds_buffer* h, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  return linear_recurrence("ds_linear_recurrence_f32", DS_FUSED_F32, a, b, h0, h, workspace,
+                           workspace_bytes, stream);
+}
+
+int ds_linear_recurrence_packed(const ds_buffer* a, const ds_buffer* b, const ds_buffer* h0,
+                             const ds_buffer* h, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  return linear_recurrence("ds_linear_recurrence_packed", DS_FUSED_PACKED, a, b, h0, h, workspace,
+                           workspace_bytes, stream);
+}
+
+int ds_linear_recurrence_vjp_f64(const ds_buffer* a, const ds_buffer* h,
+                                 const ds_buffer* grad_h, const ds_buffer* h0,
+                                 const ds_buffer* grad_a, const ds_buffer* grad_b,
+                                 const ds_buffer* grad_h0, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  return linear_recurrence_vjp("ds_linear_recurrence_vjp_f64", DS_FUSED_F64, a, h, grad_h, h0,
+                               grad_a, grad_b, grad_h0, workspace, workspace_bytes, stream);
+}
+
+int ds_linear_recurrence_vjp_f32(const ds_buffer* a, const ds_buffer* h,
+                                 const ds_buffer* grad_h, const ds_buffer* h0,
+                                 const ds_buffer* grad_a, const ds_buffer* grad_b,
+                                 const ds_buffer* grad_h0, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  return linear_recurrence_vjp("ds_linear_recurrence_vjp_f32", DS_FUSED_F32, a, h, grad_h, h0,
+                               grad_a, grad_b, grad_h0, workspace, workspace_bytes, stream);
+}
+
+int ds_linear_recurrence_vjp_packed(const ds_buffer* a, const ds_buffer* h,
+                                 const ds_buffer* grad_h, const ds_buffer* h0,
+                                 const ds_buffer* grad_a, const ds_buffer* grad_b,
+                                 const ds_buffer* grad_h0, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  return linear_recurrence_vjp("ds_linear_recurrence_vjp_packed", DS_FUSED_PACKED, a, h, grad_h, h0,
+                               grad_a, grad_b, grad_h0, workspace, workspace_bytes, stream);
+}
+
+size_t ds_ragged_dot_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
+                                    int32_t rhs_contracting) {
+  if (!valid_buffer(lhs) || !valid_buffer(rhs) || bad_dims(lhs) || bad_dims(rhs)) return 0;
+  if (total_checked(lhs) < 0 || total_checked(rhs) < 0) return 0;
+  const std::string saved = g_last_error;
+  RaggedProblem p;
+  const int st = ragged_geometry("ds_ragged_dot", lhs, rhs, rhs_contracting, p);
+  g_last_error = saved;
+  return st == DS_OK ? ragged_dot_workspace_bytes(p.M, p.K, p.N, p.G, p.rhs_t) : 0;
+}
+
+int ds_ragged_dot(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo, const ds_buffer* rhs_hi,
+                  const ds_buffer* rhs_lo, const ds_buffer* group_sizes, int32_t rhs_contracting,
+                  const ds_buffer* out_hi, const ds_buffer* out_lo, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  const std::string op("ds_ragged_dot");
+  const Named LH{lhs_hi, "lhs_hi", 4, 4}, LL{lhs_lo, "lhs_lo", 4, 4}, RH{rhs_hi, "rhs_hi", 4, 4},
+      RL{rhs_lo, "rhs_lo", 4, 4}, GS{group_sizes, "group_sizes", 4, 4},
+      OH{out_hi, "out_hi", 4, 4}, OL{out_lo, "out_lo", 4, 4};
+  if (int st = check_named(op, {LH, LL, RH, RL, GS, OH, OL})) return st;
+  if (!same_dims(lhs_hi, lhs_lo) || !same_dims(rhs_hi, rhs_lo) || !same_dims(out_hi, out_lo))
+    return invalid(op + ": hi and lo tensors must have the same shape");
+  RaggedProblem p;
+  p.lhs.hi = static_cast<const float*>(lhs_hi->data);
+  p.lhs.lo = static_cast<const float*>(lhs_lo->data);
+  p.rhs.hi = static_cast<const float*>(rhs_hi->data);
+  p.rhs.lo = static_cast<const float*>(rhs_lo->data);
+  p.out.hi = static_cast<float*>(out_hi->data);
+  p.out.lo = static_cast<float*>(out_lo->data);
+  return ragged_dot_checked(op, p, {LH, LL, RH, RL, GS}, {OH, OL}, group_sizes, rhs_contracting,
+                            workspace, workspace_bytes, stream);
+}
+
+int ds_ragged_dot_f64(const ds_buffer* lhs, const ds_buffer* rhs, const ds_buffer* group_sizes,
+                      int32_t rhs_contracting, const ds_buffer* out, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  const std::string op("ds_ragged_dot_f64");
+  const Named L{lhs, "lhs", 8, 8}, R{rhs, "rhs", 8, 8}, GS{group_sizes, "group_sizes", 4, 4},
+      O{out, "out", 8, 8};
+  if (int st = check_named(op, {L, R, GS, O})) return st;
+  RaggedProblem p;
+  p.lhs.f64 = f64p(lhs);
+  p.rhs.f64 = f64p(rhs);
+  p.out.f64 = static_cast<double*>(out->data);
+  return ragged_dot_checked(op, p, {L, R, GS}, {O}, group_sizes, rhs_contracting, workspace,
+                            workspace_bytes, stream);
+}
+
+size_t ds_ragged_dot_contract_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
+                                             const ds_buffer* group_sizes) {
+  if (!valid_buffer(lhs) || !valid_buffer(rhs) || !valid_buffer(group_sizes)) return 0;
+  if (bad_dims(lhs) || bad_dims(rhs) || bad_dims(group_sizes)) return 0;
+  if (total_checked(lhs) < 0 || total_checked(rhs) < 0) return 0;
+  const std::string saved = g_last_error;
+  RaggedProblem p;
+  const int st = contract_geometry("ds_ragged_dot_contract", lhs, rhs, group_sizes, p);
+  g_last_error = saved;
+  return st == DS_OK ? ragged_contract_workspace_bytes(p.M, p.K, p.N, p.G) : 0;
+}
+
+int ds_ragged_dot_contract(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
+                           const ds_buffer* rhs_hi, const ds_buffer* rhs_lo,
+                           const ds_buffer* group_sizes, const ds_buffer* out_hi,
+                           const ds_buffer* out_lo, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  const std::string op("ds_ragged_dot_contract");
+  const Named LH{lhs_hi, "lhs_hi", 4, 4}, LL{lhs_lo, "lhs_lo", 4, 4}, RH{rhs_hi, "rhs_hi", 4, 4},
+      RL{rhs_lo, "rhs_lo", 4, 4}, GS{group_sizes, "group_sizes", 4, 4},
+      OH{out_hi, "out_hi", 4, 4}, OL{out_lo, "out_lo", 4, 4};
+  if (int st = check_named(op, {LH, LL, RH, RL, GS, OH, OL})) return st;
+  if (!same_dims(lhs_hi, lhs_lo) || !same_dims(rhs_hi, rhs_lo) || !same_dims(out_hi, out_lo))
+    return invalid(op + ": hi and lo tensors must have the same shape");
+  RaggedProblem p;
+  p.lhs.hi = static_cast<const float*>(lhs_hi->data);
+  p.lhs.lo = static_cast<const float*>(lhs_lo->data);
+  p.rhs.hi = static_cast<const float*>(rhs_hi->data);
+  p.rhs.lo = static_cast<const float*>(rhs_lo->data);
+  p.out.hi = static_cast<float*>(out_hi->data);
+  p.out.lo = static_cast<float*>(out_lo->data);
+  return ragged_contract_checked(op, p, {LH, LL, RH, RL, GS}, {OH, OL}, group_sizes, workspace,
+                                 workspace_bytes, stream);
+}
+
+int ds_ragged_dot_contract_f64(const ds_buffer* lhs, const ds_buffer* rhs,
+                               const ds_buffer* group_sizes, const ds_buffer* out,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  const std::string op("ds_ragged_dot_contract_f64");
+  const Named L{lhs, "lhs", 8, 8}, R{rhs, "rhs", 8, 8}, GS{group_sizes, "group_sizes", 4, 4},
+      O{out, "out", 8, 8};
+  if (int st = check_named(op, {L, R, GS, O})) return st;
+  RaggedProblem p;
+  p.lhs.f64 = f64p(lhs);
+  p.rhs.f64 = f64p(rhs);
+  p.out.f64 = static_cast<double*>(out->data);
+  return ragged_contract_checked(op, p, {L, R, GS}, {O}, group_sizes, workspace, workspace_bytes,
+                                 stream);
 }
 
 }  // extern "C"

@@ -121,4 +121,38 @@ int dot_ozaki_params(int64_t K, int* moduli, int* bits);
 int dot_ozaki_kernel_info(int* cta_pairs, int* query_error);
 int dot_ozaki(const DotProblem& p, void* workspace, size_t workspace_bytes, cudaStream_t s);
 
+// sequence.cu: the linear recurrence h_t = a_t h_{t-1} + x_t over [B, T, D]
+// and its gradient.  Element types: 0 f64, 1 f32, 2 packed DS pairs.
+struct ScanArgs {
+  int type = 0;
+  int64_t B = 0, T = 0, D = 0;
+  const void* a = nullptr;
+  const void* x = nullptr;   // b, or (gradient) the gradient of every h_t
+  const void* h = nullptr;   // gradient only: the recurrence's result
+  const void* h0 = nullptr;  // state before the first step; null: zeros
+  void* out = nullptr;       // h, or (gradient) the gradient of b
+  void* grad_a = nullptr;    // gradient only
+  void* grad_h0 = nullptr;   // gradient only
+  void* workspace = nullptr;
+  size_t workspace_bytes = 0;
+};
+size_t scan_workspace_bytes(int type, int64_t B, int64_t T, int64_t D);
+int scan_launch(const ScanArgs& a, bool gradient, cudaStream_t s);
+
+// ragged.cu: products grouped by expert.  Groups take group_sizes[g] (device)
+// consecutive rows each.
+struct RaggedProblem {
+  DotOperand lhs;  // [M, K]
+  DotOperand rhs;  // [G, K, N] or, with rhs_t, [G, N, K]; contraction: [M, N]
+  DotResult out;   // [M, N]; contraction: [G, K, N]
+  const int32_t* group_sizes = nullptr;
+  int64_t M = 0, K = 0, N = 0, G = 0;
+  bool rhs_t = false;
+};
+size_t ragged_dot_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, bool rhs_t);
+int ragged_dot(const RaggedProblem& p, void* workspace, size_t workspace_bytes, cudaStream_t s);
+size_t ragged_contract_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G);
+int ragged_contract(const RaggedProblem& p, void* workspace, size_t workspace_bytes,
+                    cudaStream_t s);
+
 }  // namespace dsb

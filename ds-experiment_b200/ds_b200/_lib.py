@@ -128,6 +128,19 @@ SIGNATURES = {
                               _I32, _I32, _I32, _BUF, _BUF, _BUF, _BUF, _VP], ctypes.c_int),
     "ds_fused_reduce_rows_compile_check": ([_OPS, _I32, ctypes.POINTER(_I32), ctypes.POINTER(_BUF),
                                             _I32, _I64P, _I32, _I32, _I32], ctypes.c_int),
+    "ds_linear_recurrence_workspace_size": ([_BUF, _I32], _SZ),
+    **{f"ds_linear_recurrence_{t}": ([_BUF, _BUF, _BUF, _BUF, _VP, _SZ, _VP], ctypes.c_int)
+       for t in ("f64", "f32", "packed")},
+    **{f"ds_linear_recurrence_vjp_{t}": ([_BUF, _BUF, _BUF, _BUF, _BUF, _BUF, _BUF, _VP, _SZ, _VP],
+                                         ctypes.c_int) for t in ("f64", "f32", "packed")},
+    "ds_ragged_dot_workspace_size": ([_BUF, _BUF, _I32], _SZ),
+    "ds_ragged_dot": ([_BUF, _BUF, _BUF, _BUF, _BUF, _I32, _BUF, _BUF, _VP, _SZ, _VP],
+                      ctypes.c_int),
+    "ds_ragged_dot_f64": ([_BUF, _BUF, _BUF, _I32, _BUF, _VP, _SZ, _VP], ctypes.c_int),
+    "ds_ragged_dot_contract_workspace_size": ([_BUF, _BUF, _BUF], _SZ),
+    "ds_ragged_dot_contract": ([_BUF, _BUF, _BUF, _BUF, _BUF, _BUF, _BUF, _VP, _SZ, _VP],
+                               ctypes.c_int),
+    "ds_ragged_dot_contract_f64": ([_BUF, _BUF, _BUF, _BUF, _VP, _SZ, _VP], ctypes.c_int),
     "ds_dot_tensor_plan": ([_I64, ctypes.POINTER(_I32), ctypes.POINTER(_I32)], ctypes.c_int),
     "ds_dot_tensor_kernel_info": ([ctypes.POINTER(_I32), ctypes.POINTER(_I32)], ctypes.c_int),
     "ds_profile_enable": ([ctypes.c_int], None),

@@ -34,7 +34,7 @@ class ShapeDtypeStruct:
         object.__setattr__(self, "dtype", dtype)
 
 
-F64, F32 = torch.float64, torch.float32
+F64, F32, S32 = torch.float64, torch.float32, torch.int32
 
 
 @dataclass(frozen=True)
@@ -44,7 +44,8 @@ class _Convention:
     args: Tuple[torch.dtype, ...]
     attrs: Tuple[str, ...]
     results: Tuple[torch.dtype, ...]
-    kind: str = "plain"  # plain | reduce | reduce_f64 | dot | dot_f64
+    kind: str = "plain"  # plain | reduce | reduce_f64 | dot | dot_f64 | scan | ragged | ...
+    optional: Tuple[int, ...] = ()  # operands that may be None
 
 
 CONVENTIONS: Dict[str, _Convention] = {
@@ -80,6 +81,18 @@ CONVENTIONS: Dict[str, _Convention] = {
                                        "lhs_contracting_dimensions",
                                        "rhs_contracting_dimensions", "algorithm"),
                                       (F64,), "dot_f64"),
+    "ds_linear_recurrence_f64": _Convention((F64, F64, F64), (), (F64,), "scan", (2,)),
+    "ds_linear_recurrence_f32": _Convention((F32, F32, F32), (), (F32,), "scan", (2,)),
+    "ds_linear_recurrence_packed": _Convention((F32, F32, F32), (), (F32,), "scan", (2,)),
+    "ds_linear_recurrence_vjp_f64": _Convention((F64,) * 4, (), (F64,) * 3, "scan", (3,)),
+    "ds_linear_recurrence_vjp_f32": _Convention((F32,) * 4, (), (F32,) * 3, "scan", (3,)),
+    "ds_linear_recurrence_vjp_packed": _Convention((F32,) * 4, (), (F32,) * 3, "scan", (3,)),
+    "ds_ragged_dot": _Convention((F32, F32, F32, F32, S32), ("rhs_contracting",), (F32, F32),
+                                 "ragged"),
+    "ds_ragged_dot_f64": _Convention((F64, F64, S32), ("rhs_contracting",), (F64,), "ragged"),
+    "ds_ragged_dot_contract": _Convention((F32, F32, F32, F32, S32), (), (F32, F32),
+                                          "ragged_contract"),
+    "ds_ragged_dot_contract_f64": _Convention((F64, F64, S32), (), (F64,), "ragged_contract"),
 }
 
 # The reference's target names, each bound to its replacement entry point.
@@ -107,8 +120,13 @@ REFERENCE_TARGETS = {
     "ds_dot_general_f64": "ds_dot_general_f64",
 }
 
-# target name -> libds_b200 symbol; every reference target is bound at import.
-_registry: Dict[str, str] = dict(REFERENCE_TARGETS)
+# Targets without a counterpart in the reference: the recurrence along a
+# sequence and the products grouped by expert, with their gradients.
+SEQUENCE_TARGETS = {name: name for name, c in CONVENTIONS.items()
+                    if c.kind in ("scan", "ragged", "ragged_contract")}
+
+# target name -> libds_b200 symbol; every target is bound at import.
+_registry: Dict[str, str] = {**REFERENCE_TARGETS, **SEQUENCE_TARGETS}
 
 
 def register_ffi_target(name: str, target, platform: str = "CUDA") -> None:
@@ -243,6 +261,8 @@ def _make_call(target_name: str, result_shape_dtypes):
         if len(args) != len(conv.args):
             raise TypeError(f"{target_name}: expected {len(conv.args)} operand(s), got {len(args)}")
         for i, (t, dt) in enumerate(zip(args, conv.args)):
+            if t is None and i in conv.optional:
+                continue
             _check_tensor(t, dt, f"{target_name} operand {i}")
         unknown = set(attrs) - set(conv.attrs)
         if unknown:
@@ -262,6 +282,9 @@ def _make_call(target_name: str, result_shape_dtypes):
         return _invoke(args, attrs, device, out)
 
     def _invoke(args, attrs, device, out):
+        if conv.kind in _SEQUENCE_KINDS:
+            outs = _invoke_sequence(target_name, conv, fn, results_spec, args, attrs, device, out)
+            return outs[0] if single else tuple(outs)
         outs = out if out is not None else [
             torch.empty(s.shape, dtype=s.dtype, device=device) for s in results_spec]
         keep = []
@@ -345,6 +368,62 @@ def _make_call(target_name: str, result_shape_dtypes):
         return outs[0] if single else tuple(outs)
 
     return call
+
+
+_SEQUENCE_KINDS = ("scan", "ragged", "ragged_contract")
+_SCAN_TYPES = {"f64": _lib.DS_FUSED_F64, "f32": _lib.DS_FUSED_F32, "packed": _lib.DS_FUSED_PACKED}
+# workspace sizes of the recurrences and grouped products, by (target, device,
+# operand shapes, rhs_contracting)
+_sequence_ws: Dict[tuple, int] = {}
+
+
+def _invoke_sequence(target_name, conv, fn, results_spec, args, attrs, device, out):
+    for i, t in enumerate(args):
+        if t is not None and t.device != device:
+            raise ValueError(f"{target_name} operand {i}: operands must be on one device")
+    if out is None:
+        out = [torch.empty(s.shape, dtype=s.dtype, device=device) for s in results_spec]
+    else:
+        for i, t in enumerate(out):
+            if t.device != device:
+                raise ValueError(f"{target_name} result {i}: results must be on the operands' device")
+    keep = []
+
+    def ref(t):
+        if t is None:
+            return None
+        b, d = _lib.make_buffer(t.data_ptr(), t.shape)
+        keep.append((b, d))
+        return ctypes.byref(b)
+
+    refs = [ref(t) for t in args]
+    tail = [ref(t) for t in out]
+    L = _lib.lib()
+    if conv.kind == "scan":
+        key = (target_name, device.index, args[0].shape)
+    else:
+        contracting = int(attrs.get("rhs_contracting", 1))
+        key = (target_name, device.index, args[0].shape, args[-2].shape, args[-1].shape,
+               contracting)
+        if conv.kind == "ragged":
+            tail.insert(0, contracting)
+    ws_bytes = _sequence_ws.get(key)
+    if ws_bytes is None:
+        if conv.kind == "scan":
+            ws_bytes = L.ds_linear_recurrence_workspace_size(
+                refs[0], _SCAN_TYPES[fn.__name__.rsplit("_", 1)[1]])
+        elif conv.kind == "ragged":
+            ws_bytes = L.ds_ragged_dot_workspace_size(refs[0], refs[-2], contracting)
+        else:
+            ws_bytes = L.ds_ragged_dot_contract_workspace_size(refs[0], refs[-2], refs[-1])
+        if len(_sequence_ws) > 1024:
+            _sequence_ws.clear()
+        _sequence_ws[key] = ws_bytes
+    stream = _lib.current_stream_ptr(device)
+    ws = _workspace(ws_bytes, device, stream) if ws_bytes else None
+    wsp = None if ws is None else ws.data_ptr()
+    _lib.check(fn(*refs, *tail, wsp, ws_bytes, stream), target_name)
+    return out
 
 
 def _dot_dims(attrs, lhs_rank) -> _lib.DsDotDims:

@@ -269,3 +269,94 @@ def ds_dot_general_f64(lhs, rhs, lhs_contracting=None, rhs_contracting=None, lhs
 def ds_matmul_f64(A, B, algorithm: str = "tensor"):
     """A[M, K] @ B[K, N] in DS arithmetic, f64 in and out."""
     return ds_dot_general_f64(A, B, algorithm=algorithm)
+
+
+# ---- linear recurrence along a sequence ---------------------------------------------
+
+def _state_shape(shape, packed=False):
+    """[..., D] of [..., T, D] (packed: [..., D, 2] of [..., T, D, 2])."""
+    shape = tuple(shape)
+    at = len(shape) - (3 if packed else 2)
+    return shape[:max(at, 0)] + shape[at + 1:] if at >= 0 else shape
+
+
+def ds_linear_recurrence_f64(a, b, h0=None, out=None):
+    """h_t = a_t h_{t-1} + b_t along dim -2 of f64 a, b [..., T, D], from the
+    state h0 [..., D] (default zeros) -> h [..., T, D].  T = 1 advances the
+    state by one step; a_t = 0 starts a new sequence."""
+    return ffi_call("ds_linear_recurrence_f64", _sds(a.shape, F64))(a, b, h0, out=out)
+
+
+def ds_linear_recurrence_f32(a, b, h0=None, out=None):
+    """ds_linear_recurrence_f64 of f32 tensors: the state is held in f64 and
+    each h_t rounded once."""
+    return ffi_call("ds_linear_recurrence_f32", _sds(a.shape, F32))(a, b, h0, out=out)
+
+
+def ds_linear_recurrence_packed(a, b, h0=None, out=None):
+    """ds_linear_recurrence_f64 of packed DS tensors [..., T, D, 2] and
+    h0 [..., D, 2]."""
+    return ffi_call("ds_linear_recurrence_packed", _sds(a.shape, F32))(a, b, h0, out=out)
+
+
+def _recurrence_vjp(kind, dtype, a, h, grad_h, h0, out):
+    seq = _sds(a.shape, dtype)
+    res = (seq, seq, _sds(_state_shape(a.shape, kind == "packed"), dtype))
+    return ffi_call(f"ds_linear_recurrence_vjp_{kind}", res)(a, h, grad_h, h0, out=out)
+
+
+def ds_linear_recurrence_vjp_f64(a, h, grad_h, h0=None, out=None):
+    """The gradient of h = ds_linear_recurrence_f64(a, b, h0): with grad_h
+    [..., T, D] the gradient of every h_t -> (grad_a, grad_b [..., T, D],
+    grad_h0 [..., D])."""
+    return _recurrence_vjp("f64", F64, a, h, grad_h, h0, out)
+
+
+def ds_linear_recurrence_vjp_f32(a, h, grad_h, h0=None, out=None):
+    """ds_linear_recurrence_vjp_f64 of f32 tensors."""
+    return _recurrence_vjp("f32", F32, a, h, grad_h, h0, out)
+
+
+def ds_linear_recurrence_vjp_packed(a, h, grad_h, h0=None, out=None):
+    """ds_linear_recurrence_vjp_f64 of packed DS tensors."""
+    return _recurrence_vjp("packed", F32, a, h, grad_h, h0, out)
+
+
+# ---- products grouped by expert -------------------------------------------------------
+
+def _ragged_shape(lhs, rhs, rhs_contracting):
+    return tuple(lhs.shape[:1]) + tuple(rhs.shape[3 - int(rhs_contracting):][:1])
+
+
+def ds_ragged_dot_f64(lhs, rhs, group_sizes, rhs_contracting: int = 1, out=None):
+    """Rows of consecutive groups, each times its group's matrix: f64 lhs
+    [M, K], rhs [G, K, N] (rhs_contracting=2: [G, N, K]), int32 group_sizes
+    [G] on the device -> [M, N], zeros in rows behind the last group.  The
+    gradient of the rows is this product of the result's gradient with the
+    same matrices and the other rhs_contracting; that of the matrices is
+    ds_ragged_dot_contract_f64."""
+    res = _sds(_ragged_shape(lhs, rhs, rhs_contracting), F64)
+    return ffi_call("ds_ragged_dot_f64", res)(lhs, rhs, group_sizes,
+                                              rhs_contracting=rhs_contracting, out=out)
+
+
+def ds_ragged_dot(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes, rhs_contracting: int = 1, out=None):
+    """ds_ragged_dot_f64 on SoA DS operands -> (hi, lo)."""
+    res = _sds(_ragged_shape(lhs_hi, rhs_hi, rhs_contracting), F32)
+    return ffi_call("ds_ragged_dot", (res, res))(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes,
+                                                 rhs_contracting=rhs_contracting, out=out)
+
+
+def ds_ragged_dot_contract_f64(lhs, rhs, group_sizes, out=None):
+    """out[g] = lhs_g^T rhs_g over the rows of each group: f64 lhs [M, K],
+    rhs [M, N], int32 group_sizes [G] -> [G, K, N].  With lhs the rows and
+    rhs the result's gradient: the gradient of ds_ragged_dot_f64's matrices."""
+    res = _sds((group_sizes.shape[0],) + tuple(lhs.shape[1:2]) + tuple(rhs.shape[1:2]), F64)
+    return ffi_call("ds_ragged_dot_contract_f64", res)(lhs, rhs, group_sizes, out=out)
+
+
+def ds_ragged_dot_contract(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes, out=None):
+    """ds_ragged_dot_contract_f64 on SoA DS operands -> (hi, lo)."""
+    res = _sds((group_sizes.shape[0],) + tuple(lhs_hi.shape[1:2]) + tuple(rhs_hi.shape[1:2]), F32)
+    return ffi_call("ds_ragged_dot_contract", (res, res))(lhs_hi, lhs_lo, rhs_hi, rhs_lo,
+                                                          group_sizes, out=out)

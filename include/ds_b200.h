@@ -414,6 +414,110 @@ DS_API int ds_fused_reduce_rows_compile_check(const ds_fused_op* ops, int32_t n_
                                               const int64_t* dims, int32_t rank,
                                               int32_t n_reduced, int32_t body);
 
+/* ---- linear recurrence along a sequence ---------------------------------- */
+
+/* h_t = a_t h_{t-1} + b_t along the second-to-last dimension: a, b, h are
+   [..., T, D] (packed: [..., T, D, 2]), T >= 0 steps of D independent
+   channels for every index of the leading dimensions, and h0 [..., D]
+   (packed [..., D, 2]) is the state before the first step; h0 = NULL stands
+   for zeros.  The reference's recurrence (cpp/ds_recurrence_add_mul_to_f64_
+   cuda.cu:98-149) applies one coefficient k times to every element alone;
+   here the coefficient changes with the step (the gated linear recurrence of
+   a sequence model), a_t = 0 starts a new sequence, and T = 1 advances a
+   state by one token.
+   Every value enters as its exact f64 value (f64, f32, or hi + lo of a packed
+   pair), the state is held in f64 (one FMA per step), and each h_t is rounded
+   once to the output's type.  Long sequences are cut into chunks whose
+   carries meet in an order fixed by the shape, so results are deterministic.
+   A NaN or infinite state stays non-finite for the rest of its sequence, as
+   in the step-by-step loop; products of up to a chunk's coefficients are
+   formed, so a state that would leave the f64 range and come back inside a
+   chunk may differ from that loop.
+   Outputs must not overlap operands.  The workspace
+   (ds_linear_recurrence_workspace_size bytes, 256-byte aligned; `type` is
+   DS_FUSED_F64, DS_FUSED_F32 or DS_FUSED_PACKED) serves one call at a time. */
+DS_API size_t ds_linear_recurrence_workspace_size(const ds_buffer* a, int32_t type);
+DS_API int ds_linear_recurrence_f64(const ds_buffer* a, const ds_buffer* b, const ds_buffer* h0,
+                                    const ds_buffer* h, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+DS_API int ds_linear_recurrence_f32(const ds_buffer* a, const ds_buffer* b, const ds_buffer* h0,
+                                    const ds_buffer* h, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+DS_API int ds_linear_recurrence_packed(const ds_buffer* a, const ds_buffer* b,
+                                       const ds_buffer* h0, const ds_buffer* h, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/* The gradient of the recurrence: with grad_h [..., T, D] the gradient of
+   every h_t (add a final state's gradient to the last step's),
+     g_t = grad_h_t + a_{t+1} g_{t+1},  grad_b_t = g_t,
+     grad_a_t = g_t h_{t-1},            grad_h0 = a_0 g_0,
+   with h the recurrence's own result and h_{-1} = h0 (NULL: zeros).  grad_h0
+   [..., D] is always written (zeros for T = 0).  Types, chunks and workspace
+   as above. */
+DS_API int ds_linear_recurrence_vjp_f64(const ds_buffer* a, const ds_buffer* h,
+                                        const ds_buffer* grad_h, const ds_buffer* h0,
+                                        const ds_buffer* grad_a, const ds_buffer* grad_b,
+                                        const ds_buffer* grad_h0, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+DS_API int ds_linear_recurrence_vjp_f32(const ds_buffer* a, const ds_buffer* h,
+                                        const ds_buffer* grad_h, const ds_buffer* h0,
+                                        const ds_buffer* grad_a, const ds_buffer* grad_b,
+                                        const ds_buffer* grad_h0, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+DS_API int ds_linear_recurrence_vjp_packed(const ds_buffer* a, const ds_buffer* h,
+                                           const ds_buffer* grad_h, const ds_buffer* h0,
+                                           const ds_buffer* grad_a, const ds_buffer* grad_b,
+                                           const ds_buffer* grad_h0, void* workspace,
+                                           size_t workspace_bytes, void* stream);
+
+/* ---- products grouped by expert ------------------------------------------- */
+
+/* Rows of consecutive groups, each times its group's matrix (the form of
+   jax.lax.ragged_dot; the reference has only the dot_general of
+   DsTransformPass.cpp:337-370): lhs [M, K], group_sizes s32[G] in device
+   memory, rhs [G, K, N] (rhs_contracting = 1) or [G, N, K]
+   (rhs_contracting = 2: the gradient of the rows is this product of the
+   result's gradient with the same matrices).  Row i of `out` [M, N] is row i
+   of lhs times the matrix of the group it lies in, groups taking
+   group_sizes[g] rows each in order; rows behind the last group are zeros.
+   Sizes are read on the device, so a captured call may be replayed with
+   others: a negative size counts as 0, and groups end at row M.  A group with
+   no rows does not read its matrix.
+   Operands are f64, or DS pairs as hi / lo tensors of one shape; the result
+   is rounded once from f64 accumulations (CUDA-core and small groups) or
+   from the exact integer products of ds_dot_general's tensor-core path.  Row
+   i depends on the group sizes only through the group it lies in and that
+   group's size.  `out` must not overlap operands.  Workspace: the query's
+   bytes, 256-byte aligned. */
+DS_API size_t ds_ragged_dot_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
+                                           int32_t rhs_contracting);
+DS_API int ds_ragged_dot(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
+                         const ds_buffer* rhs_hi, const ds_buffer* rhs_lo,
+                         const ds_buffer* group_sizes, int32_t rhs_contracting,
+                         const ds_buffer* out_hi, const ds_buffer* out_lo, void* workspace,
+                         size_t workspace_bytes, void* stream);
+DS_API int ds_ragged_dot_f64(const ds_buffer* lhs, const ds_buffer* rhs,
+                             const ds_buffer* group_sizes, int32_t rhs_contracting,
+                             const ds_buffer* out, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* The groups along the contraction: lhs [M, K], rhs [M, N], group_sizes
+   s32[G] -> out [G, K, N], out[g] = lhs_g^T rhs_g over the rows of group g
+   (zeros for a group without rows; rows behind the last group take no part).
+   With lhs the rows and rhs the gradient of ds_ragged_dot's result this is
+   the gradient of its matrices.  Group sizes, types, overlap and workspace
+   as above. */
+DS_API size_t ds_ragged_dot_contract_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
+                                                    const ds_buffer* group_sizes);
+DS_API int ds_ragged_dot_contract(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
+                                  const ds_buffer* rhs_hi, const ds_buffer* rhs_lo,
+                                  const ds_buffer* group_sizes, const ds_buffer* out_hi,
+                                  const ds_buffer* out_lo, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+DS_API int ds_ragged_dot_contract_f64(const ds_buffer* lhs, const ds_buffer* rhs,
+                                      const ds_buffer* group_sizes, const ds_buffer* out,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- diagnostics (no reference counterpart) ------------------------------ */
 
 /* Per-kernel GPU time.  While enabled, each op brackets its main kernel with
