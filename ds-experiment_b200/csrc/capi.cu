@@ -456,7 +456,7 @@ int scan_elem(int type) { return type == DS_FUSED_F64 ? 8 : 4; }
 int scan_align(int type) { return type == DS_FUSED_F32 ? 4 : 8; }
 
 int scan_workspace(const std::string& op, const ScanArgs& s) {
-  const size_t need = scan_workspace_bytes(s.B, s.T, s.D);
+  const size_t need = scan_workspace_bytes(s.type, s.B, s.T, s.D);
   if (need > s.workspace_bytes || (need && !aligned(s.workspace, 256)))
     return invalid(op + ": workspace too small (need " + std::to_string(need) +
                    " bytes, 256-byte aligned)");
@@ -1020,7 +1020,7 @@ size_t ds_linear_recurrence_workspace_size(const ds_buffer* a, int32_t type) {
   ScanArgs s;
   const int st = scan_geometry("ds_linear_recurrence", a, type, s);
   g_last_error = saved;
-  return st == DS_OK ? scan_workspace_bytes(s.B, s.T, s.D) : 0;
+  return st == DS_OK ? scan_workspace_bytes(s.type, s.B, s.T, s.D) : 0;
 }
 
 int ds_linear_recurrence_f64(const ds_buffer* a, const ds_buffer* b, const ds_buffer* h0,

@@ -136,7 +136,7 @@ struct ScanArgs {
   void* workspace = nullptr;
   size_t workspace_bytes = 0;
 };
-size_t scan_workspace_bytes(int64_t B, int64_t T, int64_t D);
+size_t scan_workspace_bytes(int type, int64_t B, int64_t T, int64_t D);
 int scan_launch(const ScanArgs& a, bool gradient, cudaStream_t s);
 
 // ragged.cu: products grouped by expert.  Groups take group_sizes[g] (device)

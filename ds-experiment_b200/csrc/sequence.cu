@@ -51,6 +51,10 @@ template <> struct SeqIO<double> {
   static __device__ __forceinline__ double zero() { return 0.0; }
   static __device__ __forceinline__ double one() { return 1.0; }
   static __device__ __forceinline__ void store(double* p, double v) { __stcs(p, v); }
+  template <int V> static __device__ __forceinline__ void put(double* p, const double (&v)[V]) {
+    if constexpr (V == 1) store(p, v[0]);
+    else __stcs(reinterpret_cast<double2*>(p), make_double2(v[0], v[1]));
+  }
 };
 template <> struct SeqIO<float> {
   static __device__ __forceinline__ float load(const float* p) { return __ldcs(p); }
@@ -59,6 +63,11 @@ template <> struct SeqIO<float> {
   static __device__ __forceinline__ float one() { return 1.0f; }
   static __device__ __forceinline__ void store(float* p, double v) {
     __stcs(p, __double2float_rn(v));
+  }
+  template <int V> static __device__ __forceinline__ void put(float* p, const double (&v)[V]) {
+    if constexpr (V == 1) store(p, v[0]);
+    else __stcs(reinterpret_cast<float2*>(p),
+                make_float2(__double2float_rn(v[0]), __double2float_rn(v[1])));
   }
 };
 template <> struct SeqIO<float2> {
@@ -69,6 +78,14 @@ template <> struct SeqIO<float2> {
   static __device__ __forceinline__ void store(float2* p, double v) {
     const ds2 d = from_f64(v);
     __stcs(p, make_float2(d.hi, d.lo));
+  }
+  template <int V> static __device__ __forceinline__ void put(float2* p, const double (&v)[V]) {
+    if constexpr (V == 1) {
+      store(p, v[0]);
+    } else {
+      const ds2 d = from_f64(v[0]), e = from_f64(v[1]);
+      __stcs(reinterpret_cast<float4*>(p), make_float4(d.hi, d.lo, e.hi, e.lo));
+    }
   }
 };
 
@@ -139,10 +156,11 @@ template <class E>
 struct ChunkArgs {
   const E *a, *x, *h, *h0;
   E *out, *ga, *gh0;
-  int64_t C, T, D;  // channels of all sequences, steps, channels of one
-  int64_t tiles;    // of CT channels
-  int64_t chunks, units;
-  int round;         // chunks per round, at most kMaxRound
+  uint32_t C, D;      // channels of all sequences, of one
+  int64_t T;          // steps
+  uint32_t tiles;     // of CT channels
+  uint32_t chunks, units;
+  uint32_t round;     // chunks per round, at most kMaxRound
   uint32_t* counter;  // units taken, minus one (null: one chunk, nothing to wait for)
   uint32_t* err;      // all ones, or 1 when a wait has run out
   ulonglong2* maps;   // [chunks][tiles][CT]
@@ -150,7 +168,7 @@ struct ChunkArgs {
 };
 
 #ifndef SEQ_MR
-#define SEQ_MR 24
+#define SEQ_MR 16
 #endif
 constexpr int kMaxRound = SEQ_MR;
 constexpr uint64_t kEmpty = ~0ull;
@@ -186,7 +204,7 @@ __device__ __forceinline__ uint64_t look_at_state(const uint64_t* at) {
 }
 
 // Whether to look again: false about 2 s after t0, or when another wait has
-// run out.
+// run out.  Asked every 64th look only: it reads memory itself.
 __device__ __noinline__ bool keep_waiting(long long t0, uint32_t* err) {
   if (*reinterpret_cast<volatile uint32_t*>(err) == 1u) return false;
   if (clock64() - t0 <= kTimeoutCycles) return true;
@@ -194,232 +212,337 @@ __device__ __noinline__ bool keep_waiting(long long t0, uint32_t* err) {
   return false;
 }
 
+// Looks until the value is there; false when the wait runs out.
+template <class Look>
+__device__ __forceinline__ bool poll(Look look, uint32_t* err) {
+  const long long t0 = clock64();
+  for (uint32_t n = 1; !look(); ++n)
+    if (n % 64 == 0 && !keep_waiting(t0, err)) return false;
+  return true;
+}
+
 __device__ __forceinline__ Map wait_map(const ulonglong2* at, ulonglong2 v, uint32_t* err) {
-  if (v.x == kEmpty) {
-    const long long t0 = clock64();
-    do {
-      if (!keep_waiting(t0, err)) {
-        v.x = v.y = 0x7ff8000000000000ull;
-        break;
-      }
-      v = look_at_map(at);
-    } while (v.x == kEmpty);
-  }
+  if (v.x == kEmpty && !poll([&] { return (v = look_at_map(at)).x != kEmpty; }, err))
+    v.x = v.y = 0x7ff8000000000000ull;
   return Map{__longlong_as_double(static_cast<long long>(v.x)),
              __longlong_as_double(static_cast<long long>(v.y))};
 }
 
 __device__ __forceinline__ double wait_state(const uint64_t* at, uint32_t* err) {
-  uint64_t v = look_at_state(at);
-  if (v == kEmpty) {
-    const long long t0 = clock64();
-    do {
-      if (!keep_waiting(t0, err)) {
-        v = 0x7ff8000000000000ull;
-        break;
-      }
-      v = look_at_state(at);
-    } while (v == kEmpty);
-  }
+  uint64_t v = kEmpty;
+  if (!poll([&] { return (v = look_at_state(at)) != kEmpty; }, err)) v = 0x7ff8000000000000ull;
   return __longlong_as_double(static_cast<long long>(v));
 }
 
-template <class E>
-__device__ __forceinline__ void copy_async(E* dst, const E* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
-                   static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
-               "l"(src), "n"(sizeof(E))
-               : "memory");
+// V neighbouring channels, moved as one word.
+template <class E, int V>
+struct alignas(sizeof(E) * V) Word {
+  E v[V];
+};
+
+template <class W>
+__device__ __forceinline__ void copy_async(W* dst, const void* src) {
+  static_assert(sizeof(W) == 4 || sizeof(W) == 8 || sizeof(W) == 16, "cp.async sizes");
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  if constexpr (sizeof(W) == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(src), "n"(sizeof(W))
+                 : "memory");
 }
 
-// One thread's part of a unit: R steps of a channel.
+// One thread's part of a unit: R steps of V channels.
 struct Part {
-  int64_t chunk, tile;
-  int64_t c;     // channel
+  uint32_t chunk, tile;
+  int64_t c;     // first channel
   int64_t p0;    // first step (gradient: counted from the end)
-  int64_t base;  // element of the channel's first row
   int64_t row;   // element of the first step's row
   int n;         // steps it has
 };
 
-template <class E, int CT, int R, bool kGrad>
-__device__ __forceinline__ Part part_of(const ChunkArgs<E>& p, int64_t unit) {
-  constexpr int S = kThreads / CT;
+template <class E, int V, int CT, int R, bool kGrad>
+__device__ __forceinline__ Part part_of(const ChunkArgs<E>& p, uint32_t unit) {
+  constexpr int N = CT / V, S = kThreads / N;
   Part q;
   q.chunk = unit / p.tiles;
   q.tile = unit - q.chunk * p.tiles;
-  q.c = q.tile * CT + threadIdx.x % CT;
-  const int64_t seq = q.c / p.D;
-  q.base = seq * p.T * p.D + (q.c - seq * p.D);
-  q.p0 = (q.chunk * S + threadIdx.x / CT) * R;
-  const int64_t left = q.c < p.C ? p.T - q.p0 : 0;
+  const uint32_t c = q.tile * CT + threadIdx.x % N * V;
+  const uint32_t seq = c / p.D;
+  q.c = c;
+  q.p0 = (static_cast<int64_t>(q.chunk) * S + threadIdx.x / N) * R;
+  const int64_t left = c < p.C ? p.T - q.p0 : 0;
   q.n = left < 0 ? 0 : left < R ? static_cast<int>(left) : R;
-  q.row = q.base + (kGrad ? p.T - 1 - q.p0 : q.p0) * p.D;
+  q.row = (seq * p.T + (kGrad ? p.T - 1 - q.p0 : q.p0)) * p.D + (c - seq * p.D);
   return q;
 }
 
-template <class E, int R, bool kGrad>
+template <class E, int V, int R, bool kGrad>
 constexpr size_t stage_bytes() {
-  return sizeof(E) * (kGrad ? 3 : 2) * R * kThreads;
+  return sizeof(E) * V * (kGrad ? 3 : 2) * R * kThreads;
 }
 
-template <class E, int CT, int R, bool kGrad>
+// A thread's slots in shared memory: R words each of the coefficients, the
+// added values and (gradient) the states before.
+template <class E, int V, int R>
+struct Slots {
+  Word<E, V> *a, *x, *h;
+};
+
+// Values of a part on their way.  kFull: it has all R steps.
+template <bool kFull, class E, int V, int R, bool kGrad>
+__device__ __forceinline__ void issue_part(const ChunkArgs<E>& p, const Part& q,
+                                           const Slots<E, V, R>& s) {
+  const int64_t dir = kGrad ? -static_cast<int64_t>(p.D) : static_cast<int64_t>(p.D);
+  const E* x = p.x + q.row;
+  const E* a = p.a + q.row + (kGrad ? p.D : 0);
+  const E* h = kGrad ? p.h + q.row - p.D : nullptr;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (!kFull && i >= q.n) break;
+    copy_async(s.x + i * kThreads, x);
+    if constexpr (kGrad) {
+      // the last step in time has no coefficient after it, the first one the
+      // state h0 before it
+      if (i > 0 || q.p0 > 0) copy_async(s.a + i * kThreads, a);
+      if ((kFull && i < R - 1) || q.p0 + i < p.T - 1) copy_async(s.h + i * kThreads, h);
+      else if (p.h0) copy_async(s.h + i * kThreads, p.h0 + q.c);
+      h += dir;
+    } else {
+      copy_async(s.a + i * kThreads, a);
+    }
+    x += dir;
+    a += dir;
+  }
+}
+
+template <class E, int V, int R, bool kGrad>
+__device__ __forceinline__ void issue(const ChunkArgs<E>& p, const Part& q,
+                                      const Slots<E, V, R>& s) {
+  if (q.n == R) issue_part<true, E, V, R, kGrad>(p, q, s);
+  else if (q.n > 0) issue_part<false, E, V, R, kGrad>(p, q, s);
+}
+
+template <class E, int V, int R, bool kGrad>
+struct Values {
+  Word<E, V> a[R], x[R], h[kGrad ? R : 1];
+};
+
+// Steps that the part does not have do nothing: s -> 1 s + 0.
+template <class E, int V, int R, bool kGrad>
+__device__ __forceinline__ void read(const ChunkArgs<E>& p, const Part& q, const Slots<E, V, R>& s,
+                                     Values<E, V, R, kGrad>& v) {
+  using IO = SeqIO<E>;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const bool in = i < q.n;
+    v.x[i] = s.x[i * kThreads];
+    v.a[i] = s.a[i * kThreads];
+    if constexpr (kGrad) v.h[i] = s.h[i * kThreads];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!in) v.x[i].v[j] = IO::zero();
+      if (!in || (kGrad && i == 0 && q.p0 == 0)) v.a[i].v[j] = IO::one();
+      if constexpr (kGrad) {
+        if (!p.h0 && q.p0 + i == p.T - 1) v.h[i].v[j] = IO::zero();
+      }
+    }
+  }
+}
+
+// The steps from `state` on, stored.
+template <bool kFull, class E, int V, int R, bool kGrad>
+__device__ __forceinline__ void run_part(const ChunkArgs<E>& p, const Part& q,
+                                         const Values<E, V, R, kGrad>& v, double (&state)[V]) {
+  using IO = SeqIO<E>;
+  const int64_t dir = kGrad ? -static_cast<int64_t>(p.D) : static_cast<int64_t>(p.D);
+  E* out = p.out + q.row;
+  E* ga = kGrad ? p.ga + q.row : nullptr;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (!kFull && i >= q.n) break;
+    double g[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      state[j] = __fma_rn(IO::value(v.a[i].v[j]), state[j], IO::value(v.x[i].v[j]));
+      if constexpr (kGrad) g[j] = __dmul_rn(state[j], IO::value(v.h[i].v[j]));
+    }
+    IO::template put<V>(out, state);
+    out += dir;
+    if constexpr (kGrad) {
+      IO::template put<V>(ga, g);
+      ga += dir;
+      if ((!kFull || i == R - 1) && q.p0 + i == p.T - 1) {
+        const E* a0 = p.a + q.row + i * dir;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          IO::store(p.gh0 + q.c + j, __dmul_rn(IO::value(IO::load(a0 + j)), state[j]));
+      }
+    }
+  }
+}
+
+template <class E, int V, int CT, int R, bool kGrad>
 __global__ void __launch_bounds__(kThreads, 2)
 scan_chunk_kernel(const __grid_constant__ ChunkArgs<E> p) {
-  constexpr int S = kThreads / CT;  // threads of one channel
+  constexpr int N = CT / V;         // threads across the channels
+  constexpr int S = kThreads / N;   // and along the steps
   using IO = SeqIO<E>;
   extern __shared__ __align__(16) uint8_t smem[];
-  E* stage_a = reinterpret_cast<E*>(smem) + threadIdx.x;
-  E* stage_x = stage_a + R * kThreads;
-  E* stage_h = stage_x + R * kThreads;  // gradient only
+  Slots<E, V, R> slots;
+  slots.a = reinterpret_cast<Word<E, V>*>(smem) + threadIdx.x;
+  slots.x = slots.a + R * kThreads;
+  slots.h = slots.x + R * kThreads;  // gradient only
   __shared__ Map s_map[2][S][CT];
   __shared__ Map s_before[kMaxRound][CT];
   __shared__ double s_start[CT];
   __shared__ uint32_t s_unit[2];
-  const int cl = threadIdx.x % CT, sub = threadIdx.x / CT;
-
-  auto issue = [&](const Part& q) {
-    const int64_t dir = kGrad ? -p.D : p.D;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (i < q.n) {
-        const int64_t at = q.row + i * dir;
-        copy_async(stage_x + i * kThreads, p.x + at);
-        if constexpr (kGrad) {
-          if (q.p0 + i > 0) copy_async(stage_a + i * kThreads, p.a + at + p.D);
-          if (q.p0 + i < p.T - 1) copy_async(stage_h + i * kThreads, p.h + at - p.D);
-          else if (p.h0) copy_async(stage_h + i * kThreads, p.h0 + q.c);
-        } else {
-          copy_async(stage_a + i * kThreads, p.a + at);
-        }
-      }
-    }
-  };
+  const int tid = threadIdx.x, cl = tid % N * V, sub = tid / N;
 
   wait_previous_grid();
-  int64_t unit = blockIdx.x;
+  uint32_t unit = blockIdx.x;
   if (p.counter) {
-    if (threadIdx.x == 0) s_unit[0] = atomicAdd(p.counter, 1u) + 1u;
+    if (tid == 0) s_unit[0] = atomicAdd(p.counter, 1u) + 1u;
     __syncthreads();
     unit = s_unit[0];
   }
   Part q{};
   if (unit < p.units) {
-    q = part_of<E, CT, R, kGrad>(p, unit);
-    issue(q);
+    q = part_of<E, V, CT, R, kGrad>(p, unit);
+    issue<E, V, R, kGrad>(p, q, slots);
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
   int turn = 0;
   while (unit < p.units) {
     turn ^= 1;
-    if (p.counter && threadIdx.x == 0) s_unit[turn] = atomicAdd(p.counter, 1u) + 1u;
+    if (p.counter && tid == 0) s_unit[turn] = atomicAdd(p.counter, 1u) + 1u;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    E av[R], xv[R], hv[kGrad ? R : 1];
+    Values<E, V, R, kGrad> val;
+    read<E, V, R, kGrad>(p, q, slots, val);
+    Map m[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) m[j] = Map{1.0, 0.0};
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const bool in = i < q.n;
-      xv[i] = in ? stage_x[i * kThreads] : IO::zero();
-      av[i] = in && (!kGrad || q.p0 + i > 0) ? stage_a[i * kThreads] : IO::one();
-      if constexpr (kGrad)
-        hv[i] = in && (q.p0 + i < p.T - 1 || p.h0) ? stage_h[i * kThreads] : IO::zero();
-    }
-    Map m{1.0, 0.0};
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const double a = IO::value(av[i]);
-      m.s = __fma_rn(a, m.s, IO::value(xv[i]));
-      m.p = __dmul_rn(m.p, a);
+      for (int j = 0; j < V; ++j) {
+        const double a = IO::value(val.a[i].v[j]);
+        m[j].s = __fma_rn(a, m[j].s, IO::value(val.x[i].v[j]));
+        m[j].p = __dmul_rn(m[j].p, a);
+      }
     }
     // inclusive scan over the S threads of a channel
     int buf = 0;
-    s_map[0][sub][cl] = m;
+#pragma unroll
+    for (int j = 0; j < V; ++j) s_map[0][sub][cl + j] = m[j];
     __syncthreads();
-    const int64_t next = p.counter ? static_cast<int64_t>(s_unit[turn]) : unit + gridDim.x;
+    const uint32_t next = p.counter ? s_unit[turn] : unit + gridDim.x;
     const Part cur = q;
     if (next < p.units) {
-      q = part_of<E, CT, R, kGrad>(p, next);
-      issue(q);
+      q = part_of<E, V, CT, R, kGrad>(p, next);
+      issue<E, V, R, kGrad>(p, q, slots);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
     for (int d = 1; d < S; d <<= 1) {
-      if (sub >= d) m = compose(s_map[buf][sub - d][cl], m);
       buf ^= 1;
-      s_map[buf][sub][cl] = m;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (sub >= d) m[j] = compose(s_map[buf ^ 1][sub - d][cl + j], m[j]);
+        s_map[buf][sub][cl + j] = m[j];
+      }
       __syncthreads();
     }
-    double start = 0.0;  // state at the chunk's start (threads of sub 0)
+    // the state at the chunk's start, by one thread per channel (cs)
+    const int cs = tid;
+    const int64_t channel = static_cast<int64_t>(cur.tile) * CT + cs;
     if (p.counter) {
-      const int64_t slot = cur.chunk * p.tiles + cur.tile;
-      const int64_t rnd = cur.chunk / p.round;
+      const int64_t slot = static_cast<int64_t>(cur.chunk) * p.tiles + cur.tile;
+      const uint32_t rnd = cur.chunk / p.round;
       const int idx = static_cast<int>(cur.chunk - rnd * p.round);
-      const bool last = cur.chunk == p.chunks - 1, ends = idx == p.round - 1;
+      const bool last = cur.chunk == p.chunks - 1, ends = idx == static_cast<int>(p.round) - 1;
       // a later chunk of the round reads it
-      if (!last && !ends && sub == S - 1) put_map(p.maps + slot * CT + cl, m);
-      const ulonglong2* maps = p.maps + (slot - idx * p.tiles) * CT + cl;
-      const int64_t step = p.tiles * CT;
-      for (int i = sub; i < idx; i += 4 * S) {
+      if (!last && !ends && sub == S - 1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) put_map(p.maps + slot * CT + cl + j, m[j]);
+      }
+      // the round's earlier maps, spread over all threads
+      const ulonglong2* maps = p.maps + (slot - static_cast<int64_t>(idx) * p.tiles) * CT;
+      const int64_t step = static_cast<int64_t>(p.tiles) * CT;
+      constexpr int Q = kThreads / CT;
+      const int cm = tid % CT;
+      for (int i = tid / CT; i < idx; i += 4 * Q) {
         ulonglong2 v[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if (i + u * S < idx) v[u] = look_at_map(maps + (i + u * S) * step);
+          if (i + u * Q < idx) v[u] = look_at_map(maps + (i + u * Q) * step + cm);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if (i + u * S < idx)
-            s_before[i + u * S][cl] = wait_map(maps + (i + u * S) * step, v[u], p.err);
+          if (i + u * Q < idx)
+            s_before[i + u * Q][cm] = wait_map(maps + (i + u * Q) * step + cm, v[u], p.err);
       }
       __syncthreads();
-      if (sub == 0) {
+      if (cs < CT) {
+        double start = 0.0;
         if (rnd > 0)
-          start = wait_state(p.states + ((rnd - 1) * p.tiles + cur.tile) * CT + cl, p.err);
-        else if (!kGrad && p.h0 && cur.c < p.C)
-          start = IO::value(IO::load(p.h0 + cur.c));
-        for (int i = 0; i < idx; ++i) start = apply(s_before[i][cl], start);
-        s_start[cl] = start;
+          start = wait_state(
+              p.states + (static_cast<int64_t>(rnd - 1) * p.tiles + cur.tile) * CT + cs, p.err);
+        else if (!kGrad && p.h0 && channel < p.C)
+          start = IO::value(IO::load(p.h0 + channel));
+        for (int i = 0; i < idx; ++i) start = apply(s_before[i][cs], start);
+        s_start[cs] = start;
         if (!last && ends)
-          put_state(p.states + (rnd * p.tiles + cur.tile) * CT + cl,
-                    apply(s_map[buf][S - 1][cl], start));
+          put_state(p.states + (static_cast<int64_t>(rnd) * p.tiles + cur.tile) * CT + cs,
+                    apply(s_map[buf][S - 1][cs], start));
       }
-    } else if (sub == 0) {
-      if (!kGrad && p.h0 && cur.c < p.C) start = IO::value(IO::load(p.h0 + cur.c));
-      s_start[cl] = start;
+    } else if (cs < CT) {
+      s_start[cs] = !kGrad && p.h0 && channel < p.C ? IO::value(IO::load(p.h0 + channel)) : 0.0;
     }
     __syncthreads();
-    double state = s_start[cl];
-    if (sub > 0) state = apply(s_map[buf][sub - 1][cl], state);
-    const int64_t dir = kGrad ? -p.D : p.D;
+    double state[V];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      state = __fma_rn(IO::value(av[i]), state, IO::value(xv[i]));
-      if (i < cur.n) {
-        const int64_t at = cur.row + i * dir;
-        IO::store(p.out + at, state);
-        if constexpr (kGrad) {
-          IO::store(p.ga + at, __dmul_rn(state, IO::value(hv[i])));
-          if (cur.p0 + i == p.T - 1)
-            IO::store(p.gh0 + cur.c, __dmul_rn(IO::value(IO::load(p.a + cur.base)), state));
-        }
-      }
+    for (int j = 0; j < V; ++j) {
+      state[j] = s_start[cl + j];
+      if (sub > 0) state[j] = apply(s_map[buf][sub - 1][cl + j], state[j]);
     }
+    if (cur.n == R) run_part<true, E, V, R, kGrad>(p, cur, val, state);
+    else if (cur.n > 0) run_part<false, E, V, R, kGrad>(p, cur, val, state);
     __syncthreads();  // s_map, s_before and s_start are written again
     unit = next;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Steps per thread: registers hold two (gradient: three) values of each.
+// Steps per thread of one channel each; half as many of two channels.
+// Registers hold two (gradient: three) values of each.
 #ifndef SEQ_RF
 #define SEQ_RF 16
 #endif
 #ifndef SEQ_RG
-#define SEQ_RG 12
+#define SEQ_RG 10
 #endif
-constexpr int kSteps = SEQ_RF, kStepsGrad = SEQ_RG;
+#ifndef SEQ_RF1
+#define SEQ_RF1 16
+#endif
+#ifndef SEQ_RG1
+#define SEQ_RG1 12
+#endif
+#ifndef SEQ_C64
+#define SEQ_C64 2048
+#endif
+constexpr int steps_of(int type, bool gradient) {
+  return type == 1 ? (gradient ? SEQ_RG1 : SEQ_RF1) : (gradient ? SEQ_RG : SEQ_RF);
+}
+
+// ScanArgs::type of an element type (packed pairs and f64 are alike here).
+template <class E>
+constexpr int type_of() {
+  return sizeof(E) == 4 ? 1 : 0;
+}
 
 // Channels per unit: 64 where there are as many (512 contiguous bytes of f64
 // per step), fewer where a unit would be mostly empty.
 int unit_channels(int64_t C, int64_t T, int steps) {
-  if (C >= 64 || T <= 4 * steps) return 64;
+  if (C >= SEQ_C64 || T <= 4 * steps) return 64;
   return C >= 16 || T <= 16 * steps ? 16 : 4;
 }
 
@@ -454,7 +577,7 @@ Plan plan_of(int64_t B, int64_t T, int64_t D, int steps) {
 
 // Blocks of the kernel resident on the current device (its shared memory
 // limit raised first), once per device.
-template <class E, int CT, int R, bool kGrad>
+template <class E, int V, int CT, int R, bool kGrad>
 int resident_blocks(int* blocks) {
   static std::mutex mu;
   static std::vector<int> by_device;
@@ -463,23 +586,23 @@ int resident_blocks(int* blocks) {
   std::lock_guard<std::mutex> lock(mu);
   if (dev >= static_cast<int>(by_device.size())) by_device.resize(dev + 1, 0);
   if (by_device[dev] == 0) {
-    const int bytes = static_cast<int>(stage_bytes<E, R, kGrad>());
-    DSB_CUDA_TRY(cudaFuncSetAttribute(scan_chunk_kernel<E, CT, R, kGrad>,
+    const int bytes = static_cast<int>(stage_bytes<E, V, R, kGrad>());
+    DSB_CUDA_TRY(cudaFuncSetAttribute(scan_chunk_kernel<E, V, CT, R, kGrad>,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     int n = 0;
     DSB_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-        &n, scan_chunk_kernel<E, CT, R, kGrad>, kThreads, bytes));
+        &n, scan_chunk_kernel<E, V, CT, R, kGrad>, kThreads, bytes));
     by_device[dev] = (n < 1 ? 1 : n) * sm_count();
   }
   *blocks = by_device[dev];
   return DS_OK;
 }
 
-template <class E, int CT, bool kGrad>
+template <class E, int V, int CT, bool kGrad>
 int launch_chunks(const ScanArgs& s, const Plan& g, cudaStream_t st) {
-  constexpr int R = kGrad ? kStepsGrad : kSteps;
+  constexpr int R = steps_of(type_of<E>(), kGrad) / V;
   int resident = 0;
-  if (int rc = resident_blocks<E, CT, R, kGrad>(&resident)) return rc;
+  if (int rc = resident_blocks<E, V, CT, R, kGrad>(&resident)) return rc;
   ChunkArgs<E> p{};
   p.a = static_cast<const E*>(s.a);
   p.x = static_cast<const E*>(s.x);
@@ -488,13 +611,13 @@ int launch_chunks(const ScanArgs& s, const Plan& g, cudaStream_t st) {
   p.out = static_cast<E*>(s.out);
   p.ga = static_cast<E*>(s.grad_a);
   p.gh0 = static_cast<E*>(s.grad_h0);
-  p.C = g.C;
+  p.C = static_cast<uint32_t>(g.C);
   p.T = s.T;
-  p.D = s.D;
-  p.tiles = g.tiles;
-  p.chunks = g.chunks;
-  p.units = g.chunks * g.tiles;
-  p.round = g.round;
+  p.D = static_cast<uint32_t>(s.D);
+  p.tiles = static_cast<uint32_t>(g.tiles);
+  p.chunks = static_cast<uint32_t>(g.chunks);
+  p.units = static_cast<uint32_t>(g.chunks * g.tiles);
+  p.round = static_cast<uint32_t>(g.round);
   if (g.chunks > 1) {
     uint8_t* ws = static_cast<uint8_t*>(s.workspace);
     p.counter = reinterpret_cast<uint32_t*>(ws);
@@ -507,21 +630,35 @@ int launch_chunks(const ScanArgs& s, const Plan& g, cudaStream_t st) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(p.units < resident ? p.units : resident));
+  cfg.gridDim = dim3(p.units < static_cast<uint32_t>(resident) ? p.units : resident);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = stage_bytes<E, R, kGrad>();
+  cfg.dynamicSmemBytes = stage_bytes<E, V, R, kGrad>();
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  DSB_CUDA_TRY(cudaLaunchKernelEx(&cfg, scan_chunk_kernel<E, CT, R, kGrad>, p));
+  DSB_CUDA_TRY(cudaLaunchKernelEx(&cfg, scan_chunk_kernel<E, V, CT, R, kGrad>, p));
   return launch_status();
+}
+
+// Two channels per thread where every row starts on a word of two.
+template <class E>
+bool pairs(const ScanArgs& s) {
+  const size_t w = 2 * sizeof(E);
+  return s.D % 2 == 0 && aligned(s.a, w) && aligned(s.x, w) && aligned(s.h, w) &&
+         aligned(s.h0, w) && aligned(s.out, w) && aligned(s.grad_a, w);
+}
+
+template <class E, int CT, bool kGrad>
+int launch_chunks(const ScanArgs& s, const Plan& g, cudaStream_t st) {
+  return pairs<E>(s) ? launch_chunks<E, 2, CT, kGrad>(s, g, st)
+                     : launch_chunks<E, 1, CT, kGrad>(s, g, st);
 }
 
 template <class E, bool kGrad>
 int launch(const ScanArgs& s, cudaStream_t st) {
-  const Plan g = plan_of(s.B, s.T, s.D, kGrad ? kStepsGrad : kSteps);
+  const Plan g = plan_of(s.B, s.T, s.D, steps_of(type_of<E>(), kGrad));
   const int64_t units = g.ct ? g.chunks * g.tiles : ceil_div(g.C, kThreads);
-  if (units > 0x7fffffff)
+  if (units > 0x7fffffff || g.C > 0x7fffffff)
     return set_error(DS_INVALID_ARGUMENT, "ds_linear_recurrence: too many channels");
   if (g.ct == 64) return launch_chunks<E, 64, kGrad>(s, g, st);
   if (g.ct == 16) return launch_chunks<E, 16, kGrad>(s, g, st);
@@ -547,8 +684,9 @@ int launch(const ScanArgs& s, bool gradient, cudaStream_t st) {
 
 }  // namespace
 
-size_t scan_workspace_bytes(int64_t B, int64_t T, int64_t D) {
-  const size_t f = plan_of(B, T, D, kSteps).total, g = plan_of(B, T, D, kStepsGrad).total;
+size_t scan_workspace_bytes(int type, int64_t B, int64_t T, int64_t D) {
+  const size_t f = plan_of(B, T, D, steps_of(type, false)).total;
+  const size_t g = plan_of(B, T, D, steps_of(type, true)).total;
   return f > g ? f : g;
 }
 
