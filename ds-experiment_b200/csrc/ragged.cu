@@ -1,18 +1,26 @@
 // Products grouped by expert: rows of consecutive groups times their group's
 // matrix, and the contraction over each group's rows.
+//
+// Groups are sorted by their number of rows, on the device (prep_kernel): a
+// group of at least kTensorRows rows goes to the tensor-core product
+// (ragged_ozaki.cu), the others are multiplied here with FP64 matrix
+// instructions.  One launch serves all of a call's small groups.
+//
+// Bound: HBM while a group has few rows (each matrix is read once, 8 bytes a
+// value, for 2 rows operations), the FP64 pipe (64 FMA per clock and SM) above
+// about 20 rows.
+#include <mutex>
 #include <string>
+#include <vector>
 
 #include "common.cuh"
 #include "ds_arith.cuh"
 #include "kernels.h"
 #include "profile.h"
+#include "ragged.h"
 
 namespace dsb {
 namespace {
-
-__device__ __forceinline__ double value_at(const DotOperand& o, int64_t i) {
-  return o.f64 ? o.f64[i] : to_f64(ds2{o.hi[i], o.lo[i]});
-}
 
 __device__ __forceinline__ void put(const DotResult& c, int64_t i, double v) {
   if (c.f64) {
@@ -24,109 +32,578 @@ __device__ __forceinline__ void put(const DotResult& c, int64_t i, double v) {
   }
 }
 
-// Exclusive ends of the groups: offsets[g] = first row of group g,
-// offsets[G] = first row behind the last one.  A negative size counts as 0
-// and no group passes row M.
-__global__ void __launch_bounds__(32)
-offsets_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M,
-               int32_t* __restrict__ offsets) {
-  wait_previous_grid();
-  if (threadIdx.x != 0) return;
-  int64_t at = 0;
-  for (int64_t g = 0; g < G; ++g) {
-    offsets[g] = static_cast<int32_t>(at);
-    at += sizes[g] > 0 ? sizes[g] : 0;
-    if (at > M) at = M;
+// ---- the groups' rows and tiles ------------------------------------------------
+
+constexpr int kPrepThreads = 1024;
+
+// Exclusive sum over the block, and the block's total.
+__device__ int64_t block_scan(int64_t v, int64_t& total) {
+  __shared__ int64_t s_warp[kPrepThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
   }
-  offsets[G] = static_cast<int32_t>(at);
+  if (lane == 31) s_warp[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t w = s_warp[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, w, d);
+      if (lane >= d) w += y;
+    }
+    s_warp[lane] = w;
+  }
+  __syncthreads();
+  const int64_t before = (warp > 0 ? s_warp[warp - 1] : 0) + x - v;
+  total = s_warp[kPrepThreads / 32 - 1];
+  __syncthreads();
+  return before;
 }
 
-// The group of row `row`: the last g with offsets[g] <= row, or G behind them.
-__device__ __forceinline__ int64_t group_of(const int32_t* offsets, int64_t G, int64_t row) {
-  if (row >= offsets[G]) return G;
-  int64_t lo = 0, hi = G;  // offsets[lo] <= row < offsets[hi]
+// start[g] <= t < start[g + 1] for t in [0, start[G]).
+__device__ __forceinline__ int64_t owner_of(const int32_t* start, int64_t G, int32_t t) {
+  int64_t lo = 0, hi = G;
   while (hi - lo > 1) {
     const int64_t mid = (lo + hi) >> 1;
-    if (offsets[mid] <= row) lo = mid;
+    if (start[mid] <= t) lo = mid;
     else hi = mid;
   }
   return lo;
 }
 
-constexpr int kThreads = 128;
-
-__global__ void __launch_bounds__(kThreads)
-ragged_dot_kernel(RaggedProblem p, const int32_t* __restrict__ offsets) {
+// One block: the groups' first rows inside [begin, end) of the call's rows (a
+// negative size counts as 0, no group passes row M), and the tiles of the two
+// kinds of groups.
+__global__ void __launch_bounds__(kPrepThreads)
+prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t begin, int64_t end,
+            RaggedPlan p) {
   wait_previous_grid();
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (j >= p.N) return;
-  for (int64_t i = blockIdx.y; i < p.M; i += gridDim.y) {
-    const int64_t g = group_of(offsets, p.G, i);
-    double s = 0.0;
-    if (g < p.G)
-      for (int64_t k = 0; k < p.K; ++k)
-        s = __fma_rn(value_at(p.lhs, i * p.lhs.s_r + k * p.lhs.s_k),
-                     value_at(p.rhs, g * p.rhs.s_b + j * p.rhs.s_r + k * p.rhs.s_k), s);
-    put(p.out, i * p.N + j, s);
+  const int64_t tid = threadIdx.x;
+  for (int64_t i = tid; i < p.counters; i += kPrepThreads) p.counter[i] = 0;
+  int64_t rows_before = 0, tiles_before = 0;
+  for (int64_t g0 = 0; g0 < G; g0 += kPrepThreads) {
+    const int64_t g = g0 + tid;
+    const int64_t n = g < G && sizes[g] > 0 ? sizes[g] : 0;
+    int64_t sum, tsum;
+    int64_t lo = rows_before + block_scan(n, sum), hi = lo + n;
+    rows_before += sum;
+    // the group's rows inside the call's window
+    auto clip = [&](int64_t r) {
+      r = r < M ? r : M;
+      return r < begin ? begin : r > end ? end : r;
+    };
+    lo = clip(lo);
+    hi = clip(hi);
+    const int64_t rows = hi - lo;
+    const bool tensor = rows >= p.tensor_rows;
+    const int64_t d = tensor ? 0 : (rows + kSmallTile - 1) / kSmallTile;
+    const int64_t t = tensor ? (rows + kTensorTile - 1) / kTensorTile : 0;
+    // both counts stay below 2^31
+    const int64_t both = tiles_before + block_scan(d << 32 | t, tsum);
+    tiles_before += tsum;
+    if (g < G) {
+      p.row[g] = static_cast<int32_t>(lo);
+      p.small_start[g] = static_cast<int32_t>(both >> 32);
+      p.tensor_start[g] = static_cast<int32_t>(both & 0xffffffff);
+      if (g == G - 1) {
+        p.row[G] = static_cast<int32_t>(hi);
+        p.small_start[G] = static_cast<int32_t>((both >> 32) + d);
+        p.tensor_start[G] = static_cast<int32_t>((both & 0xffffffff) + t);
+      }
+    }
+  }
+  if (G == 0 && tid == 0) p.row[0] = p.small_start[0] = p.tensor_start[0] = 0;
+  __syncthreads();
+  auto fill = [&](const int32_t* start, int tile, RaggedTile* out, int64_t cap) {
+    const int64_t n = start[G] < cap ? start[G] : cap;
+    for (int64_t t = tid; t < n; t += kPrepThreads) {
+      const int64_t g = owner_of(start, G, static_cast<int32_t>(t));
+      const int32_t row = p.row[g] + static_cast<int32_t>(t - start[g]) * tile;
+      const int32_t left = p.row[g + 1] - row;
+      out[t] = RaggedTile{static_cast<int32_t>(g), row, left < tile ? left : tile, 0};
+    }
+  };
+  if (p.small) fill(p.small_start, kSmallTile, p.small, p.small_cap);
+  if (p.tensor) fill(p.tensor_start, kTensorTile, p.tensor, p.tensor_cap);
+}
+
+// ---- small groups: FP64 matrix instructions ---------------------------------------
+
+constexpr int kThreads = 256;
+constexpr int kTN = 64;      // columns of a tile
+constexpr int kKS = 32;      // contraction per pipeline stage
+constexpr int kStages = 3;
+// Row pitches of the staged tiles, in values: 4 (mod 16) puts the 4 x 4
+// values that half a warp reads for a fragment in 16 different 8-byte banks.
+constexpr int kPitchK = kKS + 4;       // [row or column][k]
+constexpr int kPitchN = kSmallTile + 4;  // [k][row or column]
+constexpr int kOperand = kSmallTile * kPitchK > kKS * kPitchN ? kSmallTile * kPitchK : kKS * kPitchN;
+constexpr size_t kSmallBytes = sizeof(double) * 2 * kStages * kOperand;
+static_assert(kTN == kSmallTile, "A and B are staged alike");
+
+__device__ __forceinline__ void copy_async(void* dst, const void* src, int bytes, bool valid) {
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  const int n = valid ? bytes : 0;
+  if (bytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(src), "r"(n)
+                 : "memory");
+  else if (bytes == 8)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(src), "r"(n)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(src), "r"(n)
+                 : "memory");
+}
+
+// d += a b for an 8 x 4 and a 4 x 8 fragment: lane l holds a[l / 4][l % 4],
+// b[l % 4][l / 4] and d[l / 4][2 (l % 4) + {0, 1}].
+__device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
+  asm volatile(
+      "mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+      : "+d"(d[0]), "+d"(d[1])
+      : "d"(a), "d"(b));
+}
+
+// A staged operand: f64 values, or (kPair) the hi words and behind them the
+// lo words.
+template <bool kPair>
+__device__ __forceinline__ double staged(const double* tile, int at) {
+  if constexpr (kPair) {
+    const float* f = reinterpret_cast<const float*>(tile);
+    return __dadd_rn(static_cast<double>(f[at]), static_cast<double>(f[kOperand + at]));
+  } else {
+    return tile[at];
   }
 }
 
-__global__ void __launch_bounds__(kThreads)
-ragged_contract_kernel(RaggedProblem p, const int32_t* __restrict__ offsets) {
-  wait_previous_grid();
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (j >= p.N) return;
-  for (int64_t r = blockIdx.y; r < p.G * p.K; r += gridDim.y) {
-    const int64_t g = r / p.K, i = r - g * p.K;
-    double s = 0.0;
-    for (int64_t t = offsets[g]; t < offsets[g + 1]; ++t)
-      s = __fma_rn(value_at(p.lhs, i * p.lhs.s_r + t * p.lhs.s_k),
-                   value_at(p.rhs, j * p.rhs.s_r + t * p.rhs.s_k), s);
-    put(p.out, r * p.N + j, s);
+// One operand's part of a unit: `lines` lines of `len` consecutive values,
+// line t at offset origin + t stride of the operand.
+struct Block2d {
+  int64_t origin, stride;
+  int lines, len;
+};
+
+// `lines_pad` x `len_pad` values of the block into a staged tile (pitch values
+// per line), zeros outside it; `vec` values per copy.
+template <bool kPair>
+__device__ __forceinline__ void stage_block(const DotOperand& o, const Block2d& b, int lines_pad,
+                                            int len_pad, double* tile, int pitch, int vec) {
+  constexpr int kElem = kPair ? 4 : 8;
+  const int per_line = len_pad / vec;
+  for (int e = threadIdx.x; e < lines_pad * per_line; e += kThreads) {
+    const int line = e / per_line, at = (e - line * per_line) * vec;
+    const bool in = line < b.lines && at < b.len;  // vec divides len
+    const int64_t src = in ? b.origin + line * b.stride + at : 0;
+    if constexpr (kPair) {
+      float* f = reinterpret_cast<float*>(tile) + line * pitch + at;
+      copy_async(f, o.hi + src, kElem * vec, in);
+      copy_async(f + kOperand, o.lo + src, kElem * vec, in);
+    } else {
+      copy_async(tile + line * pitch + at, o.f64 + src, kElem * vec, in);
+    }
   }
 }
 
-size_t offsets_bytes(int64_t G) { return (static_cast<size_t>(G + 1) * 4 + 255) / 256 * 256; }
+struct SmallArgs {
+  RaggedProblem q;
+  RaggedPlan p;
+  bool contract;
+  bool add;        // contraction: add to the result (a later window of rows)
+  int tiles_k;     // contraction: tiles of the result's rows
+  int tiles_n;
+  int splits;      // of the contraction (products only)
+  int64_t split_k;
+  double* partial;  // [splits][M][N]
+  int vec_a, vec_b;  // values per copy
+};
 
-int launch_offsets(const RaggedProblem& p, int32_t* offsets, cudaStream_t s) {
-  DSB_CUDA_TRY(launch_dependent(offsets_kernel, dim3(1), dim3(32), s, p.group_sizes, p.G, p.M,
-                                offsets));
-  return DS_OK;
+// A unit of work: an output tile over a range of the contraction.
+struct SmallUnit {
+  int64_t g, row, col;  // group, first output row (in the group's rows or matrix) and column
+  int rows, cols;
+  int64_t k0, k1;       // contraction range (contraction: rows of the call)
+  int split;
+  int64_t id;           // of its output tile
+};
+
+__device__ __forceinline__ int64_t units_of(const SmallArgs& a) {
+  if (a.contract) return a.q.G * a.tiles_k * a.tiles_n;
+  return static_cast<int64_t>(a.p.small_start[a.q.G]) * a.tiles_n * a.splits;
 }
 
-dim3 row_grid(int64_t N, int64_t rows) {
-  return dim3(static_cast<unsigned>((N + kThreads - 1) / kThreads),
-              static_cast<unsigned>(rows < 65535 ? rows : 65535));
+// False for a unit that belongs to the tensor-core product, or that adds
+// nothing.
+__device__ __forceinline__ bool unit_at(const SmallArgs& a, int64_t u, SmallUnit& x) {
+  if (a.contract) {
+    const int64_t per = static_cast<int64_t>(a.tiles_k) * a.tiles_n;
+    x.g = u / per;
+    const int64_t r = u - x.g * per;
+    x.row = r / a.tiles_n * kSmallTile;
+    x.col = r % a.tiles_n * kTN;
+    x.k0 = a.p.row[x.g];
+    x.k1 = a.p.row[x.g + 1];
+    x.rows = a.q.K - x.row < kSmallTile ? static_cast<int>(a.q.K - x.row) : kSmallTile;
+    x.split = 0;
+    x.id = u;
+    if (x.k1 - x.k0 >= a.p.tensor_rows || (a.add && x.k1 == x.k0)) return false;
+  } else {
+    const int64_t n = a.p.small_start[a.q.G];
+    const int64_t rest = u / n;
+    const RaggedTile t = a.p.small[u - rest * n];
+    x.g = t.group;
+    x.row = t.row;
+    x.rows = t.rows;
+    x.split = static_cast<int>(rest % a.splits);
+    const int64_t tn = rest / a.splits;
+    x.col = tn * kTN;
+    x.k0 = x.split * a.split_k;
+    x.k1 = x.k0 + a.split_k < a.q.K ? x.k0 + a.split_k : a.q.K;
+    x.id = tn * n + (u - rest * n);
+  }
+  x.cols = a.q.N - x.col < kTN ? static_cast<int>(a.q.N - x.col) : kTN;
+  return true;
+}
+
+// kA: A is staged as [k][row] (its rows are contiguous) rather than [row][k];
+// kB: B as [k][column] rather than [column][k].
+template <bool kPair, bool kA, bool kB>
+__device__ __forceinline__ void stage_unit(const SmallArgs& a, const SmallUnit& x, int64_t k,
+                                           double* sa, double* sb) {
+  const int kn = x.k1 - k < kKS ? static_cast<int>(x.k1 - k) : kKS;
+  const RaggedProblem& q = a.q;
+  const int rows_pad = x.rows <= 16 ? 16 : kSmallTile;
+  Block2d A, B;
+  if constexpr (kA) {
+    A = Block2d{x.row + k * q.lhs.s_k, q.lhs.s_k, kn, x.rows};
+    stage_block<kPair>(q.lhs, A, kKS, rows_pad, sa, kPitchN, a.vec_a);
+  } else {
+    A = Block2d{x.row * q.lhs.s_r + k, q.lhs.s_r, x.rows, kn};
+    stage_block<kPair>(q.lhs, A, rows_pad, kKS, sa, kPitchK, a.vec_a);
+  }
+  const int64_t base = a.contract ? 0 : x.g * q.rhs.s_b;
+  if constexpr (kB) {
+    B = Block2d{base + k * q.rhs.s_k + x.col, q.rhs.s_k, kn, x.cols};
+    stage_block<kPair>(q.rhs, B, kKS, kTN, sb, kPitchN, a.vec_b);
+  } else {
+    B = Block2d{base + x.col * q.rhs.s_r + k, q.rhs.s_r, x.cols, kn};
+    stage_block<kPair>(q.rhs, B, kTN, kKS, sb, kPitchK, a.vec_b);
+  }
+}
+
+// The products of one stage: warps stand kWM x (8 / kWM), each with MF x NF
+// fragments.
+template <bool kPair, bool kA, bool kB, int MF, int NF, int kWM>
+__device__ __forceinline__ void multiply_stage(const double* sa, const double* sb, int kn,
+                                               double (&acc)[4][2][2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int wm = warp % kWM * MF * 8, wn = warp / kWM * NF * 8;
+  const int r = lane >> 2, kk = lane & 3;
+#pragma unroll 4
+  for (int k = 0; k < kn; k += 4) {
+    double fa[MF], fb[NF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+      fa[i] = staged<kPair>(sa, kA ? (k + kk) * kPitchN + wm + i * 8 + r
+                                   : (wm + i * 8 + r) * kPitchK + k + kk);
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+      fb[j] = staged<kPair>(sb, kB ? (k + kk) * kPitchN + wn + j * 8 + r
+                                   : (wn + j * 8 + r) * kPitchK + k + kk);
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) mma_f64(acc[i][j], fa[i], fb[j]);
+  }
+}
+
+template <int MF, int NF, int kWM>
+__device__ __forceinline__ void store_unit(const SmallArgs& a, const SmallUnit& x,
+                                           const double (&acc)[4][2][2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int wm = warp % kWM * MF * 8, wn = warp / kWM * NF * 8;
+  const int64_t first = (a.contract ? x.g * a.q.K : 0) + x.row;
+#pragma unroll
+  for (int i = 0; i < MF; ++i) {
+    const int r = wm + i * 8 + (lane >> 2);
+    if (r >= x.rows) continue;
+    const int64_t row = (first + r) * a.q.N + x.col;
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = wn + j * 8 + 2 * (lane & 3) + h;
+        if (c >= x.cols) continue;
+        double v = acc[i][j][h];
+        if (a.splits > 1) {
+          a.partial[static_cast<int64_t>(x.split) * a.q.M * a.q.N + row + c] = v;
+          continue;
+        }
+        if (a.add) v = __dadd_rn(result_value(a.q.out, row + c), v);
+        put(a.q.out, row + c, v);
+      }
+    }
+  }
+}
+
+// Blocks stay and take every gridDim.x-th unit; the pipeline of stages runs on
+// across units.
+template <bool kPair, bool kA, bool kB>
+__global__ void __launch_bounds__(kThreads, 2)
+small_kernel(const __grid_constant__ SmallArgs a) {
+  extern __shared__ __align__(16) double stage[];
+  __shared__ int s_last;
+  wait_previous_grid();
+  // rows behind the last group
+  if (!a.contract) {
+    const int64_t end = a.q.M * a.q.N;
+    for (int64_t i = a.p.row[a.q.G] * a.q.N + static_cast<int64_t>(blockIdx.x) * kThreads +
+                     threadIdx.x;
+         i < end; i += static_cast<int64_t>(gridDim.x) * kThreads)
+      put(a.q.out, i, 0.0);
+  }
+  const int64_t units = units_of(a);
+  auto next_unit = [&](int64_t u, SmallUnit& x) {
+    while (u < units && !unit_at(a, u, x)) u += gridDim.x;
+    return u;
+  };
+  // loading runs kStages - 1 stages ahead of multiplying
+  SmallUnit lx, x;
+  int64_t lu = next_unit(blockIdx.x, lx);
+  int64_t lk = lu < units ? lx.k0 : 0;
+  int ls = 0;
+  auto load_one = [&] {
+    if (lu < units) {
+      double* sa = stage + ls * 2 * kOperand;
+      if (lk < lx.k1) stage_unit<kPair, kA, kB>(a, lx, lk, sa, sa + kOperand);
+      lk += kKS;
+      if (lk >= lx.k1) {
+        lu = next_unit(lu + gridDim.x, lx);
+        if (lu < units) lk = lx.k0;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    ls = ls + 1 == kStages ? 0 : ls + 1;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) load_one();
+  int cs = 0;
+#pragma unroll 1
+  for (int64_t u = next_unit(blockIdx.x, x); u < units; u = next_unit(u + gridDim.x, x)) {
+    double acc[4][2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j][0] = acc[i][j][1] = 0.0;
+    int64_t k = x.k0;
+    do {  // a unit without contraction takes one (empty) stage
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncthreads();
+      const double* sa = stage + cs * 2 * kOperand;
+      const int kn = x.k1 - k < kKS ? static_cast<int>(x.k1 - k) : kKS;
+      load_one();
+      if (x.rows <= 16) multiply_stage<kPair, kA, kB, 2, 1, 1>(sa, sa + kOperand, kn, acc);
+      else multiply_stage<kPair, kA, kB, 4, 2, 2>(sa, sa + kOperand, kn, acc);
+      cs = cs + 1 == kStages ? 0 : cs + 1;
+      k += kKS;
+    } while (k < x.k1);
+    if (x.rows <= 16) store_unit<2, 1, 1>(a, x, acc);
+    else store_unit<4, 2, 2>(a, x, acc);
+    if (a.splits > 1) {
+      // the last of a tile's splits adds them up in order
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) s_last = atomicAdd(a.p.counter + x.id, 1) == a.splits - 1;
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        for (int e = threadIdx.x; e < x.rows * x.cols; e += kThreads) {
+          const int64_t at = (x.row + e / x.cols) * a.q.N + x.col + e % x.cols;
+          double v = 0.0;
+          for (int s = 0; s < a.splits; ++s)
+            v = __dadd_rn(v, __ldcg(a.partial + static_cast<int64_t>(s) * a.q.M * a.q.N + at));
+          put(a.q.out, at, v);
+        }
+      }
+      __syncthreads();
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// ---- host ------------------------------------------------------------------------
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Contraction splits of the products: enough units for about four per
+// resident block when the rows are few, each of at least kSplitMin.  From the
+// call's sizes alone, so a row's rounding does not depend on other groups.
+constexpr int64_t kSplitMin = 128;
+constexpr int kMaxSplits = 16;
+
+int splits_of(int64_t M, int64_t K, int64_t N, int64_t G) {
+  const int64_t tiles = (M / kSmallTile + (G < M ? G : M)) * ceil_div(N, kTN);
+  int64_t s = tiles > 0 ? ceil_div(1184, tiles) : 1;
+  const int64_t most = K / kSplitMin;
+  s = s > most ? most : s;
+  s = s > kMaxSplits ? kMaxSplits : s;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+// Whether the tensor-core product takes groups of many rows.
+bool tensor_allowed(int64_t M, int64_t K, int64_t N) { return false; }
+
+struct Workspace {
+  size_t at = 0;
+  size_t take(size_t bytes) {
+    const size_t here = at;
+    at = (at + bytes + 255) / 256 * 256;
+    return here;
+  }
+};
+
+struct SmallLayout {
+  size_t row, small_start, tensor_start, small, tensor, counter, partial, total;
+  int64_t small_cap, tensor_cap, counters;
+  int splits;
+};
+
+SmallLayout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
+  SmallLayout l{};
+  Workspace w;
+  const int64_t groups = G < M ? G : M;  // with rows
+  l.small_cap = contract ? 0 : M / kSmallTile + groups;
+  const int64_t big = M / kTensorRows;
+  l.tensor_cap = tensor_allowed(M, K, N) ? M / kTensorTile + (groups < big ? groups : big) : 0;
+  l.splits = contract ? 1 : splits_of(M, K, N, G);
+  l.counters = l.splits > 1 ? l.small_cap * ceil_div(N, kTN) : 0;
+  l.row = w.take((G + 1) * 4);
+  l.small_start = w.take((G + 1) * 4);
+  l.tensor_start = w.take((G + 1) * 4);
+  l.small = w.take(l.small_cap * sizeof(RaggedTile));
+  l.tensor = w.take(l.tensor_cap * sizeof(RaggedTile));
+  l.counter = w.take(l.counters * 4);
+  l.partial = w.take(l.splits > 1 ? static_cast<size_t>(l.splits) * M * N * 8 : 0);
+  l.total = w.at;
+  return l;
+}
+
+RaggedPlan plan_at(const SmallLayout& l, void* workspace, bool tensor) {
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  RaggedPlan p{};
+  p.row = reinterpret_cast<int32_t*>(ws + l.row);
+  p.small_start = reinterpret_cast<int32_t*>(ws + l.small_start);
+  p.tensor_start = reinterpret_cast<int32_t*>(ws + l.tensor_start);
+  p.small = l.small_cap ? reinterpret_cast<RaggedTile*>(ws + l.small) : nullptr;
+  p.tensor = l.tensor_cap ? reinterpret_cast<RaggedTile*>(ws + l.tensor) : nullptr;
+  p.small_cap = l.small_cap;
+  p.tensor_cap = l.tensor_cap;
+  p.counter = reinterpret_cast<int32_t*>(ws + l.counter);
+  p.counters = l.counters;
+  p.tensor_rows = tensor ? kTensorRows : INT32_MAX;
+  return p;
+}
+
+// Values per copy of an operand whose lines are `len` values long at a stride
+// of `stride` values, from `origin` on.
+int copy_width(const DotOperand& o, int64_t len, int64_t stride, int64_t batch) {
+  const int wide = o.f64 ? 2 : 4;
+  const bool at = o.f64 ? aligned(o.f64, 16) : aligned(o.hi, 16) && aligned(o.lo, 16);
+  return at && len % wide == 0 && stride % wide == 0 && batch % wide == 0 ? wide : 1;
+}
+
+template <bool kPair, bool kA, bool kB>
+int launch_small(const SmallArgs& a, int64_t most_units, cudaStream_t s) {
+  static std::mutex mu;
+  static std::vector<bool> done;
+  int dev = 0;
+  DSB_CUDA_TRY(cudaGetDevice(&dev));
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= static_cast<int>(done.size())) done.resize(dev + 1, false);
+    if (!done[dev]) {
+      DSB_CUDA_TRY(cudaFuncSetAttribute(small_kernel<kPair, kA, kB>,
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        static_cast<int>(kSmallBytes)));
+      done[dev] = true;
+    }
+  }
+  const int64_t resident = 2 * static_cast<int64_t>(sm_count());
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(most_units < resident ? (most_units < 1 ? 1 : most_units)
+                                                                 : resident));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmallBytes;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  DSB_CUDA_TRY(cudaLaunchKernelEx(&cfg, small_kernel<kPair, kA, kB>, a));
+  return launch_status();
+}
+
+int launch_prep(const RaggedProblem& q, int64_t begin, int64_t end, const RaggedPlan& p,
+                cudaStream_t s) {
+  DSB_CUDA_TRY(launch_dependent(prep_kernel, dim3(1), dim3(kPrepThreads), s, q.group_sizes, q.G,
+                                q.M, begin, end, p));
+  return launch_status();
 }
 
 }  // namespace
 
-size_t ragged_dot_workspace_bytes(int64_t, int64_t, int64_t, int64_t G, bool) {
-  return offsets_bytes(G);
+size_t ragged_dot_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, bool) {
+  return layout_of(M, K, N, G, false).total;
 }
 
-int ragged_dot(const RaggedProblem& p, void* workspace, size_t, cudaStream_t s) {
-  if (p.M == 0 || p.N == 0) return ok();
-  int32_t* offsets = static_cast<int32_t*>(workspace);
+int ragged_dot(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) {
+  if (q.M == 0 || q.N == 0) return ok();
   ProfileScope prof("ragged_dot", s);
-  if (int st = launch_offsets(p, offsets, s)) return st;
-  DSB_CUDA_TRY(launch_dependent(ragged_dot_kernel, row_grid(p.N, p.M), dim3(kThreads), s, p,
-                                offsets));
-  return launch_status();
+  const SmallLayout l = layout_of(q.M, q.K, q.N, q.G, false);
+  SmallArgs a{};
+  a.q = q;
+  a.p = plan_at(l, workspace, false);
+  a.tiles_n = static_cast<int>(ceil_div(q.N, kTN));
+  a.splits = l.splits;
+  a.split_k = ceil_div(ceil_div(q.K, a.splits), kKS) * kKS;
+  a.partial = reinterpret_cast<double*>(static_cast<uint8_t*>(workspace) + l.partial);
+  a.vec_a = copy_width(q.lhs, q.K, q.lhs.s_r, 0);
+  a.vec_b = copy_width(q.rhs, q.rhs_t ? q.K : q.N, q.rhs_t ? q.rhs.s_r : q.rhs.s_k, q.rhs.s_b);
+  if (int st = launch_prep(q, 0, q.M, a.p, s)) return st;
+  const int64_t units = l.small_cap * a.tiles_n * a.splits;
+  const bool pair = q.lhs.f64 == nullptr;
+  if (q.rhs_t)
+    return pair ? launch_small<true, false, false>(a, units, s)
+                : launch_small<false, false, false>(a, units, s);
+  return pair ? launch_small<true, false, true>(a, units, s)
+              : launch_small<false, false, true>(a, units, s);
 }
 
-size_t ragged_contract_workspace_bytes(int64_t, int64_t, int64_t, int64_t G) {
-  return offsets_bytes(G);
+size_t ragged_contract_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G) {
+  return layout_of(M, K, N, G, true).total;
 }
 
-int ragged_contract(const RaggedProblem& p, void* workspace, size_t, cudaStream_t s) {
-  if (p.G == 0 || p.K == 0 || p.N == 0) return ok();
-  int32_t* offsets = static_cast<int32_t*>(workspace);
+int ragged_contract(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) {
+  if (q.G == 0 || q.K == 0 || q.N == 0) return ok();
   ProfileScope prof("ragged_dot_contract", s);
-  if (int st = launch_offsets(p, offsets, s)) return st;
-  DSB_CUDA_TRY(launch_dependent(ragged_contract_kernel, row_grid(p.N, p.G * p.K), dim3(kThreads),
-                                s, p, offsets));
-  return launch_status();
+  const SmallLayout l = layout_of(q.M, q.K, q.N, q.G, true);
+  SmallArgs a{};
+  a.q = q;
+  a.p = plan_at(l, workspace, false);
+  a.contract = true;
+  a.tiles_k = static_cast<int>(ceil_div(q.K, kSmallTile));
+  a.tiles_n = static_cast<int>(ceil_div(q.N, kTN));
+  a.splits = 1;
+  a.vec_a = copy_width(q.lhs, q.K, q.lhs.s_k, 0);
+  a.vec_b = copy_width(q.rhs, q.N, q.rhs.s_k, 0);
+  if (int st = launch_prep(q, 0, q.M, a.p, s)) return st;
+  const int64_t units = q.G * a.tiles_k * a.tiles_n;
+  return q.lhs.f64 == nullptr ? launch_small<true, true, true>(a, units, s)
+                              : launch_small<false, true, true>(a, units, s);
 }
 
 }  // namespace dsb
