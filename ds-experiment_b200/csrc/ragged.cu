@@ -9,6 +9,7 @@
 // Bound: HBM while a group has few rows (each matrix is read once, 8 bytes a
 // value, for 2 rows operations), the FP64 pipe (64 FMA per clock and SM) above
 // about 20 rows.
+#include <climits>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -84,11 +85,11 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
   wait_previous_grid();
   const int64_t tid = threadIdx.x;
   for (int64_t i = tid; i < p.counters; i += kPrepThreads) p.counter[i] = 0;
-  int64_t rows_before = 0, tiles_before = 0;
+  int64_t rows_before = 0, tiles_before = 0, slots_before = 0;
   for (int64_t g0 = 0; g0 < G; g0 += kPrepThreads) {
     const int64_t g = g0 + tid;
     const int64_t n = g < G && sizes[g] > 0 ? sizes[g] : 0;
-    int64_t sum, tsum;
+    int64_t sum, tsum, ssum;
     int64_t lo = rows_before + block_scan(n, sum), hi = lo + n;
     rows_before += sum;
     // the group's rows inside the call's window
@@ -105,18 +106,28 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
     // both counts stay below 2^31
     const int64_t both = tiles_before + block_scan(d << 32 | t, tsum);
     tiles_before += tsum;
+    const int64_t slot = slots_before + block_scan(tensor, ssum);
+    slots_before += ssum;
     if (g < G) {
       p.row[g] = static_cast<int32_t>(lo);
       p.small_start[g] = static_cast<int32_t>(both >> 32);
       p.tensor_start[g] = static_cast<int32_t>(both & 0xffffffff);
+      p.slot[g] = static_cast<int32_t>(slot);
+      if (tensor) {
+        int bits = 50;
+        for (int i = 0; i < kBitsLimits && rows > p.bits_limit[i]; ++i) --bits;
+        p.slot_group[slot] = static_cast<int32_t>(g);
+        p.slot_bits[slot] = bits;
+      }
       if (g == G - 1) {
         p.row[G] = static_cast<int32_t>(hi);
         p.small_start[G] = static_cast<int32_t>((both >> 32) + d);
         p.tensor_start[G] = static_cast<int32_t>((both & 0xffffffff) + t);
+        p.slot[G] = static_cast<int32_t>(slot + tensor);
       }
     }
   }
-  if (G == 0 && tid == 0) p.row[0] = p.small_start[0] = p.tensor_start[0] = 0;
+  if (G == 0 && tid == 0) p.row[0] = p.small_start[0] = p.tensor_start[0] = p.slot[0] = 0;
   __syncthreads();
   auto fill = [&](const int32_t* start, int tile, RaggedTile* out, int64_t cap) {
     const int64_t n = start[G] < cap ? start[G] : cap;
@@ -124,7 +135,7 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
       const int64_t g = owner_of(start, G, static_cast<int32_t>(t));
       const int32_t row = p.row[g] + static_cast<int32_t>(t - start[g]) * tile;
       const int32_t left = p.row[g + 1] - row;
-      out[t] = RaggedTile{static_cast<int32_t>(g), row, left < tile ? left : tile, 0};
+      out[t] = RaggedTile{static_cast<int32_t>(g), row, left < tile ? left : tile, p.slot[g]};
     }
   };
   if (p.small) fill(p.small_start, kSmallTile, p.small, p.small_cap);
@@ -453,57 +464,96 @@ int splits_of(int64_t M, int64_t K, int64_t N, int64_t G) {
   return s < 1 ? 1 : static_cast<int>(s);
 }
 
-// Whether the tensor-core product takes groups of many rows.
-bool tensor_allowed(int64_t M, int64_t K, int64_t N) { return false; }
+// Whether the tensor-core product takes groups of many rows: its tiles are
+// padded to 256 columns and 128 of the contraction.
+bool tensor_allowed(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
+  return M >= kTensorRows && (contract ? K >= 128 : K >= 64) && N >= 128 &&
+         ragged_tensor_fits(M, K, N, G, contract);
+}
 
-struct Workspace {
-  size_t at = 0;
-  size_t take(size_t bytes) {
-    const size_t here = at;
-    at = (at + bytes + 255) / 256 * 256;
-    return here;
-  }
-};
-
-struct SmallLayout {
-  size_t row, small_start, tensor_start, small, tensor, counter, partial, total;
-  int64_t small_cap, tensor_cap, counters;
+struct Layout {
+  size_t row, small_start, tensor_start, slot, small, tensor, slot_group, slot_bits, counter,
+      partial, tensor_ws, total;
+  int64_t small_cap, tensor_cap, slots, counters;
   int splits;
+  bool tensor_ok;
 };
 
-SmallLayout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
-  SmallLayout l{};
-  Workspace w;
+Layout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
+  Layout l{};
+  size_t at = 0;
+  auto take = [&at](size_t bytes) {
+    const size_t here = at;
+    at = (at + bytes + 1023) / 1024 * 1024;
+    return here;
+  };
   const int64_t groups = G < M ? G : M;  // with rows
+  l.tensor_ok = tensor_allowed(M, K, N, G, contract);
   l.small_cap = contract ? 0 : M / kSmallTile + groups;
-  const int64_t big = M / kTensorRows;
-  l.tensor_cap = tensor_allowed(M, K, N) ? M / kTensorTile + (groups < big ? groups : big) : 0;
+  if (l.tensor_ok) {
+    const int64_t rows = contract && M > kRaggedWindow ? kRaggedWindow : M;
+    l.slots = ragged_slots(rows, G);
+    l.tensor_cap = ragged_tensor_tiles(rows, G);
+  }
   l.splits = contract ? 1 : splits_of(M, K, N, G);
   l.counters = l.splits > 1 ? l.small_cap * ceil_div(N, kTN) : 0;
-  l.row = w.take((G + 1) * 4);
-  l.small_start = w.take((G + 1) * 4);
-  l.tensor_start = w.take((G + 1) * 4);
-  l.small = w.take(l.small_cap * sizeof(RaggedTile));
-  l.tensor = w.take(l.tensor_cap * sizeof(RaggedTile));
-  l.counter = w.take(l.counters * 4);
-  l.partial = w.take(l.splits > 1 ? static_cast<size_t>(l.splits) * M * N * 8 : 0);
-  l.total = w.at;
+  l.row = take((G + 1) * 4);
+  l.small_start = take((G + 1) * 4);
+  l.tensor_start = take((G + 1) * 4);
+  l.slot = take((G + 1) * 4);
+  l.small = take(l.small_cap * sizeof(RaggedTile));
+  l.tensor = take(l.tensor_cap * sizeof(RaggedTile));
+  l.slot_group = take(l.slots * 4);
+  l.slot_bits = take(l.slots * 4);
+  l.counter = take(l.counters * 4);
+  l.partial = take(l.splits > 1 ? static_cast<size_t>(l.splits) * M * N * 8 : 0);
+  l.tensor_ws = take(l.tensor_ok ? ragged_tensor_bytes(M, K, N, G, contract) : 0);
+  // the tensor-core part is aligned to 1024 whatever the workspace's start
+  l.total = at + 1024;
   return l;
 }
 
-RaggedPlan plan_at(const SmallLayout& l, void* workspace, bool tensor) {
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
+const int32_t* bits_limits() {
+  static int32_t limit[kBitsLimits];
+  static std::once_flag once;
+  std::call_once(once, [] {
+    for (int i = 0; i < kBitsLimits; ++i) {
+      int64_t lo = 1, hi = kRaggedWindow + 1;  // ragged_bits(lo) >= 50 - i, not so at hi
+      if (ragged_bits(kRaggedWindow) >= 50 - i) lo = kRaggedWindow;
+      while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) / 2;
+        (ragged_bits(mid) >= 50 - i ? lo : hi) = mid;
+      }
+      limit[i] = static_cast<int32_t>(lo);
+    }
+  });
+  return limit;
+}
+
+uint8_t* align_ws(void* workspace) {
+  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 1023) &
+                                    ~static_cast<uintptr_t>(1023));
+}
+
+RaggedPlan plan_at(const Layout& l, int64_t G, uint8_t* ws, bool tensor) {
+  auto ints = [&](size_t off) { return reinterpret_cast<int32_t*>(ws + off); };
   RaggedPlan p{};
-  p.row = reinterpret_cast<int32_t*>(ws + l.row);
-  p.small_start = reinterpret_cast<int32_t*>(ws + l.small_start);
-  p.tensor_start = reinterpret_cast<int32_t*>(ws + l.tensor_start);
+  p.groups = G;
+  p.row = ints(l.row);
+  p.small_start = ints(l.small_start);
+  p.tensor_start = ints(l.tensor_start);
+  p.slot = ints(l.slot);
   p.small = l.small_cap ? reinterpret_cast<RaggedTile*>(ws + l.small) : nullptr;
   p.tensor = l.tensor_cap ? reinterpret_cast<RaggedTile*>(ws + l.tensor) : nullptr;
+  p.slot_group = ints(l.slot_group);
+  p.slot_bits = ints(l.slot_bits);
   p.small_cap = l.small_cap;
   p.tensor_cap = l.tensor_cap;
-  p.counter = reinterpret_cast<int32_t*>(ws + l.counter);
+  p.counter = ints(l.counter);
   p.counters = l.counters;
   p.tensor_rows = tensor ? kTensorRows : INT32_MAX;
+  if (tensor)
+    for (int i = 0; i < kBitsLimits; ++i) p.bits_limit[i] = bits_limits()[i];
   return p;
 }
 
@@ -562,18 +612,24 @@ size_t ragged_dot_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, bo
 
 int ragged_dot(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) {
   if (q.M == 0 || q.N == 0) return ok();
-  ProfileScope prof("ragged_dot", s);
-  const SmallLayout l = layout_of(q.M, q.K, q.N, q.G, false);
+  const Layout l = layout_of(q.M, q.K, q.N, q.G, false);
+  int clusters = 0;
+  if (l.tensor_ok)
+    if (int st = ragged_tensor_clusters(&clusters)) return st;
+  uint8_t* ws = align_ws(workspace);
   SmallArgs a{};
   a.q = q;
-  a.p = plan_at(l, workspace, false);
+  a.p = plan_at(l, q.G, ws, clusters > 0);
   a.tiles_n = static_cast<int>(ceil_div(q.N, kTN));
   a.splits = l.splits;
   a.split_k = ceil_div(ceil_div(q.K, a.splits), kKS) * kKS;
-  a.partial = reinterpret_cast<double*>(static_cast<uint8_t*>(workspace) + l.partial);
+  a.partial = reinterpret_cast<double*>(ws + l.partial);
   a.vec_a = copy_width(q.lhs, q.K, q.lhs.s_r, 0);
   a.vec_b = copy_width(q.rhs, q.rhs_t ? q.K : q.N, q.rhs_t ? q.rhs.s_r : q.rhs.s_k, q.rhs.s_b);
   if (int st = launch_prep(q, 0, q.M, a.p, s)) return st;
+  if (clusters > 0)
+    if (int st = ragged_tensor_dot(q, a.p, ws + l.tensor_ws, clusters, s)) return st;
+  ProfileScope prof("ragged_small", s);
   const int64_t units = l.small_cap * a.tiles_n * a.splits;
   const bool pair = q.lhs.f64 == nullptr;
   if (q.rhs_t)
@@ -589,21 +645,34 @@ size_t ragged_contract_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t 
 
 int ragged_contract(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) {
   if (q.G == 0 || q.K == 0 || q.N == 0) return ok();
-  ProfileScope prof("ragged_dot_contract", s);
-  const SmallLayout l = layout_of(q.M, q.K, q.N, q.G, true);
+  const Layout l = layout_of(q.M, q.K, q.N, q.G, true);
+  int clusters = 0;
+  if (l.tensor_ok)
+    if (int st = ragged_tensor_clusters(&clusters)) return st;
+  uint8_t* ws = align_ws(workspace);
   SmallArgs a{};
   a.q = q;
-  a.p = plan_at(l, workspace, false);
+  a.p = plan_at(l, q.G, ws, clusters > 0);
   a.contract = true;
   a.tiles_k = static_cast<int>(ceil_div(q.K, kSmallTile));
   a.tiles_n = static_cast<int>(ceil_div(q.N, kTN));
   a.splits = 1;
   a.vec_a = copy_width(q.lhs, q.K, q.lhs.s_k, 0);
   a.vec_b = copy_width(q.rhs, q.N, q.rhs.s_k, 0);
-  if (int st = launch_prep(q, 0, q.M, a.p, s)) return st;
   const int64_t units = q.G * a.tiles_k * a.tiles_n;
-  return q.lhs.f64 == nullptr ? launch_small<true, true, true>(a, units, s)
-                              : launch_small<false, true, true>(a, units, s);
+  // without the tensor-core product one window takes all rows
+  const int64_t window = clusters > 0 ? kRaggedWindow : q.M + 1;
+  for (int64_t begin = 0; begin == 0 || begin < q.M; begin += window) {
+    a.add = begin > 0;
+    if (int st = launch_prep(q, begin, begin + window, a.p, s)) return st;
+    if (clusters > 0)
+      if (int st = ragged_tensor_contract(q, a.p, a.add, ws + l.tensor_ws, clusters, s)) return st;
+    ProfileScope prof("ragged_small", s);
+    const int st = q.lhs.f64 == nullptr ? launch_small<true, true, true>(a, units, s)
+                                        : launch_small<false, true, true>(a, units, s);
+    if (st) return st;
+  }
+  return ok();
 }
 
 }  // namespace dsb

@@ -1,0 +1,883 @@
+// The large groups of the products grouped by expert on the int8 tcgen05
+// tensor cores: the integer-residue product of dot_ozaki.cu (split, GEMM,
+// reconstruction, certificate and recomputation, with their error bounds) with
+// the groups' sizes read on the device.
+//
+// Products (rows of a group times its matrix): the rows keep their places in
+// the planes of A, [14][M][K]; a tile of the GEMM starts at any row of its
+// group and stores only the group's rows.  The matrices of the large groups
+// take slots, [14][slots][K][N] (or [N][K]): the others' are not read.
+//
+// Contraction (rows of a group contracted): both operands are split into
+// planes [14][positions][features] whose positions are the groups' rows, each
+// group padded with zeros to whole tiles of 256, and read as MN-major operands;
+// a unit of the GEMM runs over its group's tiles.  Every (group, feature) has
+// its own scale, and every group the bits its own length allows.
+//
+// A contraction longer than 32768 runs in chunks whose results are added.
+#include <cstring>
+#include <mutex>
+#include <string>
+#include <vector>
+
+#include "common.cuh"
+#include "ds_arith.cuh"
+#include "kernels.h"
+#include "ozaki.cuh"
+#include "profile.h"
+#include "ragged.h"
+
+namespace dsb {
+namespace {
+
+// The operand with its values moved by `off`.
+__device__ __forceinline__ DotOperand moved(DotOperand o, int64_t off) {
+  if (o.f64) {
+    o.f64 += off;
+  } else {
+    o.hi += off;
+    o.lo += off;
+  }
+  return o;
+}
+
+__device__ __forceinline__ int slots_of(const RaggedPlan& p) { return p.slot[p.groups]; }
+
+// ---- split ---------------------------------------------------------------------
+
+// Rows of the large groups, one block each: blockIdx.y is the row in tile
+// blockIdx.x.
+__global__ void __launch_bounds__(kSplitRowsMaxThreads, 2)
+ragged_split_rows_kernel(DotOperand o, int64_t M, int64_t K, int64_t Mp, int64_t Kp, int P,
+                         RaggedPlan p, uint8_t* __restrict__ planes, int* __restrict__ shifts,
+                         int* __restrict__ row_slot) {
+  wait_previous_grid();
+  if (static_cast<int>(blockIdx.x) >= p.tensor_start[p.groups]) return;
+  const RaggedTile t = p.tensor[blockIdx.x];
+  if (static_cast<int>(blockIdx.y) >= t.rows) return;
+  const int64_t row = t.row + static_cast<int>(blockIdx.y);
+  if (threadIdx.x == 0) row_slot[row] = t.slot + 1;
+  split_rows_body(o, M, K, Mp, Kp, 1, P, planes, shifts, row, 0);
+}
+
+// Matrices with K contiguous ([G, N, K]): column blockIdx.x of slot blockIdx.y.
+__global__ void __launch_bounds__(kSplitRowsMaxThreads, 2)
+ragged_split_matrix_rows_kernel(DotOperand o, int64_t N, int64_t K, int64_t Np, int64_t Kp,
+                                int64_t slots, int P, RaggedPlan p, uint8_t* __restrict__ planes,
+                                int* __restrict__ shifts) {
+  wait_previous_grid();
+  const int slot = blockIdx.y;
+  if (slot >= slots_of(p)) return;
+  DotOperand x = moved(o, p.slot_group[slot] * o.s_b);
+  x.s_b = 0;
+  split_rows_body(x, N, K, Np, Kp, slots, P, planes, shifts, blockIdx.x, slot);
+}
+
+// Column maxima of the matrices ([G, K, N]): slot blockIdx.z.
+__global__ void __launch_bounds__(256, 6)
+ragged_colmax_kernel(DotOperand o, int64_t N, int64_t K, int64_t Np, RaggedPlan p,
+                     int* __restrict__ codes) {
+  wait_previous_grid();
+  const int slot = blockIdx.z;
+  if (slot >= slots_of(p)) return;
+  DotOperand x = moved(o, p.slot_group[slot] * o.s_b);
+  x.s_b = 0;
+  colmax_body(x, N, K, Np, codes, blockIdx.x, blockIdx.y, slot);
+}
+
+// The same per group and feature of a contraction's operand: half blockIdx.y
+// % 2 of tile blockIdx.y / 2.
+__global__ void __launch_bounds__(256, 6)
+ragged_tile_colmax_kernel(DotOperand o, int64_t F, int64_t Fp, RaggedPlan p,
+                          int* __restrict__ codes) {
+  wait_previous_grid();
+  const int tile = blockIdx.y >> 1;
+  if (tile >= p.tensor_start[p.groups]) return;
+  const RaggedTile t = p.tensor[tile];
+  if (static_cast<int>(blockIdx.y & 1) * kColmaxSlab >= t.rows) return;
+  colmax_body(moved(o, t.row * o.s_k), F, t.rows, Fp, codes + static_cast<int64_t>(t.slot) * Fp,
+              blockIdx.x, blockIdx.y & 1, 0);
+}
+
+// DS pairs into row-contiguous planes, as split_mn_async_body does for f64:
+// each thread takes kMnCols rows at k = blockIdx.y, + gridDim.y, ...
+__device__ __forceinline__ void split_mn_pairs_body(const DotOperand& o, int64_t rows, int64_t K,
+                                                    int64_t rows_pad, int64_t Kp, int P,
+                                                    const int* __restrict__ codes,
+                                                    uint8_t* __restrict__ planes,
+                                                    size_t plane_stride, int* __restrict__ shifts) {
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kMnRows + threadIdx.x * kMnCols;
+  if (r0 >= rows_pad) return;
+  int sh[kMnCols];
+  bool z[kMnCols];
+#pragma unroll
+  for (int j = 0; j < kMnCols; ++j) {
+    const int64_t r = r0 + j;
+    const int sv = r < rows ? shift_from_code(codes[r], P) : 0;
+    if (blockIdx.y == 0) shifts[r] = sv;
+    z[j] = r >= rows || !shift_ordinary(sv);
+    sh[j] = z[j] ? 0 : sv;
+  }
+#pragma unroll 1
+  for (int64_t k = blockIdx.y; k < Kp; k += gridDim.y) {
+    Limbs x[kMnCols];
+#pragma unroll
+    for (int j = 0; j < kMnCols; ++j)
+      x[j] = limbs_of(quantise(z[j] || k >= K ? 0.0 : op_value(o, (r0 + j) * o.s_r + k * o.s_k),
+                               sh[j]));
+    store_planes_n<kMnCols, true>(x, planes + static_cast<size_t>(k) * rows_pad + r0,
+                                  plane_stride);
+  }
+}
+
+template <bool kPair>
+__device__ __forceinline__ void split_mn_body(const DotOperand& o, int64_t rows, int64_t K,
+                                              int64_t rows_pad, int64_t Kp, int P,
+                                              const int* codes, uint8_t* planes,
+                                              size_t plane_stride, int* shifts) {
+  if constexpr (kPair)
+    split_mn_pairs_body(o, rows, K, rows_pad, Kp, P, codes, planes, plane_stride, shifts);
+  else
+    split_mn_async_body(o, true, rows, K, rows_pad, Kp, P, codes, planes, plane_stride, shifts);
+}
+
+// Matrices [G, K, N] into planes [14][slots][Kp][Np]: slot blockIdx.z.
+template <bool kPair>
+__global__ void __launch_bounds__(256, 2)
+ragged_split_matrix_kernel(DotOperand o, int64_t N, int64_t K, int64_t Np, int64_t Kp,
+                           int64_t slots, int P, RaggedPlan p, const int* __restrict__ codes,
+                           uint8_t* __restrict__ planes, int* __restrict__ shifts) {
+  wait_previous_grid();
+  const int64_t slot = blockIdx.z;
+  if (slot >= slots_of(p)) return;
+  split_mn_body<kPair>(moved(o, p.slot_group[slot] * o.s_b), N, K, Np, Kp, P, codes + slot * Np,
+                       planes + static_cast<size_t>(slot) * Kp * Np,
+                       static_cast<size_t>(slots) * Kp * Np, shifts + slot * Np);
+}
+
+// A contraction's operand into planes [14][positions][Fp]: tile blockIdx.z.
+template <bool kPair>
+__global__ void __launch_bounds__(256, 2)
+ragged_split_tiles_kernel(DotOperand o, int64_t F, int64_t Fp, int64_t positions, RaggedPlan p,
+                          const int* __restrict__ codes, uint8_t* __restrict__ planes,
+                          int* __restrict__ shifts) {
+  wait_previous_grid();
+  const int tile = blockIdx.z;
+  if (tile >= p.tensor_start[p.groups]) return;
+  const RaggedTile t = p.tensor[tile];
+  split_mn_body<kPair>(moved(o, t.row * o.s_k), F, t.rows, Fp, kTensorTile, p.slot_bits[t.slot],
+                       codes + t.slot * Fp,
+                       planes + static_cast<size_t>(tile) * kTensorTile * Fp,
+                       static_cast<size_t>(positions) * Fp, shifts + t.slot * Fp);
+}
+
+// ---- GEMM ----------------------------------------------------------------------
+
+struct RaggedGemm {
+  RaggedPlan p;
+  int slots;                // of the planes
+  int tiles_m, tiles_n;     // tiles_m: contraction only
+  int stages;               // products only
+  int64_t Mp, Np;           // rows of a plane of A, columns
+  uint8_t* cres;
+};
+
+// Units (modulus, tile of rows, tile of columns), modulus outermost, so that
+// one modulus's planes stay in L2.
+template <bool kBMnPlanes>
+struct ProductWork {
+  static constexpr bool kAMn = false, kBMn = kBMnPlanes, kMasked = true;
+  const RaggedGemm& g;
+  int64_t tiles;
+  __device__ __forceinline__ int64_t units() const { return kL * tiles * g.tiles_n; }
+  __device__ __forceinline__ GemmTile at(int64_t u, uint32_t rank) const {
+    const int64_t per = tiles * g.tiles_n;
+    GemmTile t;
+    t.l = static_cast<int>(u / per);
+    const int64_t r = u - t.l * per;
+    const RaggedTile x = g.p.tensor[r / g.tiles_n];
+    const int tn = static_cast<int>(r % g.tiles_n), half = static_cast<int>(rank) * 128;
+    t.stages = g.stages;
+    t.k0 = 0;
+    t.za = 0;
+    t.a = static_cast<int>(t.l * g.Mp) + x.row + half;
+    t.zb = t.l * g.slots + x.slot;
+    t.b = (kBMn ? 0 : static_cast<int>(t.zb * g.Np)) + tn * 256 + half;
+    t.out = g.cres + (t.l * g.Mp + x.row + half) * g.Np + tn * 256;
+    t.rows = x.rows - half;
+    return t;
+  }
+};
+
+// Units (modulus, slot, tile of rows, tile of columns).
+struct ContractWork {
+  static constexpr bool kAMn = true, kBMn = true, kMasked = false;
+  const RaggedGemm& g;
+  int64_t slots;
+  __device__ __forceinline__ int64_t units() const {
+    return kL * slots * g.tiles_m * g.tiles_n;
+  }
+  __device__ __forceinline__ GemmTile at(int64_t u, uint32_t rank) const {
+    const int per = g.tiles_m * g.tiles_n;
+    const int64_t s = u / per;
+    const int r = static_cast<int>(u - s * per);
+    GemmTile t;
+    t.l = static_cast<int>(s / slots);
+    const int slot = static_cast<int>(s - t.l * slots);
+    const int group = g.p.slot_group[slot];
+    const int first = g.p.tensor_start[group];
+    const int half = static_cast<int>(rank) * 128;
+    t.stages = g.p.tensor_start[group + 1] - first;
+    t.k0 = first * kTensorTile;
+    t.za = t.zb = t.l;
+    t.a = r / g.tiles_n * 256 + half;
+    t.b = r % g.tiles_n * 256 + half;
+    t.out = g.cres + (static_cast<int64_t>(t.l * g.slots + slot) * g.Mp + t.a) * g.Np +
+            r % g.tiles_n * 256;
+    t.rows = 128;
+    return t;
+  }
+};
+static_assert(kTensorTile == kSub2 * kTileK, "a stage is a tile of positions");
+static_assert(kRaggedWindow == kMaxK, "a window of rows is one exact product");
+
+template <bool kBMn>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+ragged_product_gemm_kernel(const __grid_constant__ CUtensorMap ta,
+                           const __grid_constant__ CUtensorMap tb, RaggedGemm g, int* err) {
+  gemm2_body(ta, tb, ProductWork<kBMn>{g, g.p.tensor_start[g.p.groups]}, g.Np, err);
+}
+
+__global__ void __launch_bounds__(kGemmThreads, 1)
+ragged_contract_gemm_kernel(const __grid_constant__ CUtensorMap ta,
+                            const __grid_constant__ CUtensorMap tb, RaggedGemm g, int* err) {
+  gemm2_body(ta, tb, ContractWork{g, slots_of(g.p)}, g.Np, err);
+}
+
+// ---- reconstruction ----------------------------------------------------------------
+
+struct RaggedCrt {
+  double w[kL][2];
+  double mlimb[2];
+  double inv_m;
+  RaggedPlan p;
+  DotOperand a, b;
+  DotResult c;
+  int64_t M, K, N;       // rows; products: contraction; contraction: rows of a matrix
+  int64_t Mp, Np, slots;
+  int P;                 // products
+  const uint8_t* cres;
+  const int* sa;
+  const int* sb;
+  const int* row_slot;   // products: slot + 1 of each row
+  const int* err;
+  int* fix_count;
+  uint64_t* fix_list;
+  int64_t fix_cap;
+};
+
+// A row of the result: where its residues, scales and operands are.
+struct RowView {
+  bool live;
+  int slot, sa, P;
+  int64_t residues;      // row of the residue planes
+  int64_t out;           // row of the result
+  int64_t a, b, K;       // first elements and length of the contraction
+  double certify_below;
+};
+
+__device__ __forceinline__ double certify_below(int64_t K, int P) {
+  return (static_cast<double>(K) * pow2_normal(P) + 0x1p35) * pow2_normal(kCertifyBits);
+}
+
+template <bool kContract>
+__device__ __forceinline__ int64_t rows_of(const RaggedCrt& p) {
+  return kContract ? slots_of(p.p) * p.K : p.M;
+}
+
+template <bool kContract>
+__device__ __forceinline__ RowView view(const RaggedCrt& p, int64_t row) {
+  RowView v;
+  if constexpr (kContract) {
+    v.live = true;
+    v.slot = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(p.K));
+    const int64_t i = row - v.slot * p.K;
+    const int g = p.p.slot_group[v.slot];
+    const int64_t first = p.p.row[g];
+    v.residues = v.slot * p.Mp + i;
+    v.out = g * p.K + i;
+    v.a = first * p.a.s_k + i;
+    v.b = first * p.b.s_k;
+    v.K = p.p.row[g + 1] - first;
+    v.P = p.p.slot_bits[v.slot];
+    v.sa = p.sa[v.residues];
+  } else {
+    v.slot = p.row_slot[row] - 1;
+    v.live = v.slot >= 0;
+    if (!v.live) return v;
+    v.residues = v.out = row;
+    v.a = row * p.a.s_r;
+    v.b = p.p.slot_group[v.slot] * p.b.s_b;
+    v.K = p.K;
+    v.P = p.P;
+    v.sa = p.sa[row];
+  }
+  v.certify_below = certify_below(v.K, v.P);
+  return v;
+}
+
+// As crt_kernel in dot_ozaki.cu: kCols consecutive columns per thread over
+// rows blockIdx.y, + gridDim.y, ...
+constexpr int kRaggedCrtThreads = 128, kCols = 4;
+
+template <bool kContract>
+__global__ void __launch_bounds__(kRaggedCrtThreads, 8)
+ragged_crt_kernel(const __grid_constant__ RaggedCrt p) {
+  wait_previous_grid();
+  const size_t plane = static_cast<size_t>(kContract ? p.slots : 1) * p.Mp * p.Np;
+  const bool failed = *p.err != 0;
+  const int64_t j0 = (static_cast<int64_t>(blockIdx.x) * kRaggedCrtThreads + threadIdx.x) * kCols;
+  if (j0 >= p.N) return;
+  const int64_t rows = rows_of<kContract>(p);
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    const RowView v = view<kContract>(p, row);
+    if (!v.live) continue;
+    const uint8_t* src = p.cres + v.residues * p.Np + j0;
+    uint32_t cur[kL];
+#pragma unroll
+    for (int l = 0; l < kL; ++l)
+      cur[l] = __ldcs(reinterpret_cast<const unsigned int*>(src + l * plane));
+    double s_hi[kCols], s_lo[kCols];
+#pragma unroll
+    for (int q = 0; q < kCols; ++q) s_hi[q] = s_lo[q] = 0.0;
+#pragma unroll
+    for (int l = 0; l < kL; ++l) {
+      const double w_hi = p.w[l][0], w_lo = p.w[l][1];
+#pragma unroll
+      for (int q = 0; q < kCols; ++q) {
+        const double r = byte_to_f64(cur[l], q);
+        s_hi[q] = __fma_rn(r, w_hi, s_hi[q]);  // exact
+        s_lo[q] = __fma_rn(r, w_lo, s_lo[q]);
+      }
+    }
+    const int4 sbv = *reinterpret_cast<const int4*>(p.sb + v.slot * p.Np + j0);
+    const int sb[kCols] = {sbv.x, sbv.y, sbv.z, sbv.w};
+    double out[kCols];
+    bool put[kCols], all = j0 + kCols <= p.N;
+#pragma unroll
+    for (int q = 0; q < kCols; ++q) {
+      put[q] = j0 + q < p.N;
+      if (failed) {
+        out[q] = __longlong_as_double(0x7ff8000000000000LL);
+      } else if (shift_ordinary(v.sa) && shift_ordinary(sb[q])) {
+        const double approx = __fma_rn(s_hi[q], 0x1p70, s_lo[q]);
+        const double qt = rint(approx * p.inv_m);
+        const double t_hi = __fma_rn(-qt, p.mlimb[0], s_hi[q]);
+        const double t_lo = __fma_rn(-qt, p.mlimb[1], s_lo[q]);
+        const double c = __fma_rn(t_hi, 0x1p70, t_lo);
+        if (put[q] && !(fabs(c) >= v.certify_below)) {
+          // uncertified: listed for ragged_fix_kernel, which writes this output
+          put[q] = false;
+          const int at = atomicAdd(p.fix_count, 1);
+          if (at < p.fix_cap) p.fix_list[at] = static_cast<uint64_t>(row * p.N + j0 + q);
+        }
+        const int e = -(v.sa + sb[q]);
+        out[q] = (e >= -1022 && e <= 1023) ? c * pow2_normal(e) : scale2(scale2(c, -v.sa), -sb[q]);
+      } else if (v.sa == kShiftNonFinite || sb[q] == kShiftNonFinite) {
+        // a non-finite operand: the IEEE sum of the products
+        double s = 0.0;
+        if (put[q])
+          for (int64_t k = 0; k < v.K; ++k)
+            s += op_value(p.a, v.a + k * p.a.s_k) *
+                 op_value(p.b, v.b + (j0 + q) * p.b.s_r + k * p.b.s_k);
+        out[q] = s;
+      } else {
+        out[q] = 0.0;  // a row or column of zeros
+      }
+      all &= put[q];
+    }
+    const int64_t at = v.out * p.N + j0;
+    double* dst = p.c.f64 ? p.c.f64 + at : nullptr;
+    if (all && dst && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+      reinterpret_cast<double2*>(dst)[0] = make_double2(out[0], out[1]);
+      reinterpret_cast<double2*>(dst)[1] = make_double2(out[2], out[3]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kCols; ++q)
+        if (put[q]) put_result(p.c, at + q, out[q]);
+    }
+  }
+}
+
+// ---- recomputation of uncertified outputs -----------------------------------------
+
+constexpr int kRaggedFixThreads = 256, kFixTile = 64;
+
+// One output by one block (as dot2_block in dot_ozaki.cu): thread t sums k =
+// t, t + 256, ... in eight chains, merged in a fixed tree.
+__device__ double ragged_dot2(const RaggedCrt& p, const RowView& v, int64_t j, int da, int db) {
+  constexpr int kChains = 8;
+  __shared__ Dot2 s_warp[kRaggedFixThreads / 32];
+  const int64_t b0 = v.b + j * p.b.s_r;
+  Dot2 ch[kChains];
+  int64_t k = threadIdx.x;
+  auto add = [&](Dot2& d, int64_t at) {
+    dot2_add(d, scale2(op_value(p.a, v.a + at * p.a.s_k), da),
+             scale2(op_value(p.b, b0 + at * p.b.s_k), db));
+  };
+  for (; k + (kChains - 1) * kRaggedFixThreads < v.K; k += kChains * kRaggedFixThreads) {
+#pragma unroll
+    for (int u = 0; u < kChains; ++u) add(ch[u], k + u * kRaggedFixThreads);
+  }
+  for (; k < v.K; k += kRaggedFixThreads) add(ch[0], k);
+#pragma unroll
+  for (int w = 1; w < kChains; w <<= 1)
+#pragma unroll
+    for (int u = 0; u + w < kChains; u += 2 * w) dot2_merge(ch[u], ch[u + w]);
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    Dot2 o;
+    o.p = __shfl_down_sync(0xffffffffu, ch[0].p, off);
+    o.s = __shfl_down_sync(0xffffffffu, ch[0].s, off);
+    if (lane + off < 32) dot2_merge(ch[0], o);
+  }
+  if (lane == 0) s_warp[threadIdx.x >> 5] = ch[0];
+  __syncthreads();
+  double r = 0.0;
+  if (threadIdx.x == 0) {
+    Dot2 d = s_warp[0];
+    for (int w = 1; w < kRaggedFixThreads / 32; ++w) dot2_merge(d, s_warp[w]);
+    r = scale2(scale2(__dadd_rn(d.p, d.s), -da), -db);
+  }
+  __syncthreads();  // s_warp is reused
+  return r;
+}
+
+// Up to 64 rows from row0 on (of one group, `rows` of them) x 64 columns by
+// one block, as dot2_tile in dot_ozaki.cu.
+template <bool kContract>
+__device__ void ragged_dot2_tile(const RaggedCrt& p, int64_t row0, int rows, int64_t j0) {
+  __shared__ double sA[kFixTile][17];
+  __shared__ double sB[16][kFixTile + 1];
+  __shared__ int sShA[kFixTile], sShB[kFixTile];
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const RowView v = view<kContract>(p, row0);
+  const int64_t a_row = kContract ? 1 : p.a.s_r;  // from a row to the next
+  if (tid < kFixTile) {
+    sShA[tid] = tid < rows ? p.sa[v.residues + tid] : kShiftZero;
+    sShB[tid] = j0 + tid < p.N ? p.sb[v.slot * p.Np + j0 + tid] : kShiftZero;
+  }
+  __syncthreads();
+  Dot2 acc[4][4];
+  for (int64_t k0 = 0; k0 < v.K; k0 += 16) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int e = tid + t * kRaggedFixThreads;
+      {
+        const int r = e >> 4, kk = e & 15;
+        const bool in = k0 + kk < v.K && shift_ordinary(sShA[r]);
+        sA[r][kk] = in ? scale2(op_value(p.a, v.a + r * a_row + (k0 + kk) * p.a.s_k),
+                                sShA[r] - v.P)
+                       : 0.0;
+      }
+      {
+        const int kk = e >> 6, c = e & 63;
+        const bool in = k0 + kk < v.K && shift_ordinary(sShB[c]);
+        sB[kk][c] = in ? scale2(op_value(p.b, v.b + (j0 + c) * p.b.s_r + (k0 + kk) * p.b.s_k),
+                                sShB[c] - v.P)
+                       : 0.0;
+      }
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int kk = 0; kk < 16; ++kk) {
+      double x[4], y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = sA[ty + 16 * u][kk];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y[u] = sB[kk][tx + 16 * u];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) dot2_add(acc[u][w], x[u], y[w]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int r = ty + 16 * u;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int c = tx + 16 * w;
+      if (shift_ordinary(sShA[r]) && shift_ordinary(sShB[c]))
+        put_result(p.c, (v.out + r) * p.N + j0 + c,
+                   scale2(scale2(__dadd_rn(acc[u][w].p, acc[u][w].s), v.P - sShA[r]),
+                          v.P - sShB[c]));
+    }
+  }
+  __syncthreads();
+}
+
+// Every uncertified output: one block per listed output, or with more than
+// the list holds every output of the large groups.
+template <bool kContract>
+__global__ void __launch_bounds__(kRaggedFixThreads, 2)
+ragged_fix_kernel(const __grid_constant__ RaggedCrt p) {
+  wait_previous_grid();
+  const int count = *p.fix_count;
+  if (count == 0 || *p.err != 0) return;
+  if (count <= p.fix_cap) {
+    for (int e = blockIdx.x; e < count; e += gridDim.x) {
+      const int64_t flat = static_cast<int64_t>(p.fix_list[e]);
+      const int64_t row = flat / p.N, j = flat - row * p.N;
+      const RowView v = view<kContract>(p, row);
+      const double r = ragged_dot2(p, v, j, v.sa - v.P, p.sb[v.slot * p.Np + j] - v.P);
+      if (threadIdx.x == 0) put_result(p.c, v.out * p.N + j, r);
+    }
+    return;
+  }
+  const int64_t tn = (p.N + kFixTile - 1) / kFixTile;
+  if constexpr (kContract) {
+    const int64_t tk = (p.K + kFixTile - 1) / kFixTile, tiles = slots_of(p.p) * tk * tn;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+      const int64_t i = t / tn % tk * kFixTile;
+      ragged_dot2_tile<true>(p, t / (tn * tk) * p.K + i,
+                             p.K - i < kFixTile ? static_cast<int>(p.K - i) : kFixTile,
+                             t % tn * kFixTile);
+    }
+  } else {
+    constexpr int kParts = kTensorTile / kFixTile;
+    const int64_t tiles = p.p.tensor_start[p.p.groups] * kParts * tn;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+      const RaggedTile x = p.p.tensor[t / (tn * kParts)];
+      const int i = static_cast<int>(t / tn % kParts) * kFixTile, left = x.rows - i;
+      if (left > 0)
+        ragged_dot2_tile<false>(p, x.row + i, left < kFixTile ? left : kFixTile,
+                                t % tn * kFixTile);
+    }
+  }
+}
+
+// A later chunk of the contraction: the large groups' part added to the result.
+template <bool kContract>
+__global__ void __launch_bounds__(256)
+ragged_add_kernel(const __grid_constant__ RaggedCrt p, DotResult out) {
+  wait_previous_grid();
+  const int64_t rows = rows_of<kContract>(p);
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    const RowView v = view<kContract>(p, row);
+    if (!v.live) continue;
+    for (int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; j < p.N;
+         j += static_cast<int64_t>(gridDim.x) * 256) {
+      const int64_t at = v.out * p.N + j;
+      put_result(out, at, __dadd_rn(result_value(out, at), p.c.f64[at]));
+    }
+  }
+}
+
+// ---- host ------------------------------------------------------------------------
+
+struct TensorLayout {
+  int64_t chunk;            // longest contraction of a chunk
+  int64_t Mp, Np, Kp;       // contraction: Kp positions, Mp rows of a matrix
+  int64_t slots;
+  size_t a, b, c, sa, sb, clear, ca, cb, err, row_slot, clear_end, list, part, total;
+  int64_t fix_cap;
+};
+
+int64_t pad(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+TensorLayout tensor_layout(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
+  TensorLayout g{};
+  const int64_t length = contract ? M : K;
+  g.chunk = length < kMaxK ? length : kMaxK;
+  g.slots = ragged_slots(contract ? g.chunk : M, G);
+  g.Np = pad(N, 256);
+  size_t at = 0;
+  auto take = [&at](size_t bytes) {
+    const size_t here = at;
+    at = (at + bytes + 1023) / 1024 * 1024;
+    return here;
+  };
+  const size_t l = kL;
+  int64_t a_scales;
+  if (contract) {
+    g.Mp = pad(K, 256);
+    g.Kp = ragged_tensor_tiles(g.chunk, G) * kTensorTile;
+    g.a = take(l * g.Kp * g.Mp);
+    g.b = take(l * g.Kp * g.Np);
+    g.c = take(l * g.slots * g.Mp * g.Np);
+    a_scales = g.slots * g.Mp;
+  } else {
+    g.Mp = pad(M, 128);
+    g.Kp = pad(g.chunk, kTileK);
+    g.a = take(l * g.Mp * g.Kp);
+    g.b = take(l * g.slots * g.Np * g.Kp);
+    g.c = take(l * g.Mp * g.Np);
+    a_scales = g.Mp;
+  }
+  g.sa = take(4 * a_scales);
+  g.sb = take(4 * g.slots * g.Np);
+  // cleared together: column codes, error word and count, slots of the rows
+  g.clear = at;
+  g.ca = take(contract ? 4 * a_scales : 0);
+  g.cb = take(4 * g.slots * g.Np);
+  g.err = take(16);
+  g.row_slot = take(contract ? 0 : 4 * M);
+  g.clear_end = at;
+  const int64_t outputs = contract ? g.slots * K * N : M * N;
+  g.fix_cap = outputs < (1 << 20) ? outputs : 1 << 20;
+  g.list = take(8 * g.fix_cap);
+  g.part = take(length > g.chunk ? 8 * static_cast<size_t>(contract ? G * K * N : M * N) : 0);
+  g.total = at;
+  return g;
+}
+
+// The kernels' shared memory limit, once per device.
+int prepare_device(int* clusters) {
+  static std::mutex mu;
+  static std::vector<int> by_device;
+  int dev = 0;
+  DSB_CUDA_TRY(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lock(mu);
+  if (dev >= static_cast<int>(by_device.size())) by_device.resize(dev + 1, -1);
+  if (by_device[dev] < 0) {
+    int pairs = 0, query = 0;
+    if (int st = dot_ozaki_kernel_info(&pairs, &query)) return st;
+    const int bytes = static_cast<int>(gemm2_smem_bytes());
+    const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    DSB_CUDA_TRY(cudaFuncSetAttribute(ragged_product_gemm_kernel<false>, attr, bytes));
+    DSB_CUDA_TRY(cudaFuncSetAttribute(ragged_product_gemm_kernel<true>, attr, bytes));
+    DSB_CUDA_TRY(cudaFuncSetAttribute(ragged_contract_gemm_kernel, attr, bytes));
+    by_device[dev] = pairs;
+  }
+  *clusters = by_device[dev];
+  return DS_OK;
+}
+
+template <class Kernel>
+int launch_gemm(Kernel kernel, int clusters, const CUtensorMap& ta, const CUtensorMap& tb,
+                const RaggedGemm& g, int* err, cudaStream_t s) {
+  ProfileScope prof("ozaki_gemm", s);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = gemm2_smem_bytes();
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  DSB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ta, tb, g, err));
+  return DS_OK;
+}
+
+unsigned grid_y(int64_t n) { return static_cast<unsigned>(n < 1 ? 1 : n > 65535 ? 65535 : n); }
+
+template <bool kContract>
+int launch_rebuild(const RaggedCrt& c, int64_t rows, const DotResult* add_to, cudaStream_t s) {
+  {
+    ProfileScope prof("ozaki_crt", s);
+    const int64_t gx = (c.N + kRaggedCrtThreads * kCols - 1) / (kRaggedCrtThreads * kCols);
+    int64_t gy = (static_cast<int64_t>(sm_count()) * 16 + gx - 1) / gx;
+    if (gy > rows) gy = rows;
+    DSB_CUDA_TRY(launch_dependent(ragged_crt_kernel<kContract>,
+                                  dim3(static_cast<unsigned>(gx), grid_y(gy)),
+                                  dim3(kRaggedCrtThreads), s, c));
+  }
+  ProfileScope prof("ozaki_fix", s);
+  DSB_CUDA_TRY(launch_dependent(ragged_fix_kernel<kContract>,
+                                dim3(static_cast<unsigned>(2 * sm_count())),
+                                dim3(kRaggedFixThreads), s, c));
+  if (add_to)
+    DSB_CUDA_TRY(launch_dependent(ragged_add_kernel<kContract>,
+                                  dim3(static_cast<unsigned>((c.N + 255) / 256), grid_y(rows)),
+                                  dim3(256), s, c, *add_to));
+  return launch_status();
+}
+
+DotOperand at_k(DotOperand o, int64_t k) {
+  if (o.f64) o.f64 += k * o.s_k;
+  if (o.hi) o.hi += k * o.s_k;
+  if (o.lo) o.lo += k * o.s_k;
+  return o;
+}
+
+// Everything after the splits' shapes: fills what products and contraction
+// share.
+struct TensorRun {
+  uint8_t* ws;
+  TensorLayout g;
+  uint8_t *planes_a, *planes_b;
+  int *sa, *sb, *ca, *cb, *err, *row_slot;
+  RaggedCrt crt;
+  RaggedGemm gemm;
+};
+
+TensorRun tensor_run(const RaggedProblem& q, const RaggedPlan& p, const TensorLayout& g, void* at) {
+  TensorRun r{};
+  r.ws = static_cast<uint8_t*>(at);
+  r.g = g;
+  auto ints = [&](size_t off) { return reinterpret_cast<int*>(r.ws + off); };
+  r.planes_a = r.ws + g.a;
+  r.planes_b = r.ws + g.b;
+  r.sa = ints(g.sa);
+  r.sb = ints(g.sb);
+  r.ca = ints(g.ca);
+  r.cb = ints(g.cb);
+  r.err = ints(g.err);
+  r.row_slot = ints(g.row_slot);
+  const CrtConsts& cc = crt_consts();
+  std::memcpy(r.crt.w, cc.w, sizeof(r.crt.w));
+  std::memcpy(r.crt.mlimb, cc.mlimb, sizeof(r.crt.mlimb));
+  r.crt.inv_m = cc.inv_m;
+  r.crt.p = p;
+  r.crt.a = q.lhs;
+  r.crt.b = q.rhs;
+  r.crt.c = q.out;
+  r.crt.M = q.M;
+  r.crt.K = q.K;
+  r.crt.N = q.N;
+  r.crt.Mp = g.Mp;
+  r.crt.Np = g.Np;
+  r.crt.slots = g.slots;
+  r.crt.cres = r.ws + g.c;
+  r.crt.sa = r.sa;
+  r.crt.sb = r.sb;
+  r.crt.row_slot = r.row_slot;
+  r.crt.err = r.err;
+  r.crt.fix_count = r.err + 1;
+  r.crt.fix_list = reinterpret_cast<uint64_t*>(r.ws + g.list);
+  r.crt.fix_cap = g.fix_cap;
+  r.gemm.p = p;
+  r.gemm.slots = static_cast<int>(g.slots);
+  r.gemm.tiles_n = static_cast<int>(g.Np / 256);
+  r.gemm.Mp = g.Mp;
+  r.gemm.Np = g.Np;
+  r.gemm.cres = r.ws + g.c;
+  return r;
+}
+
+}  // namespace
+
+int ragged_bits(int64_t K) { return bits_for_k(K); }
+
+int ragged_tensor_clusters(int* clusters) { return prepare_device(clusters); }
+
+bool ragged_tensor_fits(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
+  const TensorLayout g = tensor_layout(M, K, N, G, contract);
+  const int64_t most = (1LL << 31) - 1;  // TMA coordinates and tile numbers are int32
+  if (g.total > kRaggedTensorBytes) return false;
+  if (contract) return g.slots * g.Mp <= most && g.Np <= most;
+  return kL * g.Mp <= most && kL * g.slots * g.Np <= most && g.slots <= 65535;
+}
+
+size_t ragged_tensor_bytes(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
+  return tensor_layout(M, K, N, G, contract).total;
+}
+
+int ragged_tensor_dot(const RaggedProblem& q, const RaggedPlan& p, void* workspace, int clusters,
+                      cudaStream_t s) {
+  const TensorLayout g = tensor_layout(q.M, q.K, q.N, q.G, false);
+  TensorRun r = tensor_run(q, p, g, workspace);
+  const unsigned tiles = static_cast<unsigned>(p.tensor_cap);
+  for (int64_t k0 = 0; k0 < q.K; k0 += g.chunk) {
+    const int64_t K = q.K - k0 < g.chunk ? q.K - k0 : g.chunk;
+    const int64_t Kp = pad(K, kTileK);  // of this chunk's planes
+    const int P = bits_for_k(K);
+    CUtensorMap ta, tb;
+    if (int st = make_tmap(&ta, r.planes_a, Kp, kL * g.Mp, kTileM)) return st;
+    if (q.rhs_t) {
+      if (int st = make_tmap(&tb, r.planes_b, Kp, kL * g.slots * g.Np, 128)) return st;
+    } else {
+      if (int st = make_tmap_mn(&tb, r.planes_b, g.Np, Kp, kL * g.slots)) return st;
+    }
+    const DotOperand a = at_k(q.lhs, k0), b = at_k(q.rhs, k0);
+    {
+      ProfileScope prof("ozaki_split", s);
+      DSB_CUDA_TRY(cudaMemsetAsync(r.ws + g.clear, 0, g.clear_end - g.clear, s));
+      const unsigned threads = static_cast<unsigned>(split_rows_threads(K));
+      DSB_CUDA_TRY(launch_dependent(ragged_split_rows_kernel, dim3(tiles, kTensorTile),
+                                    dim3(threads), s, a, q.M, K, g.Mp, Kp, P, p, r.planes_a, r.sa,
+                                    r.row_slot));
+      const unsigned slots = static_cast<unsigned>(g.slots);
+      if (q.rhs_t) {
+        DSB_CUDA_TRY(launch_dependent(ragged_split_matrix_rows_kernel,
+                                      dim3(static_cast<unsigned>(g.Np), slots), dim3(threads), s,
+                                      b, q.N, K, g.Np, Kp, g.slots, P, p, r.planes_b, r.sb));
+      } else {
+        DSB_CUDA_TRY(launch_dependent(
+            ragged_colmax_kernel,
+            dim3(static_cast<unsigned>(g.Np / kColTileR),
+                 static_cast<unsigned>((K + kColmaxSlab - 1) / kColmaxSlab), slots),
+            dim3(256), s, b, q.N, K, g.Np, p, r.cb));
+        const int64_t cx = (g.Np + kMnRows - 1) / kMnRows;
+        int64_t ky = (2 * static_cast<int64_t>(sm_count()) + cx - 1) / cx;
+        ky = ky > Kp / 16 ? Kp / 16 : ky;
+        const dim3 grid(static_cast<unsigned>(cx), grid_y(ky), slots);
+        if (q.rhs.f64)
+          DSB_CUDA_TRY(launch_dependent(ragged_split_matrix_kernel<false>, grid, dim3(256), s, b,
+                                        q.N, K, g.Np, Kp, g.slots, P, p, r.cb, r.planes_b,
+                                        r.sb));
+        else
+          DSB_CUDA_TRY(launch_dependent(ragged_split_matrix_kernel<true>, grid, dim3(256), s, b,
+                                        q.N, K, g.Np, Kp, g.slots, P, p, r.cb, r.planes_b,
+                                        r.sb));
+      }
+    }
+    r.gemm.stages = static_cast<int>((Kp / kTileK + kSub2 - 1) / kSub2);
+    if (int st = q.rhs_t ? launch_gemm(ragged_product_gemm_kernel<false>, clusters, ta, tb, r.gemm,
+                                       r.err, s)
+                         : launch_gemm(ragged_product_gemm_kernel<true>, clusters, ta, tb, r.gemm,
+                                       r.err, s))
+      return st;
+    r.crt.a = a;
+    r.crt.b = b;
+    r.crt.K = K;
+    r.crt.P = P;
+    if (k0 > 0) r.crt.c = DotResult{reinterpret_cast<double*>(r.ws + g.part), nullptr, nullptr};
+    if (int st = launch_rebuild<false>(r.crt, q.M, k0 > 0 ? &q.out : nullptr, s)) return st;
+  }
+  return DS_OK;
+}
+
+int ragged_tensor_contract(const RaggedProblem& q, const RaggedPlan& p, bool add, void* workspace,
+                           int clusters, cudaStream_t s) {
+  const TensorLayout g = tensor_layout(q.M, q.K, q.N, q.G, true);
+  TensorRun r = tensor_run(q, p, g, workspace);
+  const unsigned tiles = static_cast<unsigned>(p.tensor_cap);
+  CUtensorMap ta, tb;
+  if (int st = make_tmap_mn(&ta, r.planes_a, g.Mp, g.Kp, kL)) return st;
+  if (int st = make_tmap_mn(&tb, r.planes_b, g.Np, g.Kp, kL)) return st;
+  {
+    ProfileScope prof("ozaki_split", s);
+    DSB_CUDA_TRY(cudaMemsetAsync(r.ws + g.clear, 0, g.clear_end - g.clear, s));
+    auto split = [&](const DotOperand& o, int64_t F, int64_t Fp, int* codes, uint8_t* planes,
+                     int* shifts) -> int {
+      DSB_CUDA_TRY(launch_dependent(ragged_tile_colmax_kernel,
+                                    dim3(static_cast<unsigned>(Fp / kColTileR), 2 * tiles),
+                                    dim3(256), s, o, F, Fp, p, codes));
+      const dim3 grid(static_cast<unsigned>((Fp + kMnRows - 1) / kMnRows), 8, tiles);
+      if (o.f64)
+        DSB_CUDA_TRY(launch_dependent(ragged_split_tiles_kernel<false>, grid, dim3(256), s, o, F,
+                                      Fp, g.Kp, p, codes, planes, shifts));
+      else
+        DSB_CUDA_TRY(launch_dependent(ragged_split_tiles_kernel<true>, grid, dim3(256), s, o, F,
+                                      Fp, g.Kp, p, codes, planes, shifts));
+      return DS_OK;
+    };
+    if (int st = split(q.lhs, q.K, g.Mp, r.ca, r.planes_a, r.sa)) return st;
+    if (int st = split(q.rhs, q.N, g.Np, r.cb, r.planes_b, r.sb)) return st;
+  }
+  r.gemm.tiles_m = static_cast<int>(g.Mp / 256);
+  if (int st = launch_gemm(ragged_contract_gemm_kernel, clusters, ta, tb, r.gemm, r.err, s))
+    return st;
+  if (add) r.crt.c = DotResult{reinterpret_cast<double*>(r.ws + g.part), nullptr, nullptr};
+  return launch_rebuild<true>(r.crt, g.slots * q.K, add ? &q.out : nullptr, s);
+}
+
+}  // namespace dsb
