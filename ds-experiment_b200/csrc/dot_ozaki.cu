@@ -240,8 +240,7 @@ split_mn_async_kernel(DotOperand o, int64_t rows, int64_t K, int64_t rows_pad, i
                       uint8_t* __restrict__ planes, int* __restrict__ shifts) {
   wait_previous_grid();  // the column maxima
   const int64_t b = blockIdx.z;
-  o.f64 += b * o.s_b;
-  split_mn_async_body(o, (o.s_b & 1) == 0, rows, K, rows_pad, Kp, P, codes + b * rows_pad,
+  split_mn_async_body(o, b * o.s_b, (o.s_b & 1) == 0, rows, K, rows_pad, Kp, P, codes + b * rows_pad,
                       planes + static_cast<size_t>(b) * Kp * rows_pad,
                       static_cast<size_t>(batch) * Kp * rows_pad, shifts + b * rows_pad);
 }
@@ -485,7 +484,7 @@ struct UniformWork {
 };
 
 template <bool kBMn>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(kGemm2Threads, 1)
 ozaki_gemm2_kernel(const __grid_constant__ CUtensorMap tmap_a,
                    const __grid_constant__ CUtensorMap tmap_b, GemmParams p) {
   gemm2_body(tmap_a, tmap_b, UniformWork<kBMn>{p}, p.Np, p.err);
@@ -875,7 +874,7 @@ const GemmSetup& gemm_setup() {
       attr[0].val.clusterDim.y = 1;
       attr[0].val.clusterDim.z = 1;
       cfg.gridDim = dim3(2 * 74);
-      cfg.blockDim = dim3(kGemmThreads);
+      cfg.blockDim = dim3(kGemm2Threads);
       cfg.dynamicSmemBytes = gemm2_smem_bytes();
       cfg.attrs = attr;
       cfg.numAttrs = 1;
@@ -1126,7 +1125,7 @@ int dot_ozaki_one(const DotProblem& p, void* workspace, size_t workspace_bytes, 
       attr[0].val.clusterDim.y = 1;
       attr[0].val.clusterDim.z = 1;
       cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
-      cfg.blockDim = dim3(kGemmThreads);
+      cfg.blockDim = dim3(kGemm2Threads);
       cfg.dynamicSmemBytes = gemm2_smem_bytes();
       cfg.stream = st;
       cfg.attrs = attr;

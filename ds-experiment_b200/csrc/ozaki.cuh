@@ -546,7 +546,7 @@ __device__ __forceinline__ void cp_async_wait() {
 // faster than four.  (The same pipeline for A's rows, with B's column
 // maxima in a kernel of their own, was slower than split_rows_colmax_kernel:
 // 0.095 + 0.030 ms against 0.102 ms for both.)
-__device__ __forceinline__ void split_mn_async_body(const DotOperand& o, bool even_base,
+__device__ __forceinline__ void split_mn_async_body(const DotOperand& o, int64_t off, bool even_off,
                                                     int64_t rows, int64_t K, int64_t rows_pad,
                                                     int64_t Kp, int P,
                                                     const int* __restrict__ codes,
@@ -566,11 +566,11 @@ __device__ __forceinline__ void split_mn_async_body(const DotOperand& o, bool ev
     z[j] = r >= rows || sv == kShiftNonFinite || sv == kShiftZero;
     sh[j] = z[j] ? 0 : sv;
   }
-  const bool vec = r0 + kMnCols <= rows && (o.s_k & 1) == 0 && even_base &&
+  const bool vec = r0 + kMnCols <= rows && (o.s_k & 1) == 0 && even_off &&
                    (reinterpret_cast<uintptr_t>(o.f64) & 15) == 0;
   // addresses of copies that read nothing (zero fill) still point inside
   // the operand
-  const double* base = o.f64 + (r0 < rows ? r0 : 0);
+  const double* base = o.f64 + off + (r0 < rows ? r0 : 0);
   const int64_t kstep = gridDim.y;
   auto issue = [&](int64_t k, int slot) {
     double* dst = stage[slot][threadIdx.x];
@@ -760,9 +760,17 @@ __device__ __forceinline__ uint32_t mod_pack4(const uint32_t* v, uint32_t m, uin
                      __byte_perm(mod_u8(v[2], m, magic), mod_u8(v[3], m, magic), 0x0040), 0x5410);
 }
 
+// Epilogue warps of each CTA (eight, sharing the columns, were 1 to 3% slower).
+constexpr int kEpilogueWarps2 = 4;
+constexpr int kGemm2Threads = 64 + 32 * kEpilogueWarps2;
 constexpr int kStages2 = 3;
 constexpr int kSub2 = 2;  // 128-byte K sub-tiles per stage
 constexpr int kStage2 = kTileM * kTileK;  // 16 KB: A rows, or half of the B tile
+// Residues of a CTA's 128 x 256 outputs on their way to memory: a thread
+// holds a row of the accumulator, so a store from its registers would write 16
+// bytes of 32 rows at a time; staged here, each warp stores whole lines of its
+// rows.
+constexpr int kOut2 = kTileM * 256;
 constexpr uint32_t kIdesc2 = (2u << 4) | (0u << 7) | (0u << 10) | ((256u >> 3) << 17) |
                              ((256u >> 4) << 24);
 constexpr uint32_t kIdescAMajorMN = 1u << 15;  // A MN-major
@@ -819,9 +827,12 @@ __device__ __noinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, i
   return true;
 }
 
+// Arrival on another CTA's barrier, ordered after this thread's reads of TMEM
+// (tcgen05.wait::ld and the fence before it), not after its global stores: with
+// .release.cluster it waited for them too, which held the GEMM at 1.9 POPS for
+// K = 1024 (2.6 now) and at 3.32 for K = 4096 (3.46 now).
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
-               : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y,
@@ -892,7 +903,8 @@ __device__ __forceinline__ void gemm2_body(const CUtensorMap& tmap_a, const CUte
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* smem_a = smem;
   uint8_t* smem_b = smem + kStages2 * kSub2 * kStage2;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + 2 * kStages2 * kSub2 * kStage2);
+  uint8_t* smem_out = smem + 2 * kStages2 * kSub2 * kStage2;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_out + kOut2);
   uint64_t* empty = full + kStages2;
   uint64_t* tfull = empty + kStages2;
   uint64_t* tempty = tfull + 2;
@@ -909,7 +921,7 @@ __device__ __forceinline__ void gemm2_body(const CUtensorMap& tmap_a, const CUte
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 8);  // 4 epilogue warps in each of the 2 CTAs
+      mbar_init(&tempty[a], 2 * kEpilogueWarps2);  // the epilogue warps of both CTAs
     }
     mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -935,8 +947,11 @@ __device__ __forceinline__ void gemm2_body(const CUtensorMap& tmap_a, const CUte
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
+      // each unit's place is looked up while the one before it is under way
+      GemmTile next = cid < units ? work.at(cid, rank) : GemmTile{};
       for (int64_t u = cid; u < units && ok; u += ncl) {
-        const GemmTile w = work.at(u, rank);
+        const GemmTile w = next;
+        if (u + ncl < units) next = work.at(u + ncl, rank);
         for (int kb = 0; kb < w.stages; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, err, 11)) {
             ok = false;
@@ -974,13 +989,15 @@ __device__ __forceinline__ void gemm2_body(const CUtensorMap& tmap_a, const CUte
       int acc = 0;
       uint32_t acc_phase = 0;
       bool ok = true;
+      int next = cid < units ? work.at(cid, rank).stages : 0;
       for (int64_t u = cid; u < units && ok; u += ncl) {
         if (!mbar_wait_cluster(&tempty[acc], acc_phase ^ 1, err, 12)) break;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(acc * 256);
         constexpr uint32_t idesc = kIdesc2 | (Work::kAMn ? kIdescAMajorMN : 0u) |
                                    (Work::kBMn ? kIdescBMajorMN : 0u);
-        const int stages = work.at(u, rank).stages;
+        const int stages = next;
+        if (u + ncl < units) next = work.at(u + ncl, rank).stages;
         for (int kb = 0; kb < stages; ++kb) {
           if (!mbar_wait(&full[stage], phase, err, 13)) {
             ok = false;
@@ -1019,37 +1036,50 @@ __device__ __forceinline__ void gemm2_body(const CUtensorMap& tmap_a, const CUte
       }
     }
   } else {
-    // ---- epilogue (both CTAs; warps 2..5, TMEM lanes 32*(warp%4) ..) ----
+    // ---- epilogue (both CTAs; warps 2.., TMEM lanes 32*(warp%4) .., the
+    // columns shared out among the warps of the same lanes) ----
     const int quad = warp & 3;
-    const int row_in_tile = quad * 32 + lane;
+    constexpr int kCols = 256 * 4 / kEpilogueWarps2;
+    const int col0 = (warp - 2) / 4 * kCols;
     const uint32_t tempty0[2] = {in_rank0(&tempty[0]), in_rank0(&tempty[1])};
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int64_t u = cid; u < units; u += ncl) {
+      const GemmTile w = work.at(u, rank);
       if (!mbar_wait(&tfull[acc], acc_phase, err, 14)) break;
       tc_fence_after();
-      const GemmTile w = work.at(u, rank);
       const uint32_t m = static_cast<uint32_t>(mod_of(w.l));
       const uint32_t magic = epilogue_magic(m);
-      uint8_t* out = w.out + row_in_tile * Np;
       const uint32_t tbase = tmem + (static_cast<uint32_t>(quad * 32) << 16) +
                              static_cast<uint32_t>(acc * 256);
+      // the warp's 32 rows x kCols bytes, 16-byte words swizzled by the row
+      constexpr int kWords = kCols / 16;
+      uint4* own = reinterpret_cast<uint4*>(smem_out) + (warp - 2) * 32 * kWords;
 #pragma unroll 1
-      for (int c0 = 0; c0 < 256; c0 += 32) {
+      for (int c0 = 0; c0 < kCols; c0 += 32) {
         uint32_t v[32];
-        tmem_ld32(tbase + c0, v);
+        tmem_ld32(tbase + col0 + c0, v);
         uint32_t packed[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) packed[q] = mod_pack4(v + q * 4, m, magic);
-        if (!Work::kMasked || row_in_tile < w.rows) {
-          uint4* dst = reinterpret_cast<uint4*>(out + c0);
-          dst[0] = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-          dst[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
-        }
+        const int word = c0 / 16;
+        own[lane * kWords + (word ^ lane % kWords)] =
+            make_uint4(packed[0], packed[1], packed[2], packed[3]);
+        own[lane * kWords + ((word + 1) ^ lane % kWords)] =
+            make_uint4(packed[4], packed[5], packed[6], packed[7]);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(tempty0[acc]);
+      constexpr int kRowsAtOnce = 32 / kWords;
+#pragma unroll 4
+      for (int r0 = 0; r0 < 32; r0 += kRowsAtOnce) {
+        const int r = r0 + lane / kWords, word = lane % kWords;
+        if (!Work::kMasked || quad * 32 + r < w.rows)
+          *reinterpret_cast<uint4*>(w.out + static_cast<int64_t>(quad * 32 + r) * Np + col0 +
+                                    word * 16) = own[r * kWords + (word ^ r % kWords)];
+      }
+      __syncwarp();
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1;
@@ -1190,7 +1220,7 @@ size_t gemm_smem_bytes() {
 }
 
 size_t gemm2_smem_bytes() {
-  return 1024 + 2 * kStages2 * kSub2 * kStage2 + (2 * kStages2 + 5) * sizeof(uint64_t) + 16;
+  return 1024 + 2 * kStages2 * kSub2 * kStage2 + kOut2 + (2 * kStages2 + 5) * sizeof(uint64_t) + 16;
 }
 
 }  // namespace

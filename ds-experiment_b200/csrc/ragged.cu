@@ -156,17 +156,16 @@ constexpr int kOperand = kSmallTile * kPitchK > kKS * kPitchN ? kSmallTile * kPi
 constexpr size_t kSmallBytes = sizeof(double) * 2 * kStages * kOperand;
 static_assert(kTN == kSmallTile, "A and B are staged alike");
 
-__device__ __forceinline__ void copy_async(void* dst, const void* src, int bytes, bool valid) {
+template <int kBytes>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool valid) {
   const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
-  const int n = valid ? bytes : 0;
-  if (bytes == 16)
+  const int n = valid ? kBytes : 0;
+  if constexpr (kBytes == 16)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(src), "r"(n)
                  : "memory");
-  else if (bytes == 8)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(src), "r"(n)
-                 : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(src), "r"(n)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(at), "l"(src), "n"(kBytes),
+                 "r"(n)
                  : "memory");
 }
 
@@ -198,25 +197,34 @@ struct Block2d {
   int lines, len;
 };
 
-// `lines_pad` x `len_pad` values of the block into a staged tile (pitch values
-// per line), zeros outside it; `vec` values per copy.
-template <bool kPair>
-__device__ __forceinline__ void stage_block(const DotOperand& o, const Block2d& b, int lines_pad,
-                                            int len_pad, double* tile, int pitch, int vec) {
+// kLines lines of kLen values (powers of two) of the block into a staged tile
+// (pitch values per line), zeros outside it; kVec values per copy.
+template <bool kPair, int kLen, int kVec>
+__device__ __forceinline__ void stage_lines(const DotOperand& o, const Block2d& b, int lines,
+                                            double* tile, int pitch) {
   constexpr int kElem = kPair ? 4 : 8;
-  const int per_line = len_pad / vec;
-  for (int e = threadIdx.x; e < lines_pad * per_line; e += kThreads) {
-    const int line = e / per_line, at = (e - line * per_line) * vec;
-    const bool in = line < b.lines && at < b.len;  // vec divides len
+  constexpr int kPerLine = kLen / kVec, kStep = kThreads / kPerLine;
+  const int at = threadIdx.x % kPerLine * kVec;
+  const bool in_line = at < b.len;  // kVec divides len
+#pragma unroll 4
+  for (int line = threadIdx.x / kPerLine; line < lines; line += kStep) {
+    const bool in = in_line && line < b.lines;
     const int64_t src = in ? b.origin + line * b.stride + at : 0;
     if constexpr (kPair) {
       float* f = reinterpret_cast<float*>(tile) + line * pitch + at;
-      copy_async(f, o.hi + src, kElem * vec, in);
-      copy_async(f + kOperand, o.lo + src, kElem * vec, in);
+      copy_async<kElem * kVec>(f, o.hi + src, in);
+      copy_async<kElem * kVec>(f + kOperand, o.lo + src, in);
     } else {
-      copy_async(tile + line * pitch + at, o.f64 + src, kElem * vec, in);
+      copy_async<kElem * kVec>(tile + line * pitch + at, o.f64 + src, in);
     }
   }
+}
+
+template <bool kPair, int kLen>
+__device__ __forceinline__ void stage_block(const DotOperand& o, const Block2d& b, int lines,
+                                            double* tile, int pitch, int vec) {
+  if (vec > 1) stage_lines<kPair, kLen, kPair ? 4 : 2>(o, b, lines, tile, pitch);
+  else stage_lines<kPair, kLen, 1>(o, b, lines, tile, pitch);
 }
 
 struct SmallArgs {
@@ -286,22 +294,22 @@ __device__ __forceinline__ void stage_unit(const SmallArgs& a, const SmallUnit& 
                                            double* sa, double* sb) {
   const int kn = x.k1 - k < kKS ? static_cast<int>(x.k1 - k) : kKS;
   const RaggedProblem& q = a.q;
-  const int rows_pad = x.rows <= 16 ? 16 : kSmallTile;
+  [[maybe_unused]] const int rows_pad = x.rows <= 16 ? 16 : kSmallTile;
   Block2d A, B;
   if constexpr (kA) {
     A = Block2d{x.row + k * q.lhs.s_k, q.lhs.s_k, kn, x.rows};
-    stage_block<kPair>(q.lhs, A, kKS, rows_pad, sa, kPitchN, a.vec_a);
+    stage_block<kPair, kSmallTile>(q.lhs, A, kKS, sa, kPitchN, a.vec_a);
   } else {
     A = Block2d{x.row * q.lhs.s_r + k, q.lhs.s_r, x.rows, kn};
-    stage_block<kPair>(q.lhs, A, rows_pad, kKS, sa, kPitchK, a.vec_a);
+    stage_block<kPair, kKS>(q.lhs, A, rows_pad, sa, kPitchK, a.vec_a);
   }
   const int64_t base = a.contract ? 0 : x.g * q.rhs.s_b;
   if constexpr (kB) {
     B = Block2d{base + k * q.rhs.s_k + x.col, q.rhs.s_k, kn, x.cols};
-    stage_block<kPair>(q.rhs, B, kKS, kTN, sb, kPitchN, a.vec_b);
+    stage_block<kPair, kTN>(q.rhs, B, kKS, sb, kPitchN, a.vec_b);
   } else {
     B = Block2d{base + x.col * q.rhs.s_r + k, q.rhs.s_r, x.cols, kn};
-    stage_block<kPair>(q.rhs, B, kTN, kKS, sb, kPitchK, a.vec_b);
+    stage_block<kPair, kKS>(q.rhs, B, kTN, sb, kPitchK, a.vec_b);
   }
 }
 

@@ -15,7 +15,10 @@ constexpr int kSmallTile = 64;    // rows of a small group's tile
 constexpr int kTensorTile = 256;  // rows of a tile of the tensor-core product
 // Groups of at least this many rows are large: the tensor-core product takes
 // them.
-constexpr int64_t kTensorRows = 128;
+#ifndef KTR
+#define KTR 128
+#endif
+constexpr int64_t kTensorRows = KTR;
 // Longest contraction over rows that is taken at once.
 constexpr int64_t kRaggedWindow = 1 << 15;
 // Most workspace that the tensor-core product may ask for.

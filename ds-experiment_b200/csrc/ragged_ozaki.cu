@@ -138,7 +138,7 @@ __device__ __forceinline__ void split_mn_body(const DotOperand& o, int64_t rows,
   if constexpr (kPair)
     split_mn_pairs_body(o, rows, K, rows_pad, Kp, P, codes, planes, plane_stride, shifts);
   else
-    split_mn_async_body(o, true, rows, K, rows_pad, Kp, P, codes, planes, plane_stride, shifts);
+    split_mn_async_body(o, 0, true, rows, K, rows_pad, Kp, P, codes, planes, plane_stride, shifts);
 }
 
 // Matrices [G, K, N] into planes [14][slots][Kp][Np]: slot blockIdx.z.
@@ -242,13 +242,13 @@ static_assert(kTensorTile == kSub2 * kTileK, "a stage is a tile of positions");
 static_assert(kRaggedWindow == kMaxK, "a window of rows is one exact product");
 
 template <bool kBMn>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(kGemm2Threads, 1)
 ragged_product_gemm_kernel(const __grid_constant__ CUtensorMap ta,
                            const __grid_constant__ CUtensorMap tb, RaggedGemm g, int* err) {
   gemm2_body(ta, tb, ProductWork<kBMn>{g, g.p.tensor_start[g.p.groups]}, g.Np, err);
 }
 
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(kGemm2Threads, 1)
 ragged_contract_gemm_kernel(const __grid_constant__ CUtensorMap ta,
                             const __grid_constant__ CUtensorMap tb, RaggedGemm g, int* err) {
   gemm2_body(ta, tb, ContractWork{g, slots_of(g.p)}, g.Np, err);
@@ -667,7 +667,7 @@ int launch_gemm(Kernel kernel, int clusters, const CUtensorMap& ta, const CUtens
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(kGemm2Threads);
   cfg.dynamicSmemBytes = gemm2_smem_bytes();
   cfg.stream = s;
   cfg.attrs = attr;
