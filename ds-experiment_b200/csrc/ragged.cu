@@ -84,7 +84,6 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
             RaggedPlan p) {
   wait_previous_grid();
   const int64_t tid = threadIdx.x;
-  for (int64_t i = tid; i < p.counters; i += kPrepThreads) p.counter[i] = 0;
   int64_t rows_before = 0, tiles_before = 0, slots_before = 0;
   for (int64_t g0 = 0; g0 < G; g0 += kPrepThreads) {
     const int64_t g = g0 + tid;
@@ -147,19 +146,33 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
 constexpr int kThreads = 256;
 constexpr int kTN = 64;      // columns of a tile
 constexpr int kKS = 32;      // contraction per pipeline stage
-constexpr int kStages = 3;
 // Row pitches of the staged tiles, in values: 4 (mod 16) puts the 4 x 4
 // values that half a warp reads for a fragment in 16 different 8-byte banks.
-constexpr int kPitchK = kKS + 4;       // [row or column][k]
+constexpr int kPitchK = kKS + 4;         // [row or column][k]
 constexpr int kPitchN = kSmallTile + 4;  // [k][row or column]
-constexpr int kOperand = kSmallTile * kPitchK > kKS * kPitchN ? kSmallTile * kPitchK : kKS * kPitchN;
-constexpr size_t kSmallBytes = sizeof(double) * 2 * kStages * kOperand;
-static_assert(kTN == kSmallTile, "A and B are staged alike");
 
+// Values of a staged operand of up to `rows` rows or columns.
+__host__ __device__ constexpr int operand_values(int rows) {
+  return rows * kPitchK > kKS * kPitchN && rows == kSmallTile ? rows * kPitchK
+         : rows == kSmallTile                                  ? kKS * kPitchN
+                                                               : rows * kPitchK;
+}
+constexpr int kOperandB = operand_values(kTN);
+
+// Stages in flight: two blocks per SM share 227 KB.  With A tiles of at most 16
+// rows a fourth one fits.
+template <int kRows>
+struct Stages {
+  static constexpr int kCount = kRows == kSmallTile ? 3 : 4;
+  static constexpr int kOperandA = operand_values(kRows);
+  static constexpr int kStride = kOperandA + kOperandB;
+  static constexpr size_t kBytes = sizeof(double) * kCount * kStride;
+};
+
+// The first n bytes from src, zeros for the rest of kBytes.
 template <int kBytes>
-__device__ __forceinline__ void copy_async(void* dst, const void* src, bool valid) {
+__device__ __forceinline__ void copy_async(void* dst, const void* src, int n) {
   const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
-  const int n = valid ? kBytes : 0;
   if constexpr (kBytes == 16)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(src), "r"(n)
                  : "memory");
@@ -178,9 +191,20 @@ __device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
       : "d"(a), "d"(b));
 }
 
-// A staged operand: f64 values, or (kPair) the hi words and behind them the
-// lo words.
-template <bool kPair>
+// The same of a 16 x 8 and an 8 x 8 fragment: a[8 (i % 2) + l / 4][4 (i / 2) +
+// l % 4], b[4 i + l % 4][l / 4], d[8 (i / 2) + l / 4][2 (l % 4) + i % 2].
+__device__ __forceinline__ void mma_f64_wide(double (&d0)[2], double (&d1)[2],
+                                             const double (&a)[4], const double (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f64.f64.f64.f64 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+d"(d0[0]), "+d"(d0[1]), "+d"(d1[0]), "+d"(d1[1])
+      : "d"(a[0]), "d"(a[1]), "d"(a[2]), "d"(a[3]), "d"(b[0]), "d"(b[1]));
+}
+
+// A staged operand: f64 values, or (kPair) the hi words and, kOperand of them
+// further on, the lo words.
+template <bool kPair, int kOperand>
 __device__ __forceinline__ double staged(const double* tile, int at) {
   if constexpr (kPair) {
     const float* f = reinterpret_cast<const float*>(tile);
@@ -190,152 +214,295 @@ __device__ __forceinline__ double staged(const double* tile, int at) {
   }
 }
 
-// One operand's part of a unit: `lines` lines of `len` consecutive values,
+// One operand's part of a stage: `lines` lines of `len` consecutive values,
 // line t at offset origin + t stride of the operand.
 struct Block2d {
   int64_t origin, stride;
   int lines, len;
 };
 
-// kLines lines of kLen values (powers of two) of the block into a staged tile
-// (pitch values per line), zeros outside it; kVec values per copy.
-template <bool kPair, int kLen, int kVec>
-__device__ __forceinline__ void stage_lines(const DotOperand& o, const Block2d& b, int lines,
-                                            double* tile, int pitch) {
-  constexpr int kElem = kPair ? 4 : 8;
-  constexpr int kPerLine = kLen / kVec, kStep = kThreads / kPerLine;
-  const int at = threadIdx.x % kPerLine * kVec;
-  const bool in_line = at < b.len;  // kVec divides len
+// f64 lines move in 16-byte words wherever they start: a line whose first value
+// lies off the 16-byte boundary is staged one place later (odd_start), its first
+// and last value moved alone.
+__device__ __forceinline__ int odd_start(const DotOperand& o, int64_t origin, int64_t stride,
+                                         int line) {
+  return static_cast<int>((reinterpret_cast<uintptr_t>(o.f64) >> 3) + origin + line * stride) & 1;
+}
+
+// `lines_pad` lines of kLen values of the block into a staged tile (kPitch values
+// per line), zeros outside it.
+template <int kLen, int kPitch>
+__device__ __forceinline__ void stage_f64(const DotOperand& o, const Block2d& b, int lines_pad,
+                                          double* tile) {
+  constexpr int kWords = kLen / 2, kStep = kThreads / kWords;  // lines at once (even)
+  const int c = threadIdx.x % kWords, l0 = threadIdx.x / kWords;
+  const int odd = odd_start(o, b.origin, b.stride, l0);
+  const int first = 2 * c - odd, left = b.len - first;
+  const double* src = o.f64 + b.origin + l0 * b.stride + first;
+  double* dst = tile + l0 * kPitch + 2 * c;
+  if (first < 0) {  // the first value, and the last one
+    const bool last = kLen - 1 < b.len;
 #pragma unroll 4
-  for (int line = threadIdx.x / kPerLine; line < lines; line += kStep) {
-    const bool in = in_line && line < b.lines;
-    const int64_t src = in ? b.origin + line * b.stride + at : 0;
-    if constexpr (kPair) {
-      float* f = reinterpret_cast<float*>(tile) + line * pitch + at;
-      copy_async<kElem * kVec>(f, o.hi + src, in);
-      copy_async<kElem * kVec>(f + kOperand, o.lo + src, in);
-    } else {
-      copy_async<kElem * kVec>(tile + line * pitch + at, o.f64 + src, in);
+    for (int line = l0; line < lines_pad; line += kStep) {
+      const bool in = line < b.lines && b.len > 0;
+      copy_async<8>(dst + 1, in ? src + 1 : o.f64, in ? 8 : 0);
+      copy_async<8>(dst + kLen, in && last ? src + kLen : o.f64, in && last ? 8 : 0);
+      src += kStep * b.stride;
+      dst += kStep * kPitch;
     }
+    return;
+  }
+  const int bytes = left >= 2 ? 16 : left == 1 ? 8 : 0;
+#pragma unroll 4
+  for (int line = l0; line < lines_pad; line += kStep) {
+    const int n = line < b.lines ? bytes : 0;
+    copy_async<16>(dst, n ? src : o.f64 - odd_start(o, 0, 0, 0), n);
+    src += kStep * b.stride;
+    dst += kStep * kPitch;
   }
 }
 
-template <bool kPair, int kLen>
-__device__ __forceinline__ void stage_block(const DotOperand& o, const Block2d& b, int lines,
-                                            double* tile, int pitch, int vec) {
-  if (vec > 1) stage_lines<kPair, kLen, kPair ? 4 : 2>(o, b, lines, tile, pitch);
-  else stage_lines<kPair, kLen, 1>(o, b, lines, tile, pitch);
+// The same of DS pairs, kVec of them per copy.
+template <int kLen, int kPitch, int kVec, int kOperand>
+__device__ __forceinline__ void stage_pairs(const DotOperand& o, const Block2d& b, int lines_pad,
+                                            double* tile) {
+  constexpr int kWords = kLen / kVec, kStep = kThreads / kWords;
+  const int at = threadIdx.x % kWords * kVec;
+  float* f = reinterpret_cast<float*>(tile);
+#pragma unroll 4
+  for (int line = threadIdx.x / kWords; line < lines_pad; line += kStep) {
+    const bool in = line < b.lines && at < b.len;  // kVec divides len
+    const int64_t src = in ? b.origin + line * b.stride + at : 0;
+    const int n = in ? 4 * kVec : 0;
+    copy_async<4 * kVec>(f + line * kPitch + at, o.hi + src, n);
+    copy_async<4 * kVec>(f + kOperand + line * kPitch + at, o.lo + src, n);
+  }
 }
+
+template <bool kPair, int kLen, int kPitch, int kOperand>
+__device__ __forceinline__ void stage_block(const DotOperand& o, const Block2d& b, int lines_pad,
+                                            double* tile, int vec) {
+  if constexpr (!kPair) {
+    stage_f64<kLen, kPitch>(o, b, lines_pad, tile);
+  } else {
+    if (vec > 1) stage_pairs<kLen, kPitch, 4, kOperand>(o, b, lines_pad, tile);
+    else stage_pairs<kLen, kPitch, 1, kOperand>(o, b, lines_pad, tile);
+  }
+}
+
+// A thread's word of each line of an f64 operand through a unit: where it is, and
+// how it moves in a stage with all its contraction.  Lines are positions of the
+// contraction (kLinesK: [k][row]) or rows ([row][k]); values past the operand's
+// rows or columns are not staged, since their products are not stored.
+template <int kLen, int kPitch, bool kLinesK>
+struct Words {
+  static constexpr int kWords = kLen / 2, kStep = kThreads / kWords;
+  const double* src;  // of this stage
+  int bytes;          // 16; 8: half a word; 0: none; -1: the first and last value
+
+  // From `origin` on; len: rows or columns when they run along the lines.
+  __device__ __forceinline__ void start(const DotOperand& o, int64_t origin, int64_t stride,
+                                        int len) {
+    const int c = threadIdx.x % kWords, l0 = threadIdx.x / kWords;
+    const int odd = odd_start(o, origin, stride, l0), first = 2 * c - odd;
+    const int left = (kLinesK ? len : kLen) - first;
+    src = o.f64 + origin + l0 * stride + first;
+    bytes = first < 0 ? -1 : left >= 2 ? 16 : left == 1 ? 8 : 0;
+  }
+
+  // One whole stage of `lines` lines (kLinesK: kKS of them).
+  __device__ __forceinline__ void stage(double* tile, int64_t stride, int lines, int len) const {
+    if (bytes == 0) return;
+    const int l0 = threadIdx.x / kWords;
+    double* dst = tile + l0 * kPitch + threadIdx.x % kWords * 2;
+    const double* p = src;
+    const int64_t step = kStep * stride;
+    constexpr int kPasses = (kLinesK ? kKS : kSmallTile) / kStep;
+    if (bytes == 16) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        if (!kLinesK && l0 + i * kStep >= lines) break;
+        copy_async<16>(dst + i * kStep * kPitch, p, 16);
+        p += step;
+      }
+      return;
+    }
+#pragma unroll 1
+    for (int i = 0; i < kPasses; ++i) {
+      if (!kLinesK && l0 + i * kStep >= lines) break;
+      if (bytes == 8) {
+        copy_async<16>(dst, p, 8);
+      } else {
+        copy_async<8>(dst + 1, p + 1, 8);
+        if (!kLinesK || kLen - 1 < len) copy_async<8>(dst + kLen, p + kLen, 8);
+      }
+      p += step;
+      dst += kStep * kPitch;
+    }
+  }
+};
 
 struct SmallArgs {
   RaggedProblem q;
   RaggedPlan p;
   bool contract;
-  bool add;        // contraction: add to the result (a later window of rows)
-  int tiles_k;     // contraction: tiles of the result's rows
-  int tiles_n;
-  int splits;      // of the contraction (products only)
+  bool add;          // contraction: add to the result (a later window of rows)
+  uint32_t tiles_k;  // contraction: tiles of the result's rows
+  uint32_t tiles_n;
+  uint32_t splits;   // of the contraction (products only)
   int64_t split_k;
-  double* partial;  // [splits][M][N]
-  int vec_a, vec_b;  // values per copy
+  double* partial;   // [splits][M][N]
+  int vec_a, vec_b;  // DS pairs per copy
 };
 
 // A unit of work: an output tile over a range of the contraction.
 struct SmallUnit {
-  int64_t g, row, col;  // group, first output row (in the group's rows or matrix) and column
-  int rows, cols;
-  int64_t k0, k1;       // contraction range (contraction: rows of the call)
+  int g, rows, cols;
+  int64_t row, col;  // first output row (of the call, or of the group's matrix) and column
+  int64_t k0, k1;    // contraction range (contraction: rows of the call)
   int split;
-  int64_t id;           // of its output tile
 };
 
-__device__ __forceinline__ int64_t units_of(const SmallArgs& a) {
-  if (a.contract) return a.q.G * a.tiles_k * a.tiles_n;
-  return static_cast<int64_t>(a.p.small_start[a.q.G]) * a.tiles_n * a.splits;
+__device__ __forceinline__ uint32_t units_of(const SmallArgs& a) {
+  if (a.contract) return static_cast<uint32_t>(a.q.G) * a.tiles_k * a.tiles_n;
+  return static_cast<uint32_t>(a.p.small_start[a.q.G]) * a.tiles_n * a.splits;
 }
 
 // False for a unit that belongs to the tensor-core product, or that adds
 // nothing.
-__device__ __forceinline__ bool unit_at(const SmallArgs& a, int64_t u, SmallUnit& x) {
+__device__ __forceinline__ bool unit_at(const SmallArgs& a, uint32_t u, SmallUnit& x) {
   if (a.contract) {
-    const int64_t per = static_cast<int64_t>(a.tiles_k) * a.tiles_n;
-    x.g = u / per;
-    const int64_t r = u - x.g * per;
-    x.row = r / a.tiles_n * kSmallTile;
-    x.col = r % a.tiles_n * kTN;
-    x.k0 = a.p.row[x.g];
-    x.k1 = a.p.row[x.g + 1];
+    const uint32_t per = a.tiles_k * a.tiles_n, g = u / per, r = u - g * per, tk = r / a.tiles_n;
+    x.g = static_cast<int>(g);
+    x.row = static_cast<int64_t>(tk) * kSmallTile;
+    x.col = static_cast<int64_t>(r - tk * a.tiles_n) * kTN;
+    x.k0 = a.p.row[g];
+    x.k1 = a.p.row[g + 1];
     x.rows = a.q.K - x.row < kSmallTile ? static_cast<int>(a.q.K - x.row) : kSmallTile;
     x.split = 0;
-    x.id = u;
     if (x.k1 - x.k0 >= a.p.tensor_rows || (a.add && x.k1 == x.k0)) return false;
   } else {
-    const int64_t n = a.p.small_start[a.q.G];
-    const int64_t rest = u / n;
+    const uint32_t n = a.p.small_start[a.q.G], rest = u / n, tn = rest / a.splits;
     const RaggedTile t = a.p.small[u - rest * n];
     x.g = t.group;
     x.row = t.row;
     x.rows = t.rows;
-    x.split = static_cast<int>(rest % a.splits);
-    const int64_t tn = rest / a.splits;
-    x.col = tn * kTN;
+    x.split = static_cast<int>(rest - tn * a.splits);
+    x.col = static_cast<int64_t>(tn) * kTN;
     x.k0 = x.split * a.split_k;
     x.k1 = x.k0 + a.split_k < a.q.K ? x.k0 + a.split_k : a.q.K;
-    x.id = tn * n + (u - rest * n);
   }
   x.cols = a.q.N - x.col < kTN ? static_cast<int>(a.q.N - x.col) : kTN;
   return true;
 }
 
+// First value of each operand at contraction position k.
+__device__ __forceinline__ int64_t origin_a(const SmallArgs& a, const SmallUnit& x, int64_t k) {
+  return x.row * a.q.lhs.s_r + k * a.q.lhs.s_k;
+}
+__device__ __forceinline__ int64_t origin_b(const SmallArgs& a, const SmallUnit& x, int64_t k) {
+  return (a.contract ? 0 : x.g * a.q.rhs.s_b) + x.col * a.q.rhs.s_r + k * a.q.rhs.s_k;
+}
+
 // kA: A is staged as [k][row] (its rows are contiguous) rather than [row][k];
 // kB: B as [k][column] rather than [column][k].
-template <bool kPair, bool kA, bool kB>
+template <bool kPair, bool kA, bool kB, int kRows>
 __device__ __forceinline__ void stage_unit(const SmallArgs& a, const SmallUnit& x, int64_t k,
                                            double* sa, double* sb) {
   const int kn = x.k1 - k < kKS ? static_cast<int>(x.k1 - k) : kKS;
-  const RaggedProblem& q = a.q;
-  [[maybe_unused]] const int rows_pad = x.rows <= 16 ? 16 : kSmallTile;
-  Block2d A, B;
+  const DotOperand &A = a.q.lhs, &B = a.q.rhs;
+  const int64_t oa = origin_a(a, x, k), ob = origin_b(a, x, k);
+  constexpr int kOperandA = Stages<kRows>::kOperandA;
   if constexpr (kA) {
-    A = Block2d{x.row + k * q.lhs.s_k, q.lhs.s_k, kn, x.rows};
-    stage_block<kPair, kSmallTile>(q.lhs, A, kKS, sa, kPitchN, a.vec_a);
+    stage_block<kPair, kSmallTile, kPitchN, kOperandA>(A, Block2d{oa, A.s_k, kn, x.rows}, kKS, sa,
+                                                       a.vec_a);
   } else {
-    A = Block2d{x.row * q.lhs.s_r + k, q.lhs.s_r, x.rows, kn};
-    stage_block<kPair, kKS>(q.lhs, A, rows_pad, sa, kPitchK, a.vec_a);
+    const int pad = x.rows <= 16 ? 16 : x.rows <= 32 ? 32 : kSmallTile;
+    stage_block<kPair, kKS, kPitchK, kOperandA>(A, Block2d{oa, A.s_r, x.rows, kn}, pad, sa,
+                                                a.vec_a);
   }
-  const int64_t base = a.contract ? 0 : x.g * q.rhs.s_b;
-  if constexpr (kB) {
-    B = Block2d{base + k * q.rhs.s_k + x.col, q.rhs.s_k, kn, x.cols};
-    stage_block<kPair, kTN>(q.rhs, B, kKS, sb, kPitchN, a.vec_b);
-  } else {
-    B = Block2d{base + x.col * q.rhs.s_r + k, q.rhs.s_r, x.cols, kn};
-    stage_block<kPair, kKS>(q.rhs, B, kTN, sb, kPitchK, a.vec_b);
-  }
+  if constexpr (kB)
+    stage_block<kPair, kTN, kPitchN, kOperandB>(B, Block2d{ob, B.s_k, kn, x.cols}, kKS, sb,
+                                                a.vec_b);
+  else
+    stage_block<kPair, kKS, kPitchK, kOperandB>(B, Block2d{ob, B.s_r, x.cols, kn}, kTN, sb,
+                                                a.vec_b);
 }
 
 // The products of one stage: warps stand kWM x (8 / kWM), each with MF x NF
-// fragments.
-template <bool kPair, bool kA, bool kB, int MF, int NF, int kWM>
-__device__ __forceinline__ void multiply_stage(const double* sa, const double* sb, int kn,
-                                               double (&acc)[4][2][2]) {
+// 8 x 8 accumulators.  odd_a, odd_b: where this lane's lines of A and B start
+// (odd_start; the same for all its lines, which are an even number apart).
+template <bool kFull, bool kPair, bool kA, bool kB, int kRows, int MF, int NF, int kWM>
+__device__ __forceinline__ void multiply_part(const double* sa, const double* sb, int kn, int odd_a,
+                                              int odd_b, double (&acc)[4][2][2]) {
+  constexpr int kOperandA = Stages<kRows>::kOperandA;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int wm = warp % kWM * MF * 8, wn = warp / kWM * NF * 8;
   const int r = lane >> 2, kk = lane & 3;
-#pragma unroll 4
-  for (int k = 0; k < kn; k += 4) {
-    double fa[MF], fb[NF];
+  const int ia = odd_a + (kA ? kk * kPitchN + wm + r : (wm + r) * kPitchK + kk);
+  const int ib = odd_b + (kB ? kk * kPitchN + wn + r : (wn + r) * kPitchK + kk);
+  auto value_a = [&](int i, int k) {
+    return staged<kPair, kOperandA>(sa, ia + (kA ? k * kPitchN + i * 8 : i * 8 * kPitchK + k));
+  };
+  auto value_b = [&](int j, int k) {
+    return staged<kPair, kOperandB>(sb, ib + (kB ? k * kPitchN + j * 8 : j * 8 * kPitchK + k));
+  };
+  if constexpr (MF == 1) {
+    // one accumulator would chain the instructions: four take turns, added up
+    // at the end (finish_few)
 #pragma unroll
-    for (int i = 0; i < MF; ++i)
-      fa[i] = staged<kPair>(sa, kA ? (k + kk) * kPitchN + wm + i * 8 + r
-                                   : (wm + i * 8 + r) * kPitchK + k + kk);
+    for (int k = 0; k < kKS; k += 4) {
+      if (!kFull && k >= kn) break;
+      mma_f64(acc[k / 4 % 4][0], value_a(0, k), value_b(0, k));
+    }
+  } else {
 #pragma unroll
-    for (int j = 0; j < NF; ++j)
-      fb[j] = staged<kPair>(sb, kB ? (k + kk) * kPitchN + wn + j * 8 + r
-                                   : (wn + j * 8 + r) * kPitchK + k + kk);
+    for (int k = 0; k < kKS; k += 8) {
+      if (!kFull && k >= kn) break;
+      double fa[MF / 2][4], fb[NF][2];
 #pragma unroll
-    for (int i = 0; i < MF; ++i)
+      for (int i = 0; i < MF / 2; ++i)
 #pragma unroll
-      for (int j = 0; j < NF; ++j) mma_f64(acc[i][j], fa[i], fb[j]);
+        for (int e = 0; e < 4; ++e) fa[i][e] = value_a(2 * i + e % 2, k + 4 * (e / 2));
+#pragma unroll
+      for (int j = 0; j < NF; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) fb[j][e] = value_b(j, k + 4 * e);
+      if constexpr (MF == 2 && NF == 1) {
+        constexpr int kTurn = 8;
+        mma_f64_wide(acc[2 * (k / kTurn % 2)][0], acc[2 * (k / kTurn % 2) + 1][0], fa[0], fb[0]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < MF / 2; ++i)
+#pragma unroll
+          for (int j = 0; j < NF; ++j)
+            mma_f64_wide(acc[2 * i][j], acc[2 * i + 1][j], fa[i], fb[j]);
+      }
+    }
+  }
+}
+
+template <bool kPair, bool kA, bool kB, int kRows, int MF, int NF, int kWM>
+__device__ __forceinline__ void multiply_stage(const double* sa, const double* sb, int kn,
+                                               int odd_a, int odd_b, double (&acc)[4][2][2]) {
+  if (kn == kKS)
+    multiply_part<true, kPair, kA, kB, kRows, MF, NF, kWM>(sa, sb, kn, odd_a, odd_b, acc);
+  else
+    multiply_part<false, kPair, kA, kB, kRows, MF, NF, kWM>(sa, sb, kn, odd_a, odd_b, acc);
+}
+
+// The accumulators that took turns, added up in order.
+template <int MF>
+__device__ __forceinline__ void finish_few(double (&acc)[4][2][2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (MF == 1) {
+      acc[0][0][h] = __dadd_rn(__dadd_rn(acc[0][0][h], acc[1][0][h]),
+                               __dadd_rn(acc[2][0][h], acc[3][0][h]));
+    } else {
+      acc[0][0][h] = __dadd_rn(acc[0][0][h], acc[2][0][h]);
+      acc[1][0][h] = __dadd_rn(acc[1][0][h], acc[3][0][h]);
+    }
   }
 }
 
@@ -345,36 +512,39 @@ __device__ __forceinline__ void store_unit(const SmallArgs& a, const SmallUnit& 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int wm = warp % kWM * MF * 8, wn = warp / kWM * NF * 8;
   const int64_t first = (a.contract ? x.g * a.q.K : 0) + x.row;
+  DotResult out = a.q.out;
+  if (a.splits > 1) out = DotResult{a.partial + x.split * a.q.M * a.q.N, nullptr, nullptr};
+  const bool words = out.f64 && (a.q.N & 1) == 0 && (reinterpret_cast<uintptr_t>(out.f64) & 15) == 0;
 #pragma unroll
   for (int i = 0; i < MF; ++i) {
     const int r = wm + i * 8 + (lane >> 2);
     if (r >= x.rows) continue;
-    const int64_t row = (first + r) * a.q.N + x.col;
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
+      const int c = wn + j * 8 + 2 * (lane & 3);
+      const int64_t at = (first + r) * a.q.N + x.col + c;
+      double v[2] = {acc[i][j][0], acc[i][j][1]};
+      if (words && !a.add && c + 2 <= x.cols) {
+        *reinterpret_cast<double2*>(out.f64 + at) = make_double2(v[0], v[1]);
+        continue;
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int c = wn + j * 8 + 2 * (lane & 3) + h;
-        if (c >= x.cols) continue;
-        double v = acc[i][j][h];
-        if (a.splits > 1) {
-          a.partial[static_cast<int64_t>(x.split) * a.q.M * a.q.N + row + c] = v;
-          continue;
-        }
-        if (a.add) v = __dadd_rn(result_value(a.q.out, row + c), v);
-        put(a.q.out, row + c, v);
+        if (c + h >= x.cols) continue;
+        if (a.add) v[h] = __dadd_rn(result_value(out, at + h), v[h]);
+        put(out, at + h, v[h]);
       }
     }
   }
 }
 
 // Blocks stay and take every gridDim.x-th unit; the pipeline of stages runs on
-// across units.
-template <bool kPair, bool kA, bool kB>
+// across units.  kRows: most rows of a tile.
+template <bool kPair, bool kA, bool kB, int kRows>
 __global__ void __launch_bounds__(kThreads, 2)
 small_kernel(const __grid_constant__ SmallArgs a) {
+  using St = Stages<kRows>;
   extern __shared__ __align__(16) double stage[];
-  __shared__ int s_last;
   wait_previous_grid();
   // rows behind the last group
   if (!a.contract) {
@@ -384,88 +554,132 @@ small_kernel(const __grid_constant__ SmallArgs a) {
          i < end; i += static_cast<int64_t>(gridDim.x) * kThreads)
       put(a.q.out, i, 0.0);
   }
-  const int64_t units = units_of(a);
-  auto next_unit = [&](int64_t u, SmallUnit& x) {
+  const uint32_t units = units_of(a);
+  auto next_unit = [&](uint32_t u, SmallUnit& x) {
     while (u < units && !unit_at(a, u, x)) u += gridDim.x;
     return u;
   };
-  // loading runs kStages - 1 stages ahead of multiplying
+  // loading runs kCount - 1 stages ahead of multiplying
+  const DotOperand &A = a.q.lhs, &B = a.q.rhs;
+  const int64_t line_a = kA ? A.s_k : A.s_r, line_b = kB ? B.s_k : B.s_r;
+  Words<kA ? kSmallTile : kKS, kA ? kPitchN : kPitchK, kA> wa;
+  Words<kB ? kTN : kKS, kB ? kPitchN : kPitchK, kB> wb;
   SmallUnit lx, x;
-  int64_t lu = next_unit(blockIdx.x, lx);
-  int64_t lk = lu < units ? lx.k0 : 0;
+  uint32_t lu = blockIdx.x;
+  int64_t lk = 0;
+  auto start_unit = [&](uint32_t u) {
+    lu = next_unit(u, lx);
+    if (lu >= units) return;
+    lk = lx.k0;
+    if constexpr (!kPair) {
+      wa.start(A, origin_a(a, lx, lk), line_a, lx.rows);
+      wb.start(B, origin_b(a, lx, lk), line_b, lx.cols);
+    }
+  };
+  start_unit(blockIdx.x);
   int ls = 0;
   auto load_one = [&] {
     if (lu < units) {
-      double* sa = stage + ls * 2 * kOperand;
-      if (lk < lx.k1) stage_unit<kPair, kA, kB>(a, lx, lk, sa, sa + kOperand);
+      double* sa = stage + ls * St::kStride;
+      double* sb = sa + St::kOperandA;
+      if (!kPair && lk + kKS <= lx.k1) {
+        wa.stage(sa, line_a, lx.rows, lx.rows);
+        wb.stage(sb, line_b, lx.cols, lx.cols);
+      } else if (lk < lx.k1) {
+        stage_unit<kPair, kA, kB, kRows>(a, lx, lk, sa, sb);
+      }
       lk += kKS;
       if (lk >= lx.k1) {
-        lu = next_unit(lu + gridDim.x, lx);
-        if (lu < units) lk = lx.k0;
+        start_unit(lu + gridDim.x);
+      } else if constexpr (!kPair) {
+        wa.src += kKS * A.s_k;
+        wb.src += kKS * B.s_k;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    ls = ls + 1 == kStages ? 0 : ls + 1;
+    ls = ls + 1 == St::kCount ? 0 : ls + 1;
   };
 #pragma unroll 1
-  for (int i = 0; i < kStages - 1; ++i) load_one();
+  for (int i = 0; i < St::kCount - 1; ++i) load_one();
   int cs = 0;
+  const int lane = threadIdx.x & 31;
 #pragma unroll 1
-  for (int64_t u = next_unit(blockIdx.x, x); u < units; u = next_unit(u + gridDim.x, x)) {
+  for (uint32_t u = next_unit(blockIdx.x, x); u < units; u = next_unit(u + gridDim.x, x)) {
     double acc[4][2][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) acc[i][j][0] = acc[i][j][1] = 0.0;
+    int odd_a = 0, odd_b = 0;
+    if constexpr (!kPair) {
+      odd_a = kA ? odd_start(a.q.lhs, origin_a(a, x, x.k0), a.q.lhs.s_k, lane & 3)
+                 : odd_start(a.q.lhs, origin_a(a, x, x.k0), a.q.lhs.s_r, lane >> 2);
+      odd_b = kB ? odd_start(a.q.rhs, origin_b(a, x, x.k0), a.q.rhs.s_k, lane & 3)
+                 : odd_start(a.q.rhs, origin_b(a, x, x.k0), a.q.rhs.s_r, lane >> 2);
+    }
     int64_t k = x.k0;
     do {  // a unit without contraction takes one (empty) stage
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(St::kCount - 2) : "memory");
       __syncthreads();
-      const double* sa = stage + cs * 2 * kOperand;
+      const double* sa = stage + cs * St::kStride;
+      const double* sb = sa + St::kOperandA;
       const int kn = x.k1 - k < kKS ? static_cast<int>(x.k1 - k) : kKS;
       load_one();
-      if (x.rows <= 16) multiply_stage<kPair, kA, kB, 2, 1, 1>(sa, sa + kOperand, kn, acc);
-      else multiply_stage<kPair, kA, kB, 4, 2, 2>(sa, sa + kOperand, kn, acc);
-      cs = cs + 1 == kStages ? 0 : cs + 1;
+      if (x.rows <= 8)
+        multiply_stage<kPair, kA, kB, kRows, 1, 1, 1>(sa, sb, kn, odd_a, odd_b, acc);
+      else if (kRows == 16 || x.rows <= 16)
+        multiply_stage<kPair, kA, kB, kRows, 2, 1, 1>(sa, sb, kn, odd_a, odd_b, acc);
+      else if (x.rows <= 32)
+        multiply_stage<kPair, kA, kB, kRows, 2, 2, 2>(sa, sb, kn, odd_a, odd_b, acc);
+      else
+        multiply_stage<kPair, kA, kB, kRows, 4, 2, 2>(sa, sb, kn, odd_a, odd_b, acc);
+      cs = cs + 1 == St::kCount ? 0 : cs + 1;
       k += kKS;
     } while (k < x.k1);
-    if (x.rows <= 16) store_unit<2, 1, 1>(a, x, acc);
+    if (x.rows <= 8) {
+      finish_few<1>(acc);
+      store_unit<1, 1, 1>(a, x, acc);
+    } else if (kRows == 16 || x.rows <= 16) {
+      finish_few<2>(acc);
+      store_unit<2, 1, 1>(a, x, acc);
+    } else if (x.rows <= 32) store_unit<2, 2, 2>(a, x, acc);
     else store_unit<4, 2, 2>(a, x, acc);
-    if (a.splits > 1) {
-      // the last of a tile's splits adds them up in order
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) s_last = atomicAdd(a.p.counter + x.id, 1) == a.splits - 1;
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        for (int e = threadIdx.x; e < x.rows * x.cols; e += kThreads) {
-          const int64_t at = (x.row + e / x.cols) * a.q.N + x.col + e % x.cols;
-          double v = 0.0;
-          for (int s = 0; s < a.splits; ++s)
-            v = __dadd_rn(v, __ldcg(a.partial + static_cast<int64_t>(s) * a.q.M * a.q.N + at));
-          put(a.q.out, at, v);
-        }
-      }
-      __syncthreads();
-    }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// The splits of every small tile (blockIdx.y) added up in order.
+__global__ void __launch_bounds__(kThreads)
+small_sum_kernel(const __grid_constant__ SmallArgs a) {
+  wait_previous_grid();
+  if (static_cast<int>(blockIdx.y) >= a.p.small_start[a.q.G]) return;
+  const RaggedTile t = a.p.small[blockIdx.y];
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (c >= a.q.N) return;
+  const int64_t plane = a.q.M * a.q.N;
+  for (int r = blockIdx.z; r < t.rows; r += gridDim.z) {
+    const int64_t at = (t.row + r) * a.q.N + c;
+    double v = 0.0;
+#pragma unroll 4
+    for (uint32_t s = 0; s < a.splits; ++s) v = __dadd_rn(v, __ldcg(a.partial + s * plane + at));
+    put(a.q.out, at, v);
+  }
 }
 
 // ---- host ------------------------------------------------------------------------
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Contraction splits of the products: enough units for about four per
-// resident block when the rows are few, each of at least kSplitMin.  From the
-// call's sizes alone, so a row's rounding does not depend on other groups.
-constexpr int64_t kSplitMin = 128;
+// Contraction splits of the products: with few rows, units of at least kSplitMin
+// of the contraction, enough of them for kSplitUnits.  From the call's sizes
+// alone, so a row's rounding does not depend on other groups.
+constexpr int64_t kSplitMin = 128, kSplitUnits = 2400;
 constexpr int kMaxSplits = 16;
 
 int splits_of(int64_t M, int64_t K, int64_t N, int64_t G) {
   const int64_t tiles = (M / kSmallTile + (G < M ? G : M)) * ceil_div(N, kTN);
-  int64_t s = tiles > 0 ? ceil_div(1184, tiles) : 1;
+  if (tiles == 0 || tiles >= kSplitUnits / 2) return 1;
+  int64_t s = ceil_div(kSplitUnits, tiles);
   const int64_t most = K / kSplitMin;
   s = s > most ? most : s;
   s = s > kMaxSplits ? kMaxSplits : s;
@@ -480,9 +694,8 @@ bool tensor_allowed(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
 }
 
 struct Layout {
-  size_t row, small_start, tensor_start, slot, small, tensor, slot_group, slot_bits, counter,
-      partial, tensor_ws, total;
-  int64_t small_cap, tensor_cap, slots, counters;
+  size_t row, small_start, tensor_start, slot, small, tensor, slot_group, slot_bits, partial, tensor_ws, total;
+  int64_t small_cap, tensor_cap, slots;
   int splits;
   bool tensor_ok;
 };
@@ -504,7 +717,6 @@ Layout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
     l.tensor_cap = ragged_tensor_tiles(rows, G);
   }
   l.splits = contract ? 1 : splits_of(M, K, N, G);
-  l.counters = l.splits > 1 ? l.small_cap * ceil_div(N, kTN) : 0;
   l.row = take((G + 1) * 4);
   l.small_start = take((G + 1) * 4);
   l.tensor_start = take((G + 1) * 4);
@@ -513,7 +725,6 @@ Layout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
   l.tensor = take(l.tensor_cap * sizeof(RaggedTile));
   l.slot_group = take(l.slots * 4);
   l.slot_bits = take(l.slots * 4);
-  l.counter = take(l.counters * 4);
   l.partial = take(l.splits > 1 ? static_cast<size_t>(l.splits) * M * N * 8 : 0);
   l.tensor_ws = take(l.tensor_ok ? ragged_tensor_bytes(M, K, N, G, contract) : 0);
   // the tensor-core part is aligned to 1024 whatever the workspace's start
@@ -557,24 +768,22 @@ RaggedPlan plan_at(const Layout& l, int64_t G, uint8_t* ws, bool tensor) {
   p.slot_bits = ints(l.slot_bits);
   p.small_cap = l.small_cap;
   p.tensor_cap = l.tensor_cap;
-  p.counter = ints(l.counter);
-  p.counters = l.counters;
   p.tensor_rows = tensor ? kTensorRows : INT32_MAX;
   if (tensor)
     for (int i = 0; i < kBitsLimits; ++i) p.bits_limit[i] = bits_limits()[i];
   return p;
 }
 
-// Values per copy of an operand whose lines are `len` values long at a stride
-// of `stride` values, from `origin` on.
+// DS pairs per copy of an operand whose lines are `len` values long at a stride
+// of `stride` values.
 int copy_width(const DotOperand& o, int64_t len, int64_t stride, int64_t batch) {
-  const int wide = o.f64 ? 2 : 4;
-  const bool at = o.f64 ? aligned(o.f64, 16) : aligned(o.hi, 16) && aligned(o.lo, 16);
-  return at && len % wide == 0 && stride % wide == 0 && batch % wide == 0 ? wide : 1;
+  const bool at = aligned(o.hi, 16) && aligned(o.lo, 16);
+  return at && len % 4 == 0 && stride % 4 == 0 && batch % 4 == 0 ? 4 : 1;
 }
 
-template <bool kPair, bool kA, bool kB>
+template <bool kPair, bool kA, bool kB, int kRows>
 int launch_small(const SmallArgs& a, int64_t most_units, cudaStream_t s) {
+  constexpr size_t kBytes = Stages<kRows>::kBytes;
   static std::mutex mu;
   static std::vector<bool> done;
   int dev = 0;
@@ -583,12 +792,14 @@ int launch_small(const SmallArgs& a, int64_t most_units, cudaStream_t s) {
     std::lock_guard<std::mutex> lock(mu);
     if (dev >= static_cast<int>(done.size())) done.resize(dev + 1, false);
     if (!done[dev]) {
-      DSB_CUDA_TRY(cudaFuncSetAttribute(small_kernel<kPair, kA, kB>,
+      DSB_CUDA_TRY(cudaFuncSetAttribute(small_kernel<kPair, kA, kB, kRows>,
                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        static_cast<int>(kSmallBytes)));
+                                        static_cast<int>(kBytes)));
       done[dev] = true;
     }
   }
+  if (most_units > 0x7fffffff)
+    return set_error(DS_INVALID_ARGUMENT, "ds_ragged_dot: too many output tiles");
   const int64_t resident = 2 * static_cast<int64_t>(sm_count());
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -597,12 +808,31 @@ int launch_small(const SmallArgs& a, int64_t most_units, cudaStream_t s) {
   cfg.gridDim = dim3(static_cast<unsigned>(most_units < resident ? (most_units < 1 ? 1 : most_units)
                                                                  : resident));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmallBytes;
+  cfg.dynamicSmemBytes = kBytes;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  DSB_CUDA_TRY(cudaLaunchKernelEx(&cfg, small_kernel<kPair, kA, kB>, a));
+  DSB_CUDA_TRY(cudaLaunchKernelEx(&cfg, small_kernel<kPair, kA, kB, kRows>, a));
+  if (a.splits > 1) {
+    const int64_t rows = a.q.M < 8 ? a.q.M : 8;
+    DSB_CUDA_TRY(launch_dependent(small_sum_kernel,
+                                  dim3(static_cast<unsigned>(ceil_div(a.q.N, kThreads)),
+                                       static_cast<unsigned>(a.p.small_cap),
+                                       static_cast<unsigned>(rows)),
+                                  dim3(kThreads), s, a));
+  }
   return launch_status();
+}
+
+template <bool kB>
+int launch_products(const SmallArgs& a, int64_t units, cudaStream_t s) {
+  // no group has more rows than the call
+  const bool few = a.q.M <= 16;
+  if (a.q.lhs.f64)
+    return few ? launch_small<false, false, kB, 16>(a, units, s)
+               : launch_small<false, false, kB, kSmallTile>(a, units, s);
+  return few ? launch_small<true, false, kB, 16>(a, units, s)
+             : launch_small<true, false, kB, kSmallTile>(a, units, s);
 }
 
 int launch_prep(const RaggedProblem& q, int64_t begin, int64_t end, const RaggedPlan& p,
@@ -628,9 +858,9 @@ int ragged_dot(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) 
   SmallArgs a{};
   a.q = q;
   a.p = plan_at(l, q.G, ws, clusters > 0);
-  a.tiles_n = static_cast<int>(ceil_div(q.N, kTN));
-  a.splits = l.splits;
-  a.split_k = ceil_div(ceil_div(q.K, a.splits), kKS) * kKS;
+  a.tiles_n = static_cast<uint32_t>(ceil_div(q.N, kTN));
+  a.splits = static_cast<uint32_t>(l.splits);
+  a.split_k = ceil_div(ceil_div(q.K, l.splits), kKS) * kKS;
   a.partial = reinterpret_cast<double*>(ws + l.partial);
   a.vec_a = copy_width(q.lhs, q.K, q.lhs.s_r, 0);
   a.vec_b = copy_width(q.rhs, q.rhs_t ? q.K : q.N, q.rhs_t ? q.rhs.s_r : q.rhs.s_k, q.rhs.s_b);
@@ -639,12 +869,7 @@ int ragged_dot(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) 
     if (int st = ragged_tensor_dot(q, a.p, ws + l.tensor_ws, clusters, s)) return st;
   ProfileScope prof("ragged_small", s);
   const int64_t units = l.small_cap * a.tiles_n * a.splits;
-  const bool pair = q.lhs.f64 == nullptr;
-  if (q.rhs_t)
-    return pair ? launch_small<true, false, false>(a, units, s)
-                : launch_small<false, false, false>(a, units, s);
-  return pair ? launch_small<true, false, true>(a, units, s)
-              : launch_small<false, false, true>(a, units, s);
+  return q.rhs_t ? launch_products<false>(a, units, s) : launch_products<true>(a, units, s);
 }
 
 size_t ragged_contract_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G) {
@@ -662,8 +887,8 @@ int ragged_contract(const RaggedProblem& q, void* workspace, size_t, cudaStream_
   a.q = q;
   a.p = plan_at(l, q.G, ws, clusters > 0);
   a.contract = true;
-  a.tiles_k = static_cast<int>(ceil_div(q.K, kSmallTile));
-  a.tiles_n = static_cast<int>(ceil_div(q.N, kTN));
+  a.tiles_k = static_cast<uint32_t>(ceil_div(q.K, kSmallTile));
+  a.tiles_n = static_cast<uint32_t>(ceil_div(q.N, kTN));
   a.splits = 1;
   a.vec_a = copy_width(q.lhs, q.K, q.lhs.s_k, 0);
   a.vec_b = copy_width(q.rhs, q.N, q.rhs.s_k, 0);
@@ -676,8 +901,8 @@ int ragged_contract(const RaggedProblem& q, void* workspace, size_t, cudaStream_
     if (clusters > 0)
       if (int st = ragged_tensor_contract(q, a.p, a.add, ws + l.tensor_ws, clusters, s)) return st;
     ProfileScope prof("ragged_small", s);
-    const int st = q.lhs.f64 == nullptr ? launch_small<true, true, true>(a, units, s)
-                                        : launch_small<false, true, true>(a, units, s);
+    const int st = q.lhs.f64 == nullptr ? launch_small<true, true, true, kSmallTile>(a, units, s)
+                                        : launch_small<false, true, true, kSmallTile>(a, units, s);
     if (st) return st;
   }
   return ok();

@@ -53,8 +53,6 @@ struct RaggedPlan {
   int32_t* slot_group;    // of each large group: its number among all,
   int32_t* slot_bits;     // and the bits its rows allow as a contraction
   int64_t small_cap, tensor_cap;
-  int32_t* counter;       // cleared
-  int64_t counters;
   int64_t tensor_rows;    // a group of as many rows is large
   int32_t bits_limit[kBitsLimits];
 };
