@@ -15,6 +15,7 @@ once per shape.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 from dataclasses import dataclass
 from typing import Dict, Tuple
@@ -283,7 +284,7 @@ def _make_call(target_name: str, result_shape_dtypes):
 
     def _invoke(args, attrs, device, out):
         if conv.kind in _SEQUENCE_KINDS:
-            outs = _invoke_sequence(target_name, conv, fn, results_spec, args, attrs, device, out)
+            outs = _invoke_sequence(target_name, sym, conv, results_spec, args, attrs, device, out)
             return outs[0] if single else tuple(outs)
         outs = out if out is not None else [
             torch.empty(s.shape, dtype=s.dtype, device=device) for s in results_spec]
@@ -372,58 +373,141 @@ def _make_call(target_name: str, result_shape_dtypes):
 
 _SEQUENCE_KINDS = ("scan", "ragged", "ragged_contract")
 _SCAN_TYPES = {"f64": _lib.DS_FUSED_F64, "f32": _lib.DS_FUSED_F32, "packed": _lib.DS_FUSED_PACKED}
-# workspace sizes of the recurrences and grouped products, by (target, device,
-# operand shapes, rhs_contracting)
-_sequence_ws: Dict[tuple, int] = {}
 
 
-def _invoke_sequence(target_name, conv, fn, results_spec, args, attrs, device, out):
+class _Plan:
+    """What a recurrence or grouped product of given shapes needs of each call:
+    built on its first call, read-only afterwards."""
+    __slots__ = ("fn", "dtypes", "present", "dims", "specs", "workspace", "attr", "keep")
+
+
+# (entry point, device index, rhs_contracting, operand shapes...) -> _Plan
+_plans: Dict[tuple, _Plan] = {}
+_fast_fns: Dict[str, object] = {}
+
+
+def _fast_fn(sym, kind, n):
+    """The entry point with every descriptor passed as an address: three words
+    (data, dims, rank) in one array for the whole call."""
+    fn = _fast_fns.get(sym)
+    if fn is None:
+        fn = _lib.lib()[sym]  # a function object of its own
+        argtypes = [ctypes.c_void_p] * n
+        if kind == "ragged":
+            argtypes.insert(n - len(CONVENTIONS[sym].results), ctypes.c_int32)
+        fn.argtypes = argtypes + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+        _fast_fns[sym] = fn
+    return fn
+
+
+def _make_plan(sym, conv, args, specs, contracting):
+    plan = _Plan()
+    L = _lib.lib()
+    plan.dtypes = conv.args
+    plan.present = tuple(t is not None for t in args)
+    plan.keep, plan.dims = [], []
+    for shape in [None if t is None else tuple(t.shape) for t in args] + [s.shape for s in specs]:
+        if shape is None:
+            plan.dims.append(None)
+            continue
+        _, d = _lib.make_buffer(0, shape)
+        plan.keep.append(d)  # the dims the plan's addresses point into
+        plan.dims.append((ctypes.addressof(d), len(shape)))
+    plan.specs = [(s.shape, s.dtype) for s in specs]
+    plan.attr = contracting if conv.kind == "ragged" else None
+
+    def ref(t):
+        b, d = _lib.make_buffer(t.data_ptr(), t.shape)
+        plan.keep.append((b, d))
+        return ctypes.byref(b)
+
+    if conv.kind == "scan":
+        plan.workspace = L.ds_linear_recurrence_workspace_size(
+            ref(args[0]), _SCAN_TYPES[sym.rsplit("_", 1)[1]])
+    elif conv.kind == "ragged":
+        plan.workspace = L.ds_ragged_dot_workspace_size(ref(args[0]), ref(args[-2]), contracting)
+    else:
+        plan.workspace = L.ds_ragged_dot_contract_workspace_size(ref(args[0]), ref(args[-2]),
+                                                                 ref(args[-1]))
+    plan.fn = _fast_fn(sym, conv.kind, len(plan.dims))
+    return plan
+
+
+def _invoke_sequence(target_name, sym, conv, specs, args, attrs, device, out):
+    """One call of a recurrence or grouped product on checked operands."""
     for i, t in enumerate(args):
         if t is not None and t.device != device:
             raise ValueError(f"{target_name} operand {i}: operands must be on one device")
+    for i, t in enumerate(out or ()):
+        if t.device != device:
+            raise ValueError(f"{target_name} result {i}: results must be on the operands' device")
+    contracting = int(attrs.get("rhs_contracting", 1))
+    key = _plan_key(sym, device.index, contracting, args)
+    plan = _plans.get(key)
+    if plan is None or plan.specs != [(s.shape, s.dtype) for s in specs]:
+        plan = _make_plan(sym, conv, args, specs, contracting)
+    outs = _run_plan(target_name, plan, args, device.index, out)
+    if len(_plans) > 512:
+        _plans.clear()
+    _plans[key] = plan  # the call was accepted
+    return outs
+
+
+def _plan_key(sym, index, contracting, args):
+    return (sym, index, contracting, *[None if t is None else t.shape for t in args])
+
+
+def _run_plan(target_name, plan, args, index, out):
     if out is None:
-        out = [torch.empty(s.shape, dtype=s.dtype, device=device) for s in results_spec]
-    else:
-        for i, t in enumerate(out):
-            if t.device != device:
-                raise ValueError(f"{target_name} result {i}: results must be on the operands' device")
-    keep = []
-
-    def ref(t):
-        if t is None:
-            return None
-        b, d = _lib.make_buffer(t.data_ptr(), t.shape)
-        keep.append((b, d))
-        return ctypes.byref(b)
-
-    refs = [ref(t) for t in args]
-    tail = [ref(t) for t in out]
-    L = _lib.lib()
-    if conv.kind == "scan":
-        key = (target_name, device.index, args[0].shape)
-    else:
-        contracting = int(attrs.get("rhs_contracting", 1))
-        key = (target_name, device.index, args[0].shape, args[-2].shape, args[-1].shape,
-               contracting)
-        if conv.kind == "ragged":
-            tail.insert(0, contracting)
-    ws_bytes = _sequence_ws.get(key)
-    if ws_bytes is None:
-        if conv.kind == "scan":
-            ws_bytes = L.ds_linear_recurrence_workspace_size(
-                refs[0], _SCAN_TYPES[fn.__name__.rsplit("_", 1)[1]])
-        elif conv.kind == "ragged":
-            ws_bytes = L.ds_ragged_dot_workspace_size(refs[0], refs[-2], contracting)
+        first = args[0]
+        out = [first.new_empty(shape, dtype=dtype) for shape, dtype in plan.specs]
+    words = []
+    for t, d in zip((*args, *out), plan.dims):
+        if d is None:
+            words += (0, 0, 0)
         else:
-            ws_bytes = L.ds_ragged_dot_contract_workspace_size(refs[0], refs[-2], refs[-1])
-        if len(_sequence_ws) > 1024:
-            _sequence_ws.clear()
-        _sequence_ws[key] = ws_bytes
-    stream = _lib.current_stream_ptr(device)
-    ws = _workspace(ws_bytes, device, stream) if ws_bytes else None
-    wsp = None if ws is None else ws.data_ptr()
-    _lib.check(fn(*refs, *tail, wsp, ws_bytes, stream), target_name)
+            words += (t.data_ptr(), d[0], d[1])
+    table = array.array("Q", words)
+    at = table.buffer_info()[0]
+    pointers = [at + 24 * i if d is not None else None for i, d in enumerate(plan.dims)]
+    if plan.attr is not None:
+        pointers.insert(len(args), plan.attr)
+    stream = _lib.current_stream_ptr(index)
+    ws, wsp = None, None
+    if plan.workspace:
+        ws = _workspace(plan.workspace, args[0].device, stream)
+        wsp = ws.data_ptr()
+    _lib.check(plan.fn(*pointers, wsp, plan.workspace, stream), target_name)
     return out
+
+
+def sequence_call(target_name, args, specs, out=None, rhs_contracting=1):
+    """ffi_call of a recurrence or grouped product without the per-call set-up:
+    the plan of operands of these shapes is looked up, and operands that a
+    plan's first call would accept go straight to the entry point.  `specs()`
+    gives the results' ShapeDtypeStructs.  Anything else takes ffi_call, which
+    checks and reports."""
+    first = args[0]
+    if isinstance(first, torch.Tensor) and first.is_cuda:
+        index = first.get_device()
+        try:
+            plan = _plans.get(_plan_key(_registry[target_name], index, rhs_contracting, args))
+        except (AttributeError, TypeError):
+            plan = None
+        if plan is not None and out is None and torch.cuda.current_device() == index:
+            for t, dt, present in zip(args, plan.dtypes, plan.present):
+                if present and (t.dtype is not dt or t.get_device() != index or
+                                not t.is_contiguous()):
+                    break
+            else:
+                outs = _run_plan(target_name, plan, args, index, None)
+                return outs[0] if len(outs) == 1 else tuple(outs)
+    results = specs()
+    attrs = {"rhs_contracting": rhs_contracting} \
+        if CONVENTIONS[_registry[target_name]].kind == "ragged" else {}
+    return ffi_call(target_name, results if len(results) > 1 else results[0])(*args, out=out,
+                                                                              **attrs)
 
 
 def _dot_dims(attrs, lhs_rank) -> _lib.DsDotDims:

@@ -14,7 +14,7 @@ from typing import Iterable, Optional, Sequence
 import torch
 
 from . import _lib
-from .ffi import ShapeDtypeStruct, ffi_call
+from .ffi import ShapeDtypeStruct, ffi_call, sequence_call
 
 F64, F32 = torch.float64, torch.float32
 
@@ -284,25 +284,26 @@ def ds_linear_recurrence_f64(a, b, h0=None, out=None):
     """h_t = a_t h_{t-1} + b_t along dim -2 of f64 a, b [..., T, D], from the
     state h0 [..., D] (default zeros) -> h [..., T, D].  T = 1 advances the
     state by one step; a_t = 0 starts a new sequence."""
-    return ffi_call("ds_linear_recurrence_f64", _sds(a.shape, F64))(a, b, h0, out=out)
+    return sequence_call("ds_linear_recurrence_f64", (a, b, h0), lambda: (_sds(a.shape, F64),), out)
 
 
 def ds_linear_recurrence_f32(a, b, h0=None, out=None):
     """ds_linear_recurrence_f64 of f32 tensors: the state is held in f64 and
     each h_t rounded once."""
-    return ffi_call("ds_linear_recurrence_f32", _sds(a.shape, F32))(a, b, h0, out=out)
+    return sequence_call("ds_linear_recurrence_f32", (a, b, h0), lambda: (_sds(a.shape, F32),), out)
 
 
 def ds_linear_recurrence_packed(a, b, h0=None, out=None):
     """ds_linear_recurrence_f64 of packed DS tensors [..., T, D, 2] and
     h0 [..., D, 2]."""
-    return ffi_call("ds_linear_recurrence_packed", _sds(a.shape, F32))(a, b, h0, out=out)
+    return sequence_call("ds_linear_recurrence_packed", (a, b, h0), lambda: (_sds(a.shape, F32),), out)
 
 
 def _recurrence_vjp(kind, dtype, a, h, grad_h, h0, out):
-    seq = _sds(a.shape, dtype)
-    res = (seq, seq, _sds(_state_shape(a.shape, kind == "packed"), dtype))
-    return ffi_call(f"ds_linear_recurrence_vjp_{kind}", res)(a, h, grad_h, h0, out=out)
+    def specs():
+        seq = _sds(a.shape, dtype)
+        return seq, seq, _sds(_state_shape(a.shape, kind == "packed"), dtype)
+    return sequence_call(f"ds_linear_recurrence_vjp_{kind}", (a, h, grad_h, h0), specs, out)
 
 
 def ds_linear_recurrence_vjp_f64(a, h, grad_h, h0=None, out=None):
@@ -335,28 +336,33 @@ def ds_ragged_dot_f64(lhs, rhs, group_sizes, rhs_contracting: int = 1, out=None)
     gradient of the rows is this product of the result's gradient with the
     same matrices and the other rhs_contracting; that of the matrices is
     ds_ragged_dot_contract_f64."""
-    res = _sds(_ragged_shape(lhs, rhs, rhs_contracting), F64)
-    return ffi_call("ds_ragged_dot_f64", res)(lhs, rhs, group_sizes,
-                                              rhs_contracting=rhs_contracting, out=out)
+    return sequence_call("ds_ragged_dot_f64", (lhs, rhs, group_sizes),
+                         lambda: (_sds(_ragged_shape(lhs, rhs, rhs_contracting), F64),), out,
+                         rhs_contracting)
 
 
 def ds_ragged_dot(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes, rhs_contracting: int = 1, out=None):
     """ds_ragged_dot_f64 on SoA DS operands -> (hi, lo)."""
-    res = _sds(_ragged_shape(lhs_hi, rhs_hi, rhs_contracting), F32)
-    return ffi_call("ds_ragged_dot", (res, res))(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes,
-                                                 rhs_contracting=rhs_contracting, out=out)
+    return sequence_call("ds_ragged_dot", (lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes),
+                         lambda: (_sds(_ragged_shape(lhs_hi, rhs_hi, rhs_contracting), F32),) * 2,
+                         out, rhs_contracting)
+
+
+def _contract_shape(lhs, rhs, group_sizes):
+    return tuple(group_sizes.shape[:1]) + tuple(lhs.shape[1:2]) + tuple(rhs.shape[1:2])
 
 
 def ds_ragged_dot_contract_f64(lhs, rhs, group_sizes, out=None):
     """out[g] = lhs_g^T rhs_g over the rows of each group: f64 lhs [M, K],
     rhs [M, N], int32 group_sizes [G] -> [G, K, N].  With lhs the rows and
     rhs the result's gradient: the gradient of ds_ragged_dot_f64's matrices."""
-    res = _sds((group_sizes.shape[0],) + tuple(lhs.shape[1:2]) + tuple(rhs.shape[1:2]), F64)
-    return ffi_call("ds_ragged_dot_contract_f64", res)(lhs, rhs, group_sizes, out=out)
+    return sequence_call("ds_ragged_dot_contract_f64", (lhs, rhs, group_sizes),
+                         lambda: (_sds(_contract_shape(lhs, rhs, group_sizes), F64),), out)
 
 
 def ds_ragged_dot_contract(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes, out=None):
     """ds_ragged_dot_contract_f64 on SoA DS operands -> (hi, lo)."""
-    res = _sds((group_sizes.shape[0],) + tuple(lhs_hi.shape[1:2]) + tuple(rhs_hi.shape[1:2]), F32)
-    return ffi_call("ds_ragged_dot_contract", (res, res))(lhs_hi, lhs_lo, rhs_hi, rhs_lo,
-                                                          group_sizes, out=out)
+    return sequence_call("ds_ragged_dot_contract",
+                         (lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes),
+                         lambda: (_sds(_contract_shape(lhs_hi, rhs_hi, group_sizes), F32),) * 2,
+                         out)
