@@ -2,7 +2,7 @@
 // matrix, and the contraction over each group's rows.
 //
 // Groups are sorted by their number of rows, on the device (prep_kernel): a
-// group of at least kTensorRows rows goes to the tensor-core product
+// group of many rows goes to the tensor-core product
 // (ragged_ozaki.cu), the others are multiplied here with FP64 matrix
 // instructions.  One launch serves all of a call's small groups.
 //
@@ -36,6 +36,8 @@ __device__ __forceinline__ void put(const DotResult& c, int64_t i, double v) {
 // ---- the groups' rows and tiles ------------------------------------------------
 
 constexpr int kPrepThreads = 1024;
+// Most groups that are put in order of their rows (each compares itself with all).
+constexpr int64_t kOrderedGroups = 2048;
 
 // Exclusive sum over the block, and the block's total.
 __device__ int64_t block_scan(int64_t v, int64_t& total) {
@@ -128,6 +130,21 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
   }
   if (G == 0 && tid == 0) p.row[0] = p.small_start[0] = p.tensor_start[0] = p.slot[0] = 0;
   __syncthreads();
+  // the groups by falling number of rows
+  if (p.order) {
+    for (int64_t g = tid; g < G; g += kPrepThreads) {
+      const int32_t n = p.row[g + 1] - p.row[g];
+      int32_t rank = static_cast<int32_t>(g);
+      if (G <= kOrderedGroups) {
+        rank = 0;
+        for (int64_t h = 0; h < G; ++h) {
+          const int32_t m = p.row[h + 1] - p.row[h];
+          rank += m > n || (m == n && h < g);
+        }
+      }
+      p.order[rank] = static_cast<int32_t>(g);
+    }
+  }
   auto fill = [&](const int32_t* start, int tile, RaggedTile* out, int64_t cap) {
     const int64_t n = start[G] < cap ? start[G] : cap;
     for (int64_t t = tid; t < n; t += kPrepThreads) {
@@ -310,14 +327,32 @@ struct Words {
     bytes = first < 0 ? -1 : left >= 2 ? 16 : left == 1 ? 8 : 0;
   }
 
-  // One whole stage of `lines` lines (kLinesK: kKS of them).
-  __device__ __forceinline__ void stage(double* tile, int64_t stride, int lines, int len) const {
+  // One stage of `lines` lines.  kLinesK: zeros in the lines up to kKS; else the
+  // stage has all its contraction.
+  __device__ __forceinline__ void stage(const DotOperand& o, double* tile, int64_t stride,
+                                        int lines, int len) const {
     if (bytes == 0) return;
     const int l0 = threadIdx.x / kWords;
     double* dst = tile + l0 * kPitch + threadIdx.x % kWords * 2;
     const double* p = src;
     const int64_t step = kStep * stride;
     constexpr int kPasses = (kLinesK ? kKS : kSmallTile) / kStep;
+    if (kLinesK && lines < kKS) {
+      const double* none = o.f64 - odd_start(o, 0, 0, 0);  // nothing is read from it
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const bool in = l0 + i * kStep < lines;
+        if (bytes > 0) {
+          copy_async<16>(dst, in ? p : none, in ? bytes : 0);
+        } else {
+          copy_async<8>(dst + 1, in ? p + 1 : none, in ? 8 : 0);
+          if (kLen - 1 < len) copy_async<8>(dst + kLen, in ? p + kLen : none, in ? 8 : 0);
+        }
+        p += step;
+        dst += kStep * kPitch;
+      }
+      return;
+    }
     if (bytes == 16) {
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
@@ -327,17 +362,17 @@ struct Words {
       }
       return;
     }
-#pragma unroll 1
+    const bool last = !kLinesK || kLen - 1 < len;
+#pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       if (!kLinesK && l0 + i * kStep >= lines) break;
       if (bytes == 8) {
-        copy_async<16>(dst, p, 8);
+        copy_async<16>(dst + i * kStep * kPitch, p, 8);
       } else {
-        copy_async<8>(dst + 1, p + 1, 8);
-        if (!kLinesK || kLen - 1 < len) copy_async<8>(dst + kLen, p + kLen, 8);
+        copy_async<8>(dst + i * kStep * kPitch + 1, p + 1, 8);
+        if (last) copy_async<8>(dst + i * kStep * kPitch + kLen, p + kLen, 8);
       }
       p += step;
-      dst += kStep * kPitch;
     }
   }
 };
@@ -372,7 +407,8 @@ __device__ __forceinline__ uint32_t units_of(const SmallArgs& a) {
 // nothing.
 __device__ __forceinline__ bool unit_at(const SmallArgs& a, uint32_t u, SmallUnit& x) {
   if (a.contract) {
-    const uint32_t per = a.tiles_k * a.tiles_n, g = u / per, r = u - g * per, tk = r / a.tiles_n;
+    const uint32_t per = a.tiles_k * a.tiles_n, at = u / per, r = u - at * per;
+    const uint32_t tk = r / a.tiles_n, g = a.p.order[at];
     x.g = static_cast<int>(g);
     x.row = static_cast<int64_t>(tk) * kSmallTile;
     x.col = static_cast<int64_t>(r - tk * a.tiles_n) * kTN;
@@ -510,36 +546,50 @@ template <int MF, int NF, int kWM>
 __device__ __forceinline__ void store_unit(const SmallArgs& a, const SmallUnit& x,
                                            const double (&acc)[4][2][2]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int wm = warp % kWM * MF * 8, wn = warp / kWM * NF * 8;
-  const int64_t first = (a.contract ? x.g * a.q.K : 0) + x.row;
+  const int r0 = warp % kWM * MF * 8 + (lane >> 2), c0 = warp / kWM * NF * 8 + 2 * (lane & 3);
+  const int64_t N = a.q.N, first = (a.contract ? x.g * a.q.K : 0) + x.row;
   DotResult out = a.q.out;
-  if (a.splits > 1) out = DotResult{a.partial + x.split * a.q.M * a.q.N, nullptr, nullptr};
-  const bool words = out.f64 && (a.q.N & 1) == 0 && (reinterpret_cast<uintptr_t>(out.f64) & 15) == 0;
+  if (a.splits > 1) out = DotResult{a.partial + x.split * a.q.M * N, nullptr, nullptr};
+  int64_t at = (first + r0) * N + x.col + c0;
+  if (out.f64 && !a.add) {
+    const bool words = (N & 1) == 0 && (reinterpret_cast<uintptr_t>(out.f64) & 15) == 0;
+    double* p = out.f64 + at;
 #pragma unroll
-  for (int i = 0; i < MF; ++i) {
-    const int r = wm + i * 8 + (lane >> 2);
-    if (r >= x.rows) continue;
+    for (int i = 0; i < MF; ++i, p += 8 * N) {
+      if (r0 + i * 8 >= x.rows) break;
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+        const int left = x.cols - c0 - j * 8;
+        if (words && left >= 2) {
+          *reinterpret_cast<double2*>(p + j * 8) = make_double2(acc[i][j][0], acc[i][j][1]);
+        } else {
+          if (left > 0) p[j * 8] = acc[i][j][0];
+          if (left > 1) p[j * 8 + 1] = acc[i][j][1];
+        }
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < MF; ++i, at += 8 * N) {
+    if (r0 + i * 8 >= x.rows) break;
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
-      const int c = wn + j * 8 + 2 * (lane & 3);
-      const int64_t at = (first + r) * a.q.N + x.col + c;
-      double v[2] = {acc[i][j][0], acc[i][j][1]};
-      if (words && !a.add && c + 2 <= x.cols) {
-        *reinterpret_cast<double2*>(out.f64 + at) = make_double2(v[0], v[1]);
-        continue;
-      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (c + h >= x.cols) continue;
-        if (a.add) v[h] = __dadd_rn(result_value(out, at + h), v[h]);
-        put(out, at + h, v[h]);
+        if (c0 + j * 8 + h >= x.cols) continue;
+        double v = acc[i][j][h];
+        if (a.add) v = __dadd_rn(result_value(out, at + j * 8 + h), v);
+        put(out, at + j * 8 + h, v);
       }
     }
   }
 }
 
-// Blocks stay and take every gridDim.x-th unit; the pipeline of stages runs on
-// across units.  kRows: most rows of a tile.
+constexpr uint32_t kNoUnit = 0xffffffffu;
+
+// Blocks stay and share the units out; the pipeline of stages runs on across
+// units.  kRows: most rows of a tile.
 template <bool kPair, bool kA, bool kB, int kRows>
 __global__ void __launch_bounds__(kThreads, 2)
 small_kernel(const __grid_constant__ SmallArgs a) {
@@ -555,9 +605,19 @@ small_kernel(const __grid_constant__ SmallArgs a) {
       put(a.q.out, i, 0.0);
   }
   const uint32_t units = units_of(a);
-  auto next_unit = [&](uint32_t u, SmallUnit& x) {
-    while (u < units && !unit_at(a, u, x)) u += gridDim.x;
-    return u;
+  // the block's units: every gridDim.x-th; a contraction's fall in size and are
+  // taken there and back, so that every block gets about as much
+  auto unit_number = [&](uint32_t step) {
+    const bool back = a.contract && (step & 1);
+    return step * gridDim.x + (back ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  };
+  auto next_unit = [&](uint32_t step, SmallUnit& x) {
+    while (step * gridDim.x < units) {
+      const uint32_t u = unit_number(step);
+      if (u < units && unit_at(a, u, x)) return step;
+      ++step;
+    }
+    return kNoUnit;
   };
   // loading runs kCount - 1 stages ahead of multiplying
   const DotOperand &A = a.q.lhs, &B = a.q.rhs;
@@ -565,32 +625,34 @@ small_kernel(const __grid_constant__ SmallArgs a) {
   Words<kA ? kSmallTile : kKS, kA ? kPitchN : kPitchK, kA> wa;
   Words<kB ? kTN : kKS, kB ? kPitchN : kPitchK, kB> wb;
   SmallUnit lx, x;
-  uint32_t lu = blockIdx.x;
+  uint32_t lu = 0;
   int64_t lk = 0;
-  auto start_unit = [&](uint32_t u) {
-    lu = next_unit(u, lx);
-    if (lu >= units) return;
+  auto start_unit = [&](uint32_t step) {
+    lu = next_unit(step, lx);
+    if (lu == kNoUnit) return;
     lk = lx.k0;
     if constexpr (!kPair) {
       wa.start(A, origin_a(a, lx, lk), line_a, lx.rows);
       wb.start(B, origin_b(a, lx, lk), line_b, lx.cols);
     }
   };
-  start_unit(blockIdx.x);
+  start_unit(0);
   int ls = 0;
   auto load_one = [&] {
-    if (lu < units) {
+    if (lu != kNoUnit) {
       double* sa = stage + ls * St::kStride;
       double* sb = sa + St::kOperandA;
-      if (!kPair && lk + kKS <= lx.k1) {
-        wa.stage(sa, line_a, lx.rows, lx.rows);
-        wb.stage(sb, line_b, lx.cols, lx.cols);
-      } else if (lk < lx.k1) {
+      const int64_t left = lx.k1 - lk;
+      if (!kPair && (left >= kKS || (kA && kB && left > 0))) {
+        const int kn = left < kKS ? static_cast<int>(left) : kKS;
+        wa.stage(A, sa, line_a, kA ? kn : lx.rows, lx.rows);
+        wb.stage(B, sb, line_b, kB ? kn : lx.cols, lx.cols);
+      } else if (left > 0) {
         stage_unit<kPair, kA, kB, kRows>(a, lx, lk, sa, sb);
       }
       lk += kKS;
       if (lk >= lx.k1) {
-        start_unit(lu + gridDim.x);
+        start_unit(lu + 1);
       } else if constexpr (!kPair) {
         wa.src += kKS * A.s_k;
         wb.src += kKS * B.s_k;
@@ -604,7 +666,7 @@ small_kernel(const __grid_constant__ SmallArgs a) {
   int cs = 0;
   const int lane = threadIdx.x & 31;
 #pragma unroll 1
-  for (uint32_t u = next_unit(blockIdx.x, x); u < units; u = next_unit(u + gridDim.x, x)) {
+  for (uint32_t u = next_unit(0, x); u != kNoUnit; u = next_unit(u + 1, x)) {
     double acc[4][2][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -670,31 +732,51 @@ small_sum_kernel(const __grid_constant__ SmallArgs a) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Contraction splits of the products: with few rows, units of at least kSplitMin
-// of the contraction, enough of them for kSplitUnits.  From the call's sizes
-// alone, so a row's rounding does not depend on other groups.
-constexpr int64_t kSplitMin = 128, kSplitUnits = 2400;
+// Contraction splits of the products: where the tiles are few, units of at least
+// kSplitMin of the contraction, enough of them to share out evenly among the
+// resident blocks (more when no tile has over 16 rows: those only stream the
+// matrices).  From the call's sizes alone, so a row's rounding does not depend
+// on other groups.
+constexpr int64_t kSplitMin = 128;
 constexpr int kMaxSplits = 16;
 
 int splits_of(int64_t M, int64_t K, int64_t N, int64_t G) {
+  const int64_t units = M <= 16 ? 2400 : 600;
   const int64_t tiles = (M / kSmallTile + (G < M ? G : M)) * ceil_div(N, kTN);
-  if (tiles == 0 || tiles >= kSplitUnits / 2) return 1;
-  int64_t s = ceil_div(kSplitUnits, tiles);
+  if (tiles == 0 || tiles >= units) return 1;
+  int64_t s = ceil_div(units, tiles);
   const int64_t most = K / kSplitMin;
   s = s > most ? most : s;
   s = s > kMaxSplits ? kMaxSplits : s;
   return s < 1 ? 1 : static_cast<int>(s);
 }
 
-// Whether the tensor-core product takes groups of many rows: its tiles are
-// padded to 256 columns and 128 of the contraction.
+// Whether the tensor-core product takes the large groups: where its estimated
+// time is below the FP64 path's.  In microseconds, from measurements on one B200:
+// the FP64 path does 26 TFLOP/s; the tensor-core product has launches of 60 (80)
+// us, splits a value in 6.4 to 8.3 (7) ps, multiplies at 3 POPS of its 28
+// operations per product (a contraction's short units take at least 0.76 us per
+// 256 x 256 outputs), and rebuilds an output in 9 ps.  Measured with / without:
+// 2048 x 1024 x 1024 in 4 groups 140 / 190 us (contraction 191 / 175), 4096 x 1024
+// x 1024 in 8 groups 224 / 337 (286 / 323), 2048 x 2048 x 2048 in 4 groups 300 /
+// 646 (423 / 624), 8192 x 512 x 512 in 8 groups 198 / 179 (171 / 173).
 bool tensor_allowed(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
-  return M >= kTensorRows && (contract ? K >= 128 : K >= 64) && N >= 128 &&
-         ragged_tensor_fits(M, K, N, G, contract);
+  if (M < tensor_rows(contract) || K < 64 || N < 64) return false;
+  const double m = M, k = K, n = N, slots = static_cast<double>(ragged_slots(M, G, contract));
+  const double macs = m * k * n, matrices = slots * k * n;
+  const double plain = 7.7e-8 * macs;
+  double tensor;
+  if (contract) {
+    const double gemm = 9.3e-9 * macs, least = 1.15e-5 * matrices;
+    tensor = 80 + 7e-6 * m * (k + n) + (gemm > least ? gemm : least) + 9e-6 * matrices;
+  } else {
+    tensor = 60 + 6.4e-6 * m * k + 8.3e-6 * matrices + 9.3e-9 * macs + 9e-6 * m * n;
+  }
+  return tensor < plain && ragged_tensor_fits(M, K, N, G, contract);
 }
 
 struct Layout {
-  size_t row, small_start, tensor_start, slot, small, tensor, slot_group, slot_bits, partial, tensor_ws, total;
+  size_t row, small_start, tensor_start, slot, order, small, tensor, slot_group, slot_bits, partial, tensor_ws, total;
   int64_t small_cap, tensor_cap, slots;
   int splits;
   bool tensor_ok;
@@ -713,14 +795,15 @@ Layout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
   l.small_cap = contract ? 0 : M / kSmallTile + groups;
   if (l.tensor_ok) {
     const int64_t rows = contract && M > kRaggedWindow ? kRaggedWindow : M;
-    l.slots = ragged_slots(rows, G);
-    l.tensor_cap = ragged_tensor_tiles(rows, G);
+    l.slots = ragged_slots(rows, G, contract);
+    l.tensor_cap = ragged_tensor_tiles(rows, G, contract);
   }
   l.splits = contract ? 1 : splits_of(M, K, N, G);
   l.row = take((G + 1) * 4);
   l.small_start = take((G + 1) * 4);
   l.tensor_start = take((G + 1) * 4);
   l.slot = take((G + 1) * 4);
+  l.order = take(contract ? G * 4 : 0);
   l.small = take(l.small_cap * sizeof(RaggedTile));
   l.tensor = take(l.tensor_cap * sizeof(RaggedTile));
   l.slot_group = take(l.slots * 4);
@@ -754,7 +837,7 @@ uint8_t* align_ws(void* workspace) {
                                     ~static_cast<uintptr_t>(1023));
 }
 
-RaggedPlan plan_at(const Layout& l, int64_t G, uint8_t* ws, bool tensor) {
+RaggedPlan plan_at(const Layout& l, int64_t G, bool contract, uint8_t* ws, bool tensor) {
   auto ints = [&](size_t off) { return reinterpret_cast<int32_t*>(ws + off); };
   RaggedPlan p{};
   p.groups = G;
@@ -762,13 +845,14 @@ RaggedPlan plan_at(const Layout& l, int64_t G, uint8_t* ws, bool tensor) {
   p.small_start = ints(l.small_start);
   p.tensor_start = ints(l.tensor_start);
   p.slot = ints(l.slot);
+  p.order = contract ? ints(l.order) : nullptr;
   p.small = l.small_cap ? reinterpret_cast<RaggedTile*>(ws + l.small) : nullptr;
   p.tensor = l.tensor_cap ? reinterpret_cast<RaggedTile*>(ws + l.tensor) : nullptr;
   p.slot_group = ints(l.slot_group);
   p.slot_bits = ints(l.slot_bits);
   p.small_cap = l.small_cap;
   p.tensor_cap = l.tensor_cap;
-  p.tensor_rows = tensor ? kTensorRows : INT32_MAX;
+  p.tensor_rows = tensor ? tensor_rows(contract) : INT32_MAX;
   if (tensor)
     for (int i = 0; i < kBitsLimits; ++i) p.bits_limit[i] = bits_limits()[i];
   return p;
@@ -857,7 +941,7 @@ int ragged_dot(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) 
   uint8_t* ws = align_ws(workspace);
   SmallArgs a{};
   a.q = q;
-  a.p = plan_at(l, q.G, ws, clusters > 0);
+  a.p = plan_at(l, q.G, false, ws, clusters > 0);
   a.tiles_n = static_cast<uint32_t>(ceil_div(q.N, kTN));
   a.splits = static_cast<uint32_t>(l.splits);
   a.split_k = ceil_div(ceil_div(q.K, l.splits), kKS) * kKS;
@@ -885,7 +969,7 @@ int ragged_contract(const RaggedProblem& q, void* workspace, size_t, cudaStream_
   uint8_t* ws = align_ws(workspace);
   SmallArgs a{};
   a.q = q;
-  a.p = plan_at(l, q.G, ws, clusters > 0);
+  a.p = plan_at(l, q.G, true, ws, clusters > 0);
   a.contract = true;
   a.tiles_k = static_cast<uint32_t>(ceil_div(q.K, kSmallTile));
   a.tiles_n = static_cast<uint32_t>(ceil_div(q.N, kTN));

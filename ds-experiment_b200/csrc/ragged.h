@@ -14,22 +14,23 @@ namespace dsb {
 constexpr int kSmallTile = 64;    // rows of a small group's tile
 constexpr int kTensorTile = 256;  // rows of a tile of the tensor-core product
 // Groups of at least this many rows are large: the tensor-core product takes
-// them.
-#ifndef KTR
-#define KTR 128
-#endif
-constexpr int64_t kTensorRows = KTR;
+// them.  Its fixed costs are a matrix's split (products) or rebuilding (contraction):
+// 32 groups of 128 rows, 2048 x 2048 matrices, take 1.21 ms with it and 1.36
+// without as products, 1.77 and 1.39 as a contraction; 16 of 256 rows 0.79 and
+// 1.28, 1.28 and 1.28.
+constexpr int64_t tensor_rows(bool contract) { return contract ? 256 : 128; }
 // Longest contraction over rows that is taken at once.
 constexpr int64_t kRaggedWindow = 1 << 15;
 // Most workspace that the tensor-core product may ask for.
 constexpr size_t kRaggedTensorBytes = static_cast<size_t>(48) << 30;
 
 // Large groups among G with M rows, and their tiles, at most.
-inline int64_t ragged_slots(int64_t M, int64_t G) {
-  return G < M / kTensorRows ? G : M / kTensorRows;
+inline int64_t ragged_slots(int64_t M, int64_t G, bool contract) {
+  const int64_t most = M / tensor_rows(contract);
+  return G < most ? G : most;
 }
-inline int64_t ragged_tensor_tiles(int64_t M, int64_t G) {
-  return M / kTensorTile + ragged_slots(M, G);
+inline int64_t ragged_tensor_tiles(int64_t M, int64_t G, bool contract) {
+  return M / kTensorTile + ragged_slots(M, G, contract);
 }
 
 // Rows [row, row + rows) of a group; slot: its number among the large ones.
@@ -48,6 +49,7 @@ struct RaggedPlan {
   int32_t* small_start;   // [G + 1] first tile of each small group, then their number
   int32_t* tensor_start;  // [G + 1] the same of the large ones
   int32_t* slot;          // [G + 1] large groups before each, then their number
+  int32_t* order;         // [G] the groups by falling number of rows (null: not wanted)
   RaggedTile* small;      // null: not wanted
   RaggedTile* tensor;
   int32_t* slot_group;    // of each large group: its number among all,

@@ -592,7 +592,7 @@ TensorLayout tensor_layout(int64_t M, int64_t K, int64_t N, int64_t G, bool cont
   TensorLayout g{};
   const int64_t length = contract ? M : K;
   g.chunk = length < kMaxK ? length : kMaxK;
-  g.slots = ragged_slots(contract ? g.chunk : M, G);
+  g.slots = ragged_slots(contract ? g.chunk : M, G, contract);
   g.Np = pad(N, 256);
   size_t at = 0;
   auto take = [&at](size_t bytes) {
@@ -604,7 +604,7 @@ TensorLayout tensor_layout(int64_t M, int64_t K, int64_t N, int64_t G, bool cont
   int64_t a_scales;
   if (contract) {
     g.Mp = pad(K, 256);
-    g.Kp = ragged_tensor_tiles(g.chunk, G) * kTensorTile;
+    g.Kp = ragged_tensor_tiles(g.chunk, G, true) * kTensorTile;
     g.a = take(l * g.Kp * g.Mp);
     g.b = take(l * g.Kp * g.Np);
     g.c = take(l * g.slots * g.Mp * g.Np);

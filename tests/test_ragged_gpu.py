@@ -238,21 +238,248 @@ def test_side_stream():
     assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("which", ["rows", "columns"])
-def test_long_contractions(which):
+# ---- calls whose large groups take the tensor-core product ---------------------------
+# Compared on the GPU with torch's f64 products; the bounds are sequence_ref's.
+
+LARGE = [
+    (2100, 1001, 1103, [900, 0, 127, 128, 645, 257]),  # odd sizes, both kinds of groups
+    (4100, 1000, 900, [1500, -5, 2000]),               # rows behind the last group
+    (3000, 900, 1030, [40, 2900, 100]),                # a group past row M
+]
+LARGE_IDS = [f"{m}x{k}x{n}/{len(s)}" for m, k, n, s in LARGE]
+
+
+def on_gpu(*shape, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(shape, generator=g, dtype=torch.float64, device="cuda")
+
+
+def expect(a, b, pairs=False):
+    """a @ b and sequence_ref's bound, with torch's own f64 sums (their error is
+    the f64 term once more)."""
+    K = a.shape[1]
+    c, terms = a @ b, a.abs() @ b.abs()
+    chunks = -(-K // 32768)
+    P = min(50, int((110.2 - 2 - np.log2(min(K, 32768))) // 2))
+    if chunks > 1:
+        P = int((110.2 - 2 - 15) // 2)
+    unit = 4.0 * a.abs().amax(1)[:, None] * b.abs().amax(0)[None, :] * 2.0 ** -P
+    f64 = (K + 2) * 2 * ref.U * terms
+    bound = f64 + torch.maximum(f64, (K + 2.0 ** (35 - P) * chunks) * unit +
+                                (2 + chunks) * ref.U * c.abs())
+    return c, bound + (c.abs() * 2.0 ** -48 + 2.0 ** -150 if pairs else 0.0)
+
+
+def within(got, want, bound):
+    assert bool(((got - want).abs() <= bound).all())
+
+
+class Reached:
+    """The calls inside ran the tensor-core product."""
+
+    def __enter__(self):
+        from ds_b200 import _lib
+        _lib.profile_enable(True)
+        _lib.profile_reset()
+
+    def __exit__(self, *exc):
+        from ds_b200 import _lib
+        n = _lib.profile_read("ozaki_gemm")[1]
+        _lib.profile_enable(False)
+        if exc[0] is None:
+            assert n > 0, "the tensor-core product did not run"
+
+
+def pair(x):
+    hi = x.float()
+    return hi, (x - hi.double()).float()
+
+
+@pytest.mark.parametrize("case", LARGE, ids=LARGE_IDS)
+@pytest.mark.parametrize("contracting", [1, 2])
+def test_large_products(case, contracting):
+    from ds_b200 import ops
+    M, K, N, sizes = case
+    x, w = on_gpu(M, K, seed=1), on_gpu(len(sizes), K, N, seed=2)
+    wt = w if contracting == 1 else w.transpose(1, 2).contiguous()
+    s = sz(sizes)
+    with Reached():
+        out = ops.ds_ragged_dot_f64(x, wt, s, rhs_contracting=contracting)
+        hi, lo = ops.ds_ragged_dot(*pair(x), *pair(wt), s, rhs_contracting=contracting)
+    end = 0
+    for g, b, e in ref.spans(sizes, M):
+        if e > b:
+            within(out[b:e], *expect(x[b:e], w[g]))
+            xp, wp = (sum(v.double() for v in pair(t)) for t in (x[b:e], w[g]))
+            within(hi[b:e].double() + lo[b:e].double(), *expect(xp, wp, pairs=True))
+        end = e
+    assert not out[end:].any() and not hi[end:].any() and not lo[end:].any()
+    assert torch.equal(out, ops.ds_ragged_dot_f64(x, wt, s, rhs_contracting=contracting))
+
+
+@pytest.mark.parametrize("case", [(4100, 1000, 900, [1500, -5, 2000]),
+                                  (5000, 901, 1103, [255, 2000, 0, 256, 1700, 30])],
+                         ids=["even", "odd"])
+def test_large_contraction(case):
+    from ds_b200 import ops
+    M, K, N, sizes = case
+    x, y, s = on_gpu(M, K, seed=3), on_gpu(M, N, seed=4), sz(sizes)
+    with Reached():
+        out = ops.ds_ragged_dot_contract_f64(x, y, s)
+        hi, lo = ops.ds_ragged_dot_contract(*pair(x), *pair(y), s)
+    for g, b, e in ref.spans(sizes, M):
+        if e > b:
+            within(out[g], *expect(x[b:e].T, y[b:e]))
+            xp, yp = (sum(v.double() for v in pair(t)) for t in (x[b:e], y[b:e]))
+            within(hi[g].double() + lo[g].double(), *expect(xp.T, yp, pairs=True))
+        else:
+            assert not out[g].any() and not hi[g].any() and not lo[g].any()
+    assert torch.equal(out, ops.ds_ragged_dot_contract_f64(x, y, s))
+
+
+def test_large_views_off_the_boundary_and_guards():
+    """Operands one value into their storage, results inside a larger buffer."""
+    from ds_b200 import ops
+    M, K, N, sizes = LARGE[0]
+    x, w, s = on_gpu(M, K, seed=5), on_gpu(len(sizes), K, N, seed=6), sz(sizes)
+
+    def off(t):
+        v = torch.empty(t.numel() + 1, dtype=torch.float64, device="cuda")
+        v[1:] = t.flatten()
+        return v[1:].view(t.shape)
+
+    want = ops.ds_ragged_dot_f64(x, w, s)
+    buf = torch.full((M * N + 65,), 7.0, dtype=torch.float64, device="cuda")
+    out = buf[33:33 + M * N].view(M, N)
+    ops.ds_ragged_dot_f64(off(x), off(w), s, out=out)
+    assert torch.equal(out, want)
+    assert bool((buf[:33] == 7.0).all()) and bool((buf[33 + M * N:] == 7.0).all())
+    M, K, N, sizes = 4100, 1000, 901, [1500, 0, 2000]
+    x, y, s = on_gpu(M, K, seed=7), on_gpu(M, N, seed=8), sz(sizes)
+    want = ops.ds_ragged_dot_contract_f64(x, y, s)
+    n = want.numel()
+    buf = torch.full((n + 65,), 7.0, dtype=torch.float64, device="cuda")
+    out = buf[33:33 + n].view(want.shape)
+    with Reached():
+        ops.ds_ragged_dot_contract_f64(off(x), off(y), s, out=out)
+    assert torch.equal(out, want)
+    assert bool((buf[:33] == 7.0).all()) and bool((buf[33 + n:] == 7.0).all())
+
+
+def test_large_non_finite_stays_in_its_group():
+    from ds_b200 import ops
+    M, K, N, sizes = 4100, 1000, 900, [1500, 0, 2000, 300]
+    x, w, y = on_gpu(M, K, seed=9), on_gpu(4, K, N, seed=10), on_gpu(M, N, seed=11)
+    s = sz(sizes)
+    bad = torch.zeros((M, N), dtype=torch.bool, device="cuda")
+    badc = torch.zeros((4, K, N), dtype=torch.bool, device="cuda")
+    want, wantc = (f(*v, s) for f, v in ((ops.ds_ragged_dot_f64, (x, w)),
+                                         (ops.ds_ragged_dot_contract_f64, (x, y))))
+    w[1] = float("nan")                     # nobody's matrix
+    x[3800:], y[3800:] = float("nan"), float("inf")  # behind the last group
+    x[3, 7] = float("nan")
+    bad[3], badc[0, 7] = True, True
+    w[2, 5, 11] = float("inf")
+    bad[1500:3500, 11] = True
+    y[3600, 20] = -float("inf")
+    badc[3, :, 20] = True
+    with Reached():
+        got, gotc = ops.ds_ragged_dot_f64(x, w, s), ops.ds_ragged_dot_contract_f64(x, y, s)
+    assert torch.equal(~got.isfinite(), bad)
+    assert torch.equal(~gotc.isfinite(), badc)
+    assert torch.equal(got[~bad], want[~bad]) and torch.equal(gotc[~badc], wantc[~badc])
+    assert not got[3800:].any()
+
+
+def test_large_zero_rows_columns_and_wide_range():
+    """Rows and columns of zeros give exact zeros; with values over 60 binades
+    and large entries facing zeros most outputs fail the certificate and are
+    summed again: each stays within 2^-24 of itself or the f64 sums' bound."""
+    from ds_b200 import ops
+    M, K, N, sizes = 4100, 700, 1000, [1500, 0, 2000, 300]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(12)
+
+    def spread(t):
+        e = torch.randint(-60, 1, t.shape, generator=g, device="cuda")
+        return t * torch.pow(torch.tensor(2.0, dtype=torch.float64, device="cuda"), e)
+
+    x, w, y = spread(on_gpu(M, K, seed=13)), spread(on_gpu(4, K, N, seed=14)), \
+        spread(on_gpu(M, N, seed=15))
+    x[:, 0], w[:, 0] = 2.0 ** 40, 0.0
+    x[5], w[2, :, 9], y[:1500, 4] = 0.0, 0.0, 0.0
+    s = sz(sizes)
+    with Reached():
+        out, outc = ops.ds_ragged_dot_f64(x, w, s), ops.ds_ragged_dot_contract_f64(x, y, s)
+    assert not out[5].any() and not out[1500:3500, 9].any() and not outc[0, :, 4].any()
+    for i, b, e in ref.spans(sizes, M):
+        for got, p, q in ((out[b:e], x[b:e], w[i]), (outc[i], x[b:e].T, y[b:e])):
+            if e > b:
+                terms = p.abs() @ q.abs()
+                within(got, p @ q, (p.shape[1] + 2) * 4 * ref.U * terms + 2.0 ** -24 * got.abs())
+
+
+def test_large_graph_replayed_with_other_sizes():
+    """One captured graph for every split of the rows: groups change kind."""
+    from ds_b200 import ops
+    M, K, N = 4100, 1000, 900
+    x, w, y = on_gpu(M, K, seed=16), on_gpu(4, K, N, seed=17), on_gpu(M, N, seed=18)
+    s = sz([1500, 0, 2000, 300])
+    ops.ds_ragged_dot_f64(x, w, s)
+    ops.ds_ragged_dot_contract_f64(x, y, s)
+    torch.cuda.synchronize()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        o1 = ops.ds_ragged_dot_f64(x, w, s)
+    with torch.cuda.graph(g2):
+        o2 = ops.ds_ragged_dot_contract_f64(x, y, s)
+    for sizes in ([1500, 0, 2000, 300], [0, 0, 0, 4100], [1, 127, 128, 129], [0] * 4,
+                  [255, 256, 257, 3000], [4100, 5, 5, -1]):
+        s.copy_(sz(sizes))
+        g2.replay()
+        g1.replay()
+        assert torch.equal(o1, ops.ds_ragged_dot_f64(x, w, s))
+        assert torch.equal(o2, ops.ds_ragged_dot_contract_f64(x, y, s))
+        end = 0
+        for i, b, e in ref.spans(sizes, M):
+            if e > b:
+                within(o1[b:e], *expect(x[b:e], w[i]))
+                within(o2[i], *expect(x[b:e].T, y[b:e]))
+            else:
+                assert not o2[i].any()
+            end = e
+        assert not o1[end:].any()
+
+
+def test_long_contractions():
     """Contractions above 32768, which the tensor-core product takes in chunks."""
     from ds_b200 import ops
-    rng = np.random.default_rng(9)
     n = 33000 + 41
-    if which == "rows":
-        x, w = rng.standard_normal((150, n)), rng.standard_normal((2, n, 130))
-        check(host(ops.ds_ragged_dot_f64(cu(x), cu(w), sz([130, 20]))),
-              *ref.ragged_dot(x, w, [130, 20]))
-    else:
-        x, y = rng.standard_normal((n, 130)), rng.standard_normal((n, 140))
-        for sizes in ([n - 3, 3], [100, 32700, 241], [0, 32768, 0, 273]):
-            check(host(ops.ds_ragged_dot_contract_f64(cu(x), cu(y), sz(sizes))),
-                  *ref.ragged_contract(x, y, sizes))
+    x, w = on_gpu(700, n, seed=19), on_gpu(3, n, 300, seed=20)
+    wt = w.transpose(1, 2).contiguous()
+    with Reached():
+        out = ops.ds_ragged_dot_f64(x, w, sz([400, 40, 250]))
+        outt = ops.ds_ragged_dot_f64(x, wt, sz([400, 40, 250]), rhs_contracting=2)
+    for g, b, e in ref.spans([400, 40, 250], 700):
+        within(out[b:e], *expect(x[b:e], w[g]))
+        within(outt[b:e], *expect(x[b:e], w[g]))
+    assert not out[690:].any()
+    x, y = on_gpu(n, 300, seed=21), on_gpu(n, 400, seed=22)
+    for sizes in ([n - 3, 3], [100, 32700, 241], [0, 32768, 0, 273], [32500, 541],
+                  [32768 - 100, 100, 273]):
+        with Reached():
+            out = ops.ds_ragged_dot_contract_f64(x, y, sz(sizes))
+            hi, lo = ops.ds_ragged_dot_contract(*pair(x), *pair(y), sz(sizes))
+        xp, yp = (sum(v.double() for v in pair(t)) for t in (x, y))
+        for g, b, e in ref.spans(sizes, n):
+            if e > b:
+                within(out[g], *expect(x[b:e].T, y[b:e]))
+                want, bound = expect(xp[b:e].T, yp[b:e], pairs=True)
+                # the pairs of two chunks are rounded twice
+                within(hi[g].double() + lo[g].double(), want, bound + want.abs() * 2.0 ** -47)
+            else:
+                assert not out[g].any() and not hi[g].any()
 
 
 def test_gradients_are_the_adjoint():
