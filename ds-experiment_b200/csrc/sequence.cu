@@ -14,22 +14,28 @@
 // them, and once the state at the chunk's start is known each thread runs its
 // steps again from its own start and stores them.
 //
-// The state at a chunk's start comes from the chunks before it through the
-// workspace.  Chunks stand in rounds of `round` chunks: a chunk publishes
-// (P, S) as soon as it has read its values; it takes those of the earlier
-// chunks of its round and the state the last round ended with, and applies
-// them in order; the round's last chunk publishes that state.  So the chain
-// has one hop per round rather than per chunk, and the order of every
+// The state at a chunk's start is the last one's end where a block takes all
+// chunks of its channels (many channels).  Otherwise it comes from the chunks
+// before it through the workspace: chunks stand in rounds of `round` chunks; a
+// chunk publishes (P, S) as soon as it has read its values; it takes those of the
+// earlier chunks of its round and the state the last round ended with, and
+// applies them in order; the round's last chunk publishes that state.  So the
+// chain has one hop per round rather than per chunk, and the order of every
 // operation is fixed by the shape.  A published value is its own message: the
 // workspace starts as all ones (a NaN no result has), and a reader polls the
 // value itself, so there is no flag, fence or barrier between the two.
 //
-// Blocks stay on their SM and take units from a counter, chunk by chunk, one
-// ahead: the next unit's values travel to shared memory (cp.async, each thread
-// into slots of its own) while the current one waits for its state.  What a
-// unit waits for is an earlier unit, and the earliest unfinished one is always
-// some block's current one, so the chain moves; each wait is bounded (about
-// 2 s), after which the unit works with NaN.
+// Blocks stay on their SM; the next unit's values travel to shared memory
+// (cp.async, each thread into slots of its own) while the current one is worked
+// on.  Chunks of all tiles are taken from a counter, chunk by chunk, one ahead:
+// what a unit waits for is an earlier unit, and the earliest unfinished one is
+// always some block's current one, so the chain moves; each wait is bounded
+// (about 2 s), after which the unit works with NaN.
+//
+// Measured on one B200 (cold L2, launch included): f64 [8, 2048, 1024] 80 us =
+// 5.0 TB/s, its gradient 129 us = 5.2 TB/s, [1, 65536, 250] 112 us, f32 [4, 4096,
+// 2048] 90 us.  A plain kernel that reads two arrays of that size and writes a
+// third takes 70 us (5.8 TB/s), whatever the width of its rows.
 #include <mutex>
 #include <vector>
 
@@ -140,16 +146,26 @@ struct Map {
   double p, s;  // state -> p state + s
 };
 
+__device__ __forceinline__ bool not_finite(double v) {
+  return (__double2hiint(v) & 0x7ff00000) == 0x7ff00000;
+}
+
 // A zero state stays out of the product, so that coefficients whose product
 // has overflowed do not turn it into NaN (a coefficient that is itself NaN or
-// infinite has made s NaN already).
+// infinite has made s NaN already).  Looked at only where the result is not
+// finite: 0 p + s is s for a finite p, and a comparison in f64 costs as much as
+// the step.
 __device__ __forceinline__ double apply(const Map& m, double state) {
-  return state == 0.0 ? m.s : __fma_rn(m.p, state, m.s);
+  const double r = __fma_rn(m.p, state, m.s);
+  if (not_finite(r) && state == 0.0) return m.s;
+  return r;
 }
 
 // first, then second.
 __device__ __forceinline__ Map compose(const Map& first, const Map& second) {
-  return Map{first.p == 0.0 ? 0.0 : __dmul_rn(second.p, first.p), apply(second, first.s)};
+  double p = __dmul_rn(second.p, first.p);
+  if (not_finite(p) && first.p == 0.0) p = 0.0;
+  return Map{p, apply(second, first.s)};
 }
 
 template <class E>
@@ -161,16 +177,13 @@ struct ChunkArgs {
   uint32_t tiles;     // of CT channels
   uint32_t chunks, units;
   uint32_t round;     // chunks per round, at most kMaxRound
-  uint32_t* counter;  // units taken, minus one (null: one chunk, nothing to wait for)
+  uint32_t* counter;  // units taken, minus one (null: a block takes whole tiles)
   uint32_t* err;      // all ones, or 1 when a wait has run out
   ulonglong2* maps;   // [chunks][tiles][CT]
   uint64_t* states;   // [rounds][tiles][CT]
 };
 
-#ifndef SEQ_MR
-#define SEQ_MR 16
-#endif
-constexpr int kMaxRound = SEQ_MR;
+constexpr int kMaxRound = 16;
 constexpr uint64_t kEmpty = ~0ull;
 
 // The bits of v, a NaN's made the ordinary one (never kEmpty).
@@ -322,28 +335,46 @@ __device__ __forceinline__ void issue(const ChunkArgs<E>& p, const Part& q,
   else if (q.n > 0) issue_part<false, E, V, R, kGrad>(p, q, s);
 }
 
-template <class E, int V, int R, bool kGrad>
+// A part's values, widened once: a conversion costs a quarter of the FP64 rate.
+template <int V, int R, bool kGrad>
 struct Values {
-  Word<E, V> a[R], x[R], h[kGrad ? R : 1];
+  double a[R][V], x[R][V], h[kGrad ? R : 1][V];
 };
 
 // Steps that the part does not have do nothing: s -> 1 s + 0.
 template <class E, int V, int R, bool kGrad>
 __device__ __forceinline__ void read(const ChunkArgs<E>& p, const Part& q, const Slots<E, V, R>& s,
-                                     Values<E, V, R, kGrad>& v) {
+                                     Values<V, R, kGrad>& v) {
   using IO = SeqIO<E>;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const bool in = i < q.n;
-    v.x[i] = s.x[i * kThreads];
-    v.a[i] = s.a[i * kThreads];
-    if constexpr (kGrad) v.h[i] = s.h[i * kThreads];
+    const Word<E, V> x = s.x[i * kThreads], a = s.a[i * kThreads];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (!in) v.x[i].v[j] = IO::zero();
-      if (!in || (kGrad && i == 0 && q.p0 == 0)) v.a[i].v[j] = IO::one();
+      v.x[i][j] = IO::value(x.v[j]);
+      v.a[i][j] = IO::value(a.v[j]);
+    }
+    if constexpr (kGrad) {
+      const Word<E, V> h = s.h[i * kThreads];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v.h[i][j] = IO::value(h.v[j]);
+    }
+  }
+  if (kGrad && q.p0 == 0) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v.a[0][j] = 1.0;
+  }
+  if (q.n == R && !(kGrad && !p.h0 && q.p0 + R == p.T)) return;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (i >= q.n) {
+        v.x[i][j] = 0.0;
+        v.a[i][j] = 1.0;
+      }
       if constexpr (kGrad) {
-        if (!p.h0 && q.p0 + i == p.T - 1) v.h[i].v[j] = IO::zero();
+        if (!p.h0 && q.p0 + i == p.T - 1) v.h[i][j] = 0.0;
       }
     }
   }
@@ -352,7 +383,7 @@ __device__ __forceinline__ void read(const ChunkArgs<E>& p, const Part& q, const
 // The steps from `state` on, stored.
 template <bool kFull, class E, int V, int R, bool kGrad>
 __device__ __forceinline__ void run_part(const ChunkArgs<E>& p, const Part& q,
-                                         const Values<E, V, R, kGrad>& v, double (&state)[V]) {
+                                         const Values<V, R, kGrad>& v, double (&state)[V]) {
   using IO = SeqIO<E>;
   const int64_t dir = kGrad ? -static_cast<int64_t>(p.D) : static_cast<int64_t>(p.D);
   E* out = p.out + q.row;
@@ -363,8 +394,8 @@ __device__ __forceinline__ void run_part(const ChunkArgs<E>& p, const Part& q,
     double g[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      state[j] = __fma_rn(IO::value(v.a[i].v[j]), state[j], IO::value(v.x[i].v[j]));
-      if constexpr (kGrad) g[j] = __dmul_rn(state[j], IO::value(v.h[i].v[j]));
+      state[j] = __fma_rn(v.a[i][j], state[j], v.x[i][j]);
+      if constexpr (kGrad) g[j] = __dmul_rn(state[j], v.h[i][j]);
     }
     IO::template put<V>(out, state);
     out += dir;
@@ -392,32 +423,44 @@ scan_chunk_kernel(const __grid_constant__ ChunkArgs<E> p) {
   slots.a = reinterpret_cast<Word<E, V>*>(smem) + threadIdx.x;
   slots.x = slots.a + R * kThreads;
   slots.h = slots.x + R * kThreads;  // gradient only
-  __shared__ Map s_map[2][S][CT];
+  __shared__ Map s_map[2][S][CT];  // channel V c + j at j N + c: no bank twice
   __shared__ Map s_before[kMaxRound][CT];
   __shared__ double s_start[CT];
   __shared__ uint32_t s_unit[2];
   const int tid = threadIdx.x, cl = tid % N * V, sub = tid / N;
 
   wait_previous_grid();
+  // a block with tiles of its own takes their chunks one after another
   uint32_t unit = blockIdx.x;
+  auto after = [&](uint32_t u) {
+    if (u + p.tiles < p.units) return u + p.tiles;
+    return u % p.tiles + gridDim.x < p.tiles ? u % p.tiles + gridDim.x : p.units;
+  };
   if (p.counter) {
     if (tid == 0) s_unit[0] = atomicAdd(p.counter, 1u) + 1u;
     __syncthreads();
     unit = s_unit[0];
   }
-  Part q{};
-  if (unit < p.units) {
-    q = part_of<E, V, CT, R, kGrad>(p, unit);
-    issue<E, V, R, kGrad>(p, q, slots);
-  }
-  asm volatile("cp.async.commit_group;" ::: "memory");
+  if (unit >= p.units) return;
+  Part q = part_of<E, V, CT, R, kGrad>(p, unit);
+  issue<E, V, R, kGrad>(p, q, slots);
   int turn = 0;
-  while (unit < p.units) {
+  for (;;) {
     turn ^= 1;
     if (p.counter && tid == 0) s_unit[turn] = atomicAdd(p.counter, 1u) + 1u;
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    Values<E, V, R, kGrad> val;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    Values<V, R, kGrad> val;
     read<E, V, R, kGrad>(p, q, slots, val);
+    // the slots are this thread's own: the next unit's values may come
+    const Part cur = q;
+    uint32_t next = p.units;
+    if (!p.counter) {
+      next = after(unit);
+      if (next < p.units) {
+        q = part_of<E, V, CT, R, kGrad>(p, next);
+        issue<E, V, R, kGrad>(p, q, slots);
+      }
+    }
     Map m[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) m[j] = Map{1.0, 0.0};
@@ -425,30 +468,29 @@ scan_chunk_kernel(const __grid_constant__ ChunkArgs<E> p) {
     for (int i = 0; i < R; ++i) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const double a = IO::value(val.a[i].v[j]);
-        m[j].s = __fma_rn(a, m[j].s, IO::value(val.x[i].v[j]));
-        m[j].p = __dmul_rn(m[j].p, a);
+        m[j].s = __fma_rn(val.a[i][j], m[j].s, val.x[i][j]);
+        m[j].p = __dmul_rn(m[j].p, val.a[i][j]);
       }
     }
     // inclusive scan over the S threads of a channel
     int buf = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) s_map[0][sub][cl + j] = m[j];
+    for (int j = 0; j < V; ++j) s_map[0][sub][j * N + tid % N] = m[j];
     __syncthreads();
-    const uint32_t next = p.counter ? s_unit[turn] : unit + gridDim.x;
-    const Part cur = q;
-    if (next < p.units) {
-      q = part_of<E, V, CT, R, kGrad>(p, next);
-      issue<E, V, R, kGrad>(p, q, slots);
+    if (p.counter) {
+      next = s_unit[turn];
+      if (next < p.units) {
+        q = part_of<E, V, CT, R, kGrad>(p, next);
+        issue<E, V, R, kGrad>(p, q, slots);
+      }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
     for (int d = 1; d < S; d <<= 1) {
       buf ^= 1;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (sub >= d) m[j] = compose(s_map[buf ^ 1][sub - d][cl + j], m[j]);
-        s_map[buf][sub][cl + j] = m[j];
+        if (sub >= d) m[j] = compose(s_map[buf ^ 1][sub - d][j * N + tid % N], m[j]);
+        s_map[buf][sub][j * N + tid % N] = m[j];
       }
       __syncthreads();
     }
@@ -492,45 +534,37 @@ scan_chunk_kernel(const __grid_constant__ ChunkArgs<E> p) {
         s_start[cs] = start;
         if (!last && ends)
           put_state(p.states + (static_cast<int64_t>(rnd) * p.tiles + cur.tile) * CT + cs,
-                    apply(s_map[buf][S - 1][cs], start));
+                    apply(s_map[buf][S - 1][cs % V * N + cs / V], start));
       }
-    } else if (cs < CT) {
+    } else if (cs < CT && cur.chunk == 0) {
       s_start[cs] = !kGrad && p.h0 && channel < p.C ? IO::value(IO::load(p.h0 + channel)) : 0.0;
     }
-    __syncthreads();
+    if (p.counter || cur.chunk == 0) __syncthreads();
     double state[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       state[j] = s_start[cl + j];
-      if (sub > 0) state[j] = apply(s_map[buf][sub - 1][cl + j], state[j]);
+      if (sub > 0) state[j] = apply(s_map[buf][sub - 1][j * N + tid % N], state[j]);
     }
     if (cur.n == R) run_part<true, E, V, R, kGrad>(p, cur, val, state);
     else if (cur.n > 0) run_part<false, E, V, R, kGrad>(p, cur, val, state);
     __syncthreads();  // s_map, s_before and s_start are written again
+    if (!p.counter && sub == S - 1) {
+      // where the tile's next chunk starts
+#pragma unroll
+      for (int j = 0; j < V; ++j) s_start[cl + j] = state[j];
+    }
+    if (next >= p.units) break;
     unit = next;
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Steps per thread of one channel each; half as many of two channels.
-// Registers hold two (gradient: three) values of each.
-#ifndef SEQ_RF
-#define SEQ_RF 16
-#endif
-#ifndef SEQ_RG
-#define SEQ_RG 10
-#endif
-#ifndef SEQ_RF1
-#define SEQ_RF1 16
-#endif
-#ifndef SEQ_RG1
-#define SEQ_RG1 12
-#endif
-#ifndef SEQ_C64
-#define SEQ_C64 2048
-#endif
+// Steps of one channel per thread, half as many of two channels (f32; f64 and
+// pairs).  Registers hold two (gradient: three) f64 values of each: two blocks per
+// SM with 128 registers.  8 or 12 of f64 instead of 16 were 5 to 15% slower, 20
+// and 24 of f32 4 to 8%, 6 and 8 of the gradient's 10 up to 18%.
 constexpr int steps_of(int type, bool gradient) {
-  return type == 1 ? (gradient ? SEQ_RG1 : SEQ_RF1) : (gradient ? SEQ_RG : SEQ_RF);
+  return type == 1 ? (gradient ? 12 : 16) : (gradient ? 10 : 16);
 }
 
 // ScanArgs::type of an element type (packed pairs and f64 are alike here).
@@ -539,15 +573,9 @@ constexpr int type_of() {
   return sizeof(E) == 4 ? 1 : 0;
 }
 
-// Channels per unit: 64 where there are as many (512 contiguous bytes of f64
-// per step), fewer where a unit would be mostly empty.
-int unit_channels(int64_t C, int64_t T, int steps) {
-  if (C >= SEQ_C64 || T <= 4 * steps) return 64;
-  return C >= 16 || T <= 16 * steps ? 16 : 4;
-}
-
 struct Plan {
   int ct;
+  bool own;  // a block takes whole tiles
   int64_t C, tiles, chunks, rounds;
   int round;
   size_t off_maps, off_states, total;
@@ -555,16 +583,36 @@ struct Plan {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The workspace: counter, error word, maps, states; every call sets it to
-// ones.
+// Blocks that work at a time: two per SM of B200 (the plan goes by it on every
+// device, so that results do not depend on the device).
+constexpr int64_t kBlocks = 296;
+
+// Channels per unit, and who carries the state.  Where tiles of 64, 32 or 16
+// channels keep at least 0.8 of the blocks busy, each block takes whole tiles,
+// chunk by chunk, and nothing is waited for: [8, 2048, 1024] of f64 in 256 tiles
+// of 32 takes 80 us, through the workspace 84, and f32 [4, 4096, 2048] 98 and 104.
+// Otherwise the chunks of all tiles are shared out: 64 channels per unit (512
+// contiguous bytes of f64 per step), 16 where the channels are few, so that a
+// unit has more steps and the chain fewer hops ([1, 65536, 250]: 115 us, with 64
+// channels 145), 4 for a handful of channels.  The workspace holds the counter,
+// the error word, maps and states; every call sets it to ones.
 Plan plan_of(int64_t B, int64_t T, int64_t D, int steps) {
   Plan g{};
   g.C = B * D;
   if (g.C == 0 || T <= kShort) return g;
-  g.ct = unit_channels(g.C, T, steps);
+  for (int ct = 64; ct >= 16 && !g.own; ct /= 2) {
+    const int64_t tiles = ceil_div(g.C, ct);
+    if (tiles * 5 >= ceil_div(tiles, kBlocks) * kBlocks * 4 || T <= kThreads / ct * steps) {
+      g.own = true;
+      g.ct = ct;
+    }
+  }
+  if (!g.own) g.ct = g.C >= 2048 ? 64 : g.C >= 16 ? 16 : 4;
+  const int64_t rows = kThreads / g.ct * steps;
   g.tiles = ceil_div(g.C, g.ct);
-  g.chunks = ceil_div(T, kThreads / g.ct * steps);
-  if (g.chunks == 1) return g;
+  g.chunks = ceil_div(T, rows);
+  if (g.chunks == 1) g.own = true;
+  if (g.own) return g;
   const int64_t want = ceil_div(512, g.tiles);
   g.round = want < 4 ? 4 : want > kMaxRound ? kMaxRound : static_cast<int>(want);
   g.rounds = ceil_div(g.chunks, g.round);
@@ -618,7 +666,7 @@ int launch_chunks(const ScanArgs& s, const Plan& g, cudaStream_t st) {
   p.chunks = static_cast<uint32_t>(g.chunks);
   p.units = static_cast<uint32_t>(g.chunks * g.tiles);
   p.round = static_cast<uint32_t>(g.round);
-  if (g.chunks > 1) {
+  if (!g.own) {
     uint8_t* ws = static_cast<uint8_t*>(s.workspace);
     p.counter = reinterpret_cast<uint32_t*>(ws);
     p.err = p.counter + 1;
@@ -630,7 +678,8 @@ int launch_chunks(const ScanArgs& s, const Plan& g, cudaStream_t st) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(p.units < static_cast<uint32_t>(resident) ? p.units : resident);
+  const uint32_t most = g.own ? p.tiles : p.units;
+  cfg.gridDim = dim3(most < static_cast<uint32_t>(resident) ? most : resident);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = stage_bytes<E, V, R, kGrad>();
   cfg.stream = st;
@@ -661,6 +710,7 @@ int launch(const ScanArgs& s, cudaStream_t st) {
   if (units > 0x7fffffff || g.C > 0x7fffffff)
     return set_error(DS_INVALID_ARGUMENT, "ds_linear_recurrence: too many channels");
   if (g.ct == 64) return launch_chunks<E, 64, kGrad>(s, g, st);
+  if (g.ct == 32) return launch_chunks<E, 32, kGrad>(s, g, st);
   if (g.ct == 16) return launch_chunks<E, 16, kGrad>(s, g, st);
   if (g.ct == 4) return launch_chunks<E, 4, kGrad>(s, g, st);
   auto in = [](const void* p) { return static_cast<const E*>(p); };
