@@ -298,6 +298,24 @@ __device__ __forceinline__ int shift_from_code(int code, int P) {
   return P - (code - kExpBias);
 }
 
+// The certificate by the operands' own 1-norms (the products grouped by expert).
+// In units of C_int the quantisation error of an output is at most
+// (||a_int||_1 + ||b_int||_1) / 2 + K / 4, and ||a_int||_1 <= sum |a| 2^sa + K / 2.
+// A row's (column's) part of 2^kCertifyBits times that, rounded up: the sums and
+// the conversion lose less than 2^-20 of it.
+constexpr int kCertifyBits = 24;
+
+__device__ __forceinline__ float certify_part(double sum, int shift, int64_t K) {
+  if (shift == kShiftNonFinite || shift == kShiftZero) return 0.0f;
+  const double units = scale2(sum, shift) + 0.5 * static_cast<double>(K);
+  return __double2float_ru(0.5 * units * ((1 << kCertifyBits) * (1.0 + 0x1p-18)));
+}
+
+// A slab's sum, rounded up, as an int that keeps the order: the largest one over
+// the slabs does not depend on their order, as a sum of them would.
+__device__ __forceinline__ int norm_code(double sum) { return __double2hiint(sum) + 1; }
+__device__ __forceinline__ double norm_of(int code) { return __hiloint2double(code, 0); }
+
 // Operand rows contiguous in K (s_k == 1): one block per (row, batch), of
 // 256 threads, or 512 for rows longer than 4096.  An f64 row of at most 16
 // values per thread at a 16-byte aligned address is read into registers
@@ -312,19 +330,25 @@ __host__ __device__ constexpr int split_rows_threads(int64_t K) {
   return K > 4096 && K <= 16 * kSplitRowsMaxThreads ? kSplitRowsMaxThreads : 256;
 }
 
+//
+// kNorm: norm[b rows_pad + r] also takes the row's part of the certificate
+// (certify_part).
+template <bool kNorm = false>
 __device__ __forceinline__ void split_rows_body(const DotOperand& o, int64_t rows, int64_t K,
                                                 int64_t rows_pad, int64_t Kp, int64_t batch,
                                                 int P, uint8_t* __restrict__ planes,
-                                                int* __restrict__ shifts, int64_t r, int64_t b) {
+                                                int* __restrict__ shifts, int64_t r, int64_t b,
+                                                float* norm = nullptr) {
   __shared__ double s_max[kSplitRowsMaxThreads / 32];
   __shared__ int s_bad[kSplitRowsMaxThreads / 32];
+  __shared__ double s_sum[kNorm ? kSplitRowsMaxThreads / 32 : 1];
   const bool live = r < rows;
   const int64_t base = b * o.s_b + r * o.s_r;
   const bool vec = o.f64 && o.s_k == 1 && (reinterpret_cast<uintptr_t>(o.f64 + base) & 15) == 0;
   const int64_t group = 4 * static_cast<int64_t>(blockDim.x);  // k covered by one group
   const bool in_regs = vec && K <= 4 * group;
   double v[16];
-  double mx = 0.0;
+  double mx = 0.0, sum = 0.0;
   bool bad = false;
   if (in_regs) {
 #pragma unroll
@@ -347,22 +371,26 @@ __device__ __forceinline__ void split_rows_body(const DotOperand& o, int64_t row
     for (int j = 0; j < 16; ++j) {
       bad |= !isfinite(v[j]);
       mx = fmax(mx, fabs(v[j]));
+      if constexpr (kNorm) sum += fabs(v[j]);
     }
   } else if (live) {
     for (int64_t k = threadIdx.x; k < K; k += blockDim.x) {
       const double x = op_value(o, base + k * o.s_k);
       bad |= !isfinite(x);
       mx = fmax(mx, fabs(x));
+      if constexpr (kNorm) sum += fabs(x);
     }
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
     mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, d));
     bad |= __shfl_xor_sync(0xffffffffu, static_cast<int>(bad), d) != 0;
+    if constexpr (kNorm) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   }
   if ((threadIdx.x & 31) == 0) {
     s_max[threadIdx.x >> 5] = mx;
     s_bad[threadIdx.x >> 5] = bad;
+    if constexpr (kNorm) s_sum[threadIdx.x >> 5] = sum;
   }
   __syncthreads();
   mx = 0.0;
@@ -372,7 +400,14 @@ __device__ __forceinline__ void split_rows_body(const DotOperand& o, int64_t row
     bad |= s_bad[w] != 0;
   }
   const int shift = live ? shift_for(mx, bad, P) : 0;
-  if (threadIdx.x == 0) shifts[b * rows_pad + r] = shift;
+  if (threadIdx.x == 0) {
+    shifts[b * rows_pad + r] = shift;
+    if constexpr (kNorm) {
+      double all = 0.0;
+      for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) all += s_sum[w];
+      norm[b * rows_pad + r] = certify_part(all, shift, K);
+    }
+  }
   const bool zero = !live || shift == kShiftNonFinite || shift == kShiftZero;
   const int sh = zero ? 0 : shift;
   const size_t plane_stride = static_cast<size_t>(batch) * rows_pad * Kp;
@@ -458,11 +493,17 @@ __device__ __forceinline__ void load_row_pair(const DotOperand& o, bool paired, 
 // across blocks with atomicMax on an encoded exponent (codes start at 0).
 constexpr int kColmaxSlab = 128;
 
+// kNorm: norm_codes also takes the largest slab sum of each row's magnitudes
+// (norm_code).
+template <bool kNorm = false>
 __device__ __forceinline__ void colmax_body(const DotOperand& o, int64_t rows, int64_t K,
                                             int64_t rows_pad, int* __restrict__ codes,
-                                            int64_t bx, int64_t by, int64_t b) {
+                                            int64_t bx, int64_t by, int64_t b,
+                                            int* __restrict__ norm_codes = nullptr) {
   __shared__ double s_max[8][kColTileR];
   __shared__ int s_bad[8][kColTileR];
+  __shared__ double s_sum[kNorm ? 8 : 1][kColTileR];
+  double n0 = 0.0, n1 = 0.0;
   const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t r0 = bx * kColTileR;
   const int64_t row = r0 + 2 * lane;
@@ -479,6 +520,10 @@ __device__ __forceinline__ void colmax_body(const DotOperand& o, int64_t rows, i
       bad1 |= !isfinite(d.y);
       m0 = fmax(m0, fabs(d.x));
       m1 = fmax(m1, fabs(d.y));
+      if constexpr (kNorm) {
+        n0 += fabs(d.x);
+        n1 += fabs(d.y);
+      }
     }
   } else {
     for (int64_t k = k0 + ty; k < k1; k += 8) {
@@ -488,12 +533,20 @@ __device__ __forceinline__ void colmax_body(const DotOperand& o, int64_t rows, i
       bad1 |= !isfinite(x1);
       m0 = fmax(m0, fabs(x0));
       m1 = fmax(m1, fabs(x1));
+      if constexpr (kNorm) {
+        n0 += fabs(x0);
+        n1 += fabs(x1);
+      }
     }
   }
   s_max[ty][2 * lane] = m0;
   s_max[ty][2 * lane + 1] = m1;
   s_bad[ty][2 * lane] = bad;
   s_bad[ty][2 * lane + 1] = bad1;
+  if constexpr (kNorm) {
+    s_sum[ty][2 * lane] = n0;
+    s_sum[ty][2 * lane + 1] = n1;
+  }
   __syncthreads();
   if (threadIdx.x < kColTileR) {
     const int64_t r = r0 + threadIdx.x;
@@ -505,6 +558,11 @@ __device__ __forceinline__ void colmax_body(const DotOperand& o, int64_t rows, i
     }
     const int code = nf ? kExpNonFinite : (mx == 0.0 ? 0 : ilogb(mx) + 1 + kExpBias);
     if (r < rows && code != 0) atomicMax(&codes[b * rows_pad + r], code);
+    if constexpr (kNorm) {
+      double sum = 0.0;
+      for (int w = 0; w < 8; ++w) sum += s_sum[w][threadIdx.x];
+      if (r < rows && sum > 0.0) atomicMax(&norm_codes[b * rows_pad + r], norm_code(sum));
+    }
   }
 }
 
@@ -1128,7 +1186,6 @@ __device__ __forceinline__ double pow2_normal(int e) {
 // fails exactly where those maxima do not take part in the output: a large
 // entry facing zeros, values spread over many binades, or cancellation.
 // Such outputs are recomputed with a compensated dot product (fix_kernel).
-constexpr int kCertifyBits = 24;
 
 __device__ __forceinline__ bool shift_ordinary(int s) {
   return s != kShiftNonFinite && s != kShiftZero;

@@ -78,61 +78,56 @@ __device__ __forceinline__ int64_t owner_of(const int32_t* start, int64_t G, int
   return lo;
 }
 
-// One block: the groups' first rows inside [begin, end) of the call's rows (a
-// negative size counts as 0, no group passes row M), and the tiles of the two
-// kinds of groups.
-__global__ void __launch_bounds__(kPrepThreads)
-prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t begin, int64_t end,
-            RaggedPlan p) {
-  wait_previous_grid();
-  const int64_t tid = threadIdx.x;
-  int64_t rows_before = 0, tiles_before = 0, slots_before = 0;
-  for (int64_t g0 = 0; g0 < G; g0 += kPrepThreads) {
-    const int64_t g = g0 + tid;
-    const int64_t n = g < G && sizes[g] > 0 ? sizes[g] : 0;
-    int64_t sum, tsum, ssum;
-    int64_t lo = rows_before + block_scan(n, sum), hi = lo + n;
-    rows_before += sum;
-    // the group's rows inside the call's window
-    auto clip = [&](int64_t r) {
-      r = r < M ? r : M;
-      return r < begin ? begin : r > end ? end : r;
-    };
-    lo = clip(lo);
-    hi = clip(hi);
-    const int64_t rows = hi - lo;
-    const bool tensor = rows >= p.tensor_rows;
-    const int64_t d = tensor ? 0 : (rows + kSmallTile - 1) / kSmallTile;
-    const int64_t t = tensor ? (rows + kTensorTile - 1) / kTensorTile : 0;
-    // both counts stay below 2^31
-    const int64_t both = tiles_before + block_scan(d << 32 | t, tsum);
-    tiles_before += tsum;
-    const int64_t slot = slots_before + block_scan(tensor, ssum);
-    slots_before += ssum;
-    if (g < G) {
-      p.row[g] = static_cast<int32_t>(lo);
-      p.small_start[g] = static_cast<int32_t>(both >> 32);
-      p.tensor_start[g] = static_cast<int32_t>(both & 0xffffffff);
-      p.slot[g] = static_cast<int32_t>(slot);
-      if (tensor) {
-        int bits = 50;
-        for (int i = 0; i < kBitsLimits && rows > p.bits_limit[i]; ++i) --bits;
-        p.slot_group[slot] = static_cast<int32_t>(g);
-        p.slot_bits[slot] = bits;
-      }
-      if (g == G - 1) {
-        p.row[G] = static_cast<int32_t>(hi);
-        p.small_start[G] = static_cast<int32_t>((both >> 32) + d);
-        p.tensor_start[G] = static_cast<int32_t>((both & 0xffffffff) + t);
-        p.slot[G] = static_cast<int32_t>(slot + tensor);
-      }
-    }
+// A group's rows inside [begin, end) of the call's rows, given its first row and
+// number (a negative one counts as 0; no group passes row M), and its tiles.
+struct GroupShape {
+  int32_t row, end, small, tensor;  // tiles of its kind; 0 of the other
+  bool large;
+};
+
+__device__ __forceinline__ GroupShape shape_of(int64_t first, int64_t n, int64_t M, int64_t begin,
+                                               int64_t end, const RaggedPlan& p) {
+  auto clip = [&](int64_t r) {
+    r = r < M ? r : M;
+    return r < begin ? begin : r > end ? end : r;
+  };
+  const int64_t lo = clip(first), hi = clip(first + n), rows = hi - lo;
+  GroupShape g;
+  g.row = static_cast<int32_t>(lo);
+  g.end = static_cast<int32_t>(hi);
+  g.large = rows >= p.tensor_rows;
+  g.small = g.large ? 0 : static_cast<int32_t>((rows + kSmallTile - 1) / kSmallTile);
+  g.tensor = g.large ? static_cast<int32_t>((rows + kTensorTile - 1) / kTensorTile) : 0;
+  return g;
+}
+
+// Writes group g's places, given the small tiles, large tiles and large groups
+// before it.
+__device__ __forceinline__ void put_group(const RaggedPlan& p, int64_t g, const GroupShape& x,
+                                          int64_t small, int64_t tensor, int64_t slot) {
+  p.row[g] = x.row;
+  p.small_start[g] = static_cast<int32_t>(small);
+  p.tensor_start[g] = static_cast<int32_t>(tensor);
+  p.slot[g] = static_cast<int32_t>(slot);
+  if (x.large) {
+    int bits = 50;
+    for (int i = 0; i < kBitsLimits && x.end - x.row > p.bits_limit[i]; ++i) --bits;
+    p.slot_group[slot] = static_cast<int32_t>(g);
+    p.slot_bits[slot] = bits;
   }
-  if (G == 0 && tid == 0) p.row[0] = p.small_start[0] = p.tensor_start[0] = p.slot[0] = 0;
-  __syncthreads();
+  if (g == p.groups - 1) {
+    p.row[g + 1] = x.end;
+    p.small_start[g + 1] = static_cast<int32_t>(small + x.small);
+    p.tensor_start[g + 1] = static_cast<int32_t>(tensor + x.tensor);
+    p.slot[g + 1] = static_cast<int32_t>(slot + x.large);
+  }
+}
+
+// The tile tables and the groups' order, from what put_group wrote.
+__device__ void put_tables(const RaggedPlan& p, int64_t G, int64_t tid, int64_t threads) {
   // the groups by falling number of rows
   if (p.order) {
-    for (int64_t g = tid; g < G; g += kPrepThreads) {
+    for (int64_t g = tid; g < G; g += threads) {
       const int32_t n = p.row[g + 1] - p.row[g];
       int32_t rank = static_cast<int32_t>(g);
       if (G <= kOrderedGroups) {
@@ -147,7 +142,7 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
   }
   auto fill = [&](const int32_t* start, int tile, RaggedTile* out, int64_t cap) {
     const int64_t n = start[G] < cap ? start[G] : cap;
-    for (int64_t t = tid; t < n; t += kPrepThreads) {
+    for (int64_t t = tid; t < n; t += threads) {
       const int64_t g = owner_of(start, G, static_cast<int32_t>(t));
       const int32_t row = p.row[g] + static_cast<int32_t>(t - start[g]) * tile;
       const int32_t left = p.row[g + 1] - row;
@@ -156,6 +151,61 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
   };
   if (p.small) fill(p.small_start, kSmallTile, p.small, p.small_cap);
   if (p.tensor) fill(p.tensor_start, kTensorTile, p.tensor, p.tensor_cap);
+}
+
+// One block for any number of groups.
+__global__ void __launch_bounds__(kPrepThreads)
+prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t begin, int64_t end,
+            RaggedPlan p) {
+  wait_previous_grid();
+  const int64_t tid = threadIdx.x;
+  int64_t rows_before = 0, tiles_before = 0, slots_before = 0;
+  for (int64_t g0 = 0; g0 < G; g0 += kPrepThreads) {
+    const int64_t g = g0 + tid;
+    const int64_t n = g < G && sizes[g] > 0 ? sizes[g] : 0;
+    int64_t rows, tiles, slots;
+    const GroupShape x = shape_of(rows_before + block_scan(n, rows), n, M, begin, end, p);
+    // both counts stay below 2^31
+    const int64_t both =
+        tiles_before + block_scan(static_cast<int64_t>(x.small) << 32 | x.tensor, tiles);
+    const int64_t slot = slots_before + block_scan(x.large, slots);
+    rows_before += rows;
+    tiles_before += tiles;
+    slots_before += slots;
+    if (g < G) put_group(p, g, x, both >> 32, both & 0xffffffff, slot);
+  }
+  if (G == 0 && tid == 0) p.row[0] = p.small_start[0] = p.tensor_start[0] = p.slot[0] = 0;
+  __syncthreads();
+  put_tables(p, G, tid, kPrepThreads);
+}
+
+// The same for at most 32 groups, by one warp's shuffles (3.6 us instead of 5.3).
+constexpr int kPrepFewThreads = 128;
+
+__global__ void __launch_bounds__(kPrepFewThreads)
+prep_few_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t begin,
+                int64_t end, RaggedPlan p) {
+  wait_previous_grid();
+  const int lane = threadIdx.x;
+  if (lane < 32) {
+    const int64_t n = lane < G && sizes[lane] > 0 ? sizes[lane] : 0;
+    auto before = [&](int64_t v) {
+      int64_t x = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      return x - v;
+    };
+    const GroupShape x = shape_of(before(n), n, M, begin, end, p);
+    const int64_t both = before(static_cast<int64_t>(x.small) << 32 | x.tensor);
+    const int slot = __popc(__ballot_sync(0xffffffffu, x.large) & ((1u << lane) - 1u));
+    if (lane < G) put_group(p, lane, x, both >> 32, both & 0xffffffff, slot);
+    if (G == 0 && lane == 0) p.row[0] = p.small_start[0] = p.tensor_start[0] = p.slot[0] = 0;
+  }
+  __syncthreads();
+  put_tables(p, G, threadIdx.x, kPrepFewThreads);
 }
 
 // ---- small groups: FP64 matrix instructions ---------------------------------------
@@ -737,7 +787,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // resident blocks (more when no tile has over 16 rows: those only stream the
 // matrices).  From the call's sizes alone, so a row's rounding does not depend
 // on other groups.
-constexpr int64_t kSplitMin = 128;
+constexpr int64_t kSplitMin = 256;
 constexpr int kMaxSplits = 16;
 
 int splits_of(int64_t M, int64_t K, int64_t N, int64_t G) {
@@ -921,8 +971,12 @@ int launch_products(const SmallArgs& a, int64_t units, cudaStream_t s) {
 
 int launch_prep(const RaggedProblem& q, int64_t begin, int64_t end, const RaggedPlan& p,
                 cudaStream_t s) {
-  DSB_CUDA_TRY(launch_dependent(prep_kernel, dim3(1), dim3(kPrepThreads), s, q.group_sizes, q.G,
-                                q.M, begin, end, p));
+  if (q.G <= 32)
+    DSB_CUDA_TRY(launch_dependent(prep_few_kernel, dim3(1), dim3(kPrepFewThreads), s,
+                                  q.group_sizes, q.G, q.M, begin, end, p));
+  else
+    DSB_CUDA_TRY(launch_dependent(prep_kernel, dim3(1), dim3(kPrepThreads), s, q.group_sizes, q.G,
+                                  q.M, begin, end, p));
   return launch_status();
 }
 

@@ -45,58 +45,74 @@ __device__ __forceinline__ int slots_of(const RaggedPlan& p) { return p.slot[p.g
 
 // ---- split ---------------------------------------------------------------------
 
+struct RowSplit {
+  DotOperand o;
+  int64_t M, K, Mp, Kp;
+  int P;
+  uint8_t* planes;
+  int* shifts;
+  int* row_slot;
+  float* part;
+};
+
 // Rows of the large groups, one block each: blockIdx.y is the row in tile
-// blockIdx.x.
+// blockIdx.x.  (In one launch with the column maxima of the matrices, their
+// blocks interleaved, it took as long as both.)
 __global__ void __launch_bounds__(kSplitRowsMaxThreads, 2)
-ragged_split_rows_kernel(DotOperand o, int64_t M, int64_t K, int64_t Mp, int64_t Kp, int P,
-                         RaggedPlan p, uint8_t* __restrict__ planes, int* __restrict__ shifts,
-                         int* __restrict__ row_slot) {
+ragged_split_rows_kernel(RowSplit r, RaggedPlan p) {
   wait_previous_grid();
   if (static_cast<int>(blockIdx.x) >= p.tensor_start[p.groups]) return;
   const RaggedTile t = p.tensor[blockIdx.x];
   if (static_cast<int>(blockIdx.y) >= t.rows) return;
-  const int64_t row = t.row + static_cast<int>(blockIdx.y);
-  if (threadIdx.x == 0) row_slot[row] = t.slot + 1;
-  split_rows_body(o, M, K, Mp, Kp, 1, P, planes, shifts, row, 0);
+  const int64_t at = t.row + static_cast<int64_t>(blockIdx.y);
+  if (threadIdx.x == 0) r.row_slot[at] = t.slot + 1;
+  split_rows_body<true>(r.o, r.M, r.K, r.Mp, r.Kp, 1, r.P, r.planes, r.shifts, at, 0, r.part);
 }
 
 // Matrices with K contiguous ([G, N, K]): column blockIdx.x of slot blockIdx.y.
 __global__ void __launch_bounds__(kSplitRowsMaxThreads, 2)
 ragged_split_matrix_rows_kernel(DotOperand o, int64_t N, int64_t K, int64_t Np, int64_t Kp,
                                 int64_t slots, int P, RaggedPlan p, uint8_t* __restrict__ planes,
-                                int* __restrict__ shifts) {
+                                int* __restrict__ shifts, float* __restrict__ part) {
   wait_previous_grid();
   const int slot = blockIdx.y;
   if (slot >= slots_of(p)) return;
   DotOperand x = moved(o, p.slot_group[slot] * o.s_b);
   x.s_b = 0;
-  split_rows_body(x, N, K, Np, Kp, slots, P, planes, shifts, blockIdx.x, slot);
+  split_rows_body<true>(x, N, K, Np, Kp, slots, P, planes, shifts, blockIdx.x, slot, part);
 }
+
+struct ColumnMax {
+  DotOperand o;
+  int64_t N, K, Np;
+  int* codes;
+  int* norms;
+};
 
 // Column maxima of the matrices ([G, K, N]): slot blockIdx.z.
 __global__ void __launch_bounds__(256, 6)
-ragged_colmax_kernel(DotOperand o, int64_t N, int64_t K, int64_t Np, RaggedPlan p,
-                     int* __restrict__ codes) {
+ragged_colmax_kernel(ColumnMax c, RaggedPlan p) {
   wait_previous_grid();
   const int slot = blockIdx.z;
   if (slot >= slots_of(p)) return;
-  DotOperand x = moved(o, p.slot_group[slot] * o.s_b);
+  DotOperand x = moved(c.o, p.slot_group[slot] * c.o.s_b);
   x.s_b = 0;
-  colmax_body(x, N, K, Np, codes, blockIdx.x, blockIdx.y, slot);
+  colmax_body<true>(x, c.N, c.K, c.Np, c.codes, blockIdx.x, blockIdx.y, slot, c.norms);
 }
 
 // The same per group and feature of a contraction's operand: half blockIdx.y
 // % 2 of tile blockIdx.y / 2.
 __global__ void __launch_bounds__(256, 6)
 ragged_tile_colmax_kernel(DotOperand o, int64_t F, int64_t Fp, RaggedPlan p,
-                          int* __restrict__ codes) {
+                          int* __restrict__ codes, int* __restrict__ norms) {
   wait_previous_grid();
   const int tile = blockIdx.y >> 1;
   if (tile >= p.tensor_start[p.groups]) return;
   const RaggedTile t = p.tensor[tile];
   if (static_cast<int>(blockIdx.y & 1) * kColmaxSlab >= t.rows) return;
-  colmax_body(moved(o, t.row * o.s_k), F, t.rows, Fp, codes + static_cast<int64_t>(t.slot) * Fp,
-              blockIdx.x, blockIdx.y & 1, 0);
+  const int64_t at = static_cast<int64_t>(t.slot) * Fp;
+  colmax_body<true>(moved(o, t.row * o.s_k), F, t.rows, Fp, codes + at, blockIdx.x,
+                    blockIdx.y & 1, 0, norms + at);
 }
 
 // DS pairs into row-contiguous planes, as split_mn_async_body does for f64:
@@ -141,15 +157,34 @@ __device__ __forceinline__ void split_mn_body(const DotOperand& o, int64_t rows,
     split_mn_async_body(o, 0, true, rows, K, rows_pad, Kp, P, codes, planes, plane_stride, shifts);
 }
 
+// Certificate parts of this thread's columns, from the column maxima's codes, by
+// the blocks that start at k = 0.
+__device__ __forceinline__ void column_parts(int64_t rows, int64_t rows_pad, int64_t K, int P,
+                                             const int* __restrict__ codes,
+                                             const int* __restrict__ norms,
+                                             float* __restrict__ part) {
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kMnRows + threadIdx.x * kMnCols;
+  if (blockIdx.y != 0 || r0 >= rows_pad) return;
+  const double slabs = static_cast<double>((K + kColmaxSlab - 1) / kColmaxSlab);
+#pragma unroll
+  for (int j = 0; j < kMnCols; ++j) {
+    const int64_t r = r0 + j;
+    part[r] = r < rows ? certify_part(slabs * norm_of(norms[r]), shift_from_code(codes[r], P), K)
+                       : 0.0f;
+  }
+}
+
 // Matrices [G, K, N] into planes [14][slots][Kp][Np]: slot blockIdx.z.
 template <bool kPair>
 __global__ void __launch_bounds__(256, 2)
 ragged_split_matrix_kernel(DotOperand o, int64_t N, int64_t K, int64_t Np, int64_t Kp,
                            int64_t slots, int P, RaggedPlan p, const int* __restrict__ codes,
-                           uint8_t* __restrict__ planes, int* __restrict__ shifts) {
+                           const int* __restrict__ norms, uint8_t* __restrict__ planes,
+                           int* __restrict__ shifts, float* __restrict__ part) {
   wait_previous_grid();
   const int64_t slot = blockIdx.z;
   if (slot >= slots_of(p)) return;
+  column_parts(N, Np, K, P, codes + slot * Np, norms + slot * Np, part + slot * Np);
   split_mn_body<kPair>(moved(o, p.slot_group[slot] * o.s_b), N, K, Np, Kp, P, codes + slot * Np,
                        planes + static_cast<size_t>(slot) * Kp * Np,
                        static_cast<size_t>(slots) * Kp * Np, shifts + slot * Np);
@@ -159,12 +194,17 @@ ragged_split_matrix_kernel(DotOperand o, int64_t N, int64_t K, int64_t Np, int64
 template <bool kPair>
 __global__ void __launch_bounds__(256, 2)
 ragged_split_tiles_kernel(DotOperand o, int64_t F, int64_t Fp, int64_t positions, RaggedPlan p,
-                          const int* __restrict__ codes, uint8_t* __restrict__ planes,
-                          int* __restrict__ shifts) {
+                          const int* __restrict__ codes, const int* __restrict__ norms,
+                          uint8_t* __restrict__ planes, int* __restrict__ shifts,
+                          float* __restrict__ part) {
   wait_previous_grid();
   const int tile = blockIdx.z;
   if (tile >= p.tensor_start[p.groups]) return;
   const RaggedTile t = p.tensor[tile];
+  const int64_t at = static_cast<int64_t>(t.slot) * Fp;
+  if (tile == p.tensor_start[t.group])
+    column_parts(F, Fp, p.row[t.group + 1] - p.row[t.group], p.slot_bits[t.slot], codes + at,
+                 norms + at, part + at);
   split_mn_body<kPair>(moved(o, t.row * o.s_k), F, t.rows, Fp, kTensorTile, p.slot_bits[t.slot],
                        codes + t.slot * Fp,
                        planes + static_cast<size_t>(tile) * kTensorTile * Fp,
@@ -269,6 +309,8 @@ struct RaggedCrt {
   const uint8_t* cres;
   const int* sa;
   const int* sb;
+  const float* pa;       // certificate parts of the rows and columns
+  const float* pb;
   const int* row_slot;   // products: slot + 1 of each row
   const int* err;
   int* fix_count;
@@ -283,11 +325,12 @@ struct RowView {
   int64_t residues;      // row of the residue planes
   int64_t out;           // row of the result
   int64_t a, b, K;       // first elements and length of the contraction
-  double certify_below;
+  double part;           // of the certificate: without the column's
 };
 
-__device__ __forceinline__ double certify_below(int64_t K, int P) {
-  return (static_cast<double>(K) * pow2_normal(P) + 0x1p35) * pow2_normal(kCertifyBits);
+// The certificate's K / 4 and the low limb's rounding.
+__device__ __forceinline__ double certify_rest(int64_t K) {
+  return (0.25 * static_cast<double>(K) + 0x1p35) * pow2_normal(kCertifyBits);
 }
 
 template <bool kContract>
@@ -322,7 +365,7 @@ __device__ __forceinline__ RowView view(const RaggedCrt& p, int64_t row) {
     v.P = p.P;
     v.sa = p.sa[row];
   }
-  v.certify_below = certify_below(v.K, v.P);
+  v.part = certify_rest(v.K) + static_cast<double>(p.pa[v.residues]);
   return v;
 }
 
@@ -362,6 +405,8 @@ ragged_crt_kernel(const __grid_constant__ RaggedCrt p) {
     }
     const int4 sbv = *reinterpret_cast<const int4*>(p.sb + v.slot * p.Np + j0);
     const int sb[kCols] = {sbv.x, sbv.y, sbv.z, sbv.w};
+    const float4 pbv = *reinterpret_cast<const float4*>(p.pb + v.slot * p.Np + j0);
+    const float pb[kCols] = {pbv.x, pbv.y, pbv.z, pbv.w};
     double out[kCols];
     bool put[kCols], all = j0 + kCols <= p.N;
 #pragma unroll
@@ -375,7 +420,7 @@ ragged_crt_kernel(const __grid_constant__ RaggedCrt p) {
         const double t_hi = __fma_rn(-qt, p.mlimb[0], s_hi[q]);
         const double t_lo = __fma_rn(-qt, p.mlimb[1], s_lo[q]);
         const double c = __fma_rn(t_hi, 0x1p70, t_lo);
-        if (put[q] && !(fabs(c) >= v.certify_below)) {
+        if (put[q] && !(fabs(c) >= v.part + static_cast<double>(pb[q]))) {
           // uncertified: listed for ragged_fix_kernel, which writes this output
           put[q] = false;
           const int at = atomicAdd(p.fix_count, 1);
@@ -582,7 +627,7 @@ struct TensorLayout {
   int64_t chunk;            // longest contraction of a chunk
   int64_t Mp, Np, Kp;       // contraction: Kp positions, Mp rows of a matrix
   int64_t slots;
-  size_t a, b, c, sa, sb, clear, ca, cb, err, row_slot, clear_end, list, part, total;
+  size_t a, b, c, sa, sb, pa, pb, clear, ca, cb, na, nb, err, row_slot, clear_end, list, part, total;
   int64_t fix_cap;
 };
 
@@ -619,10 +664,15 @@ TensorLayout tensor_layout(int64_t M, int64_t K, int64_t N, int64_t G, bool cont
   }
   g.sa = take(4 * a_scales);
   g.sb = take(4 * g.slots * g.Np);
-  // cleared together: column codes, error word and count, slots of the rows
+  g.pa = take(4 * a_scales);
+  g.pb = take(4 * g.slots * g.Np);
+  // cleared together: column codes and norms, error word and count, slots of the
+  // rows
   g.clear = at;
   g.ca = take(contract ? 4 * a_scales : 0);
   g.cb = take(4 * g.slots * g.Np);
+  g.na = take(contract ? 4 * a_scales : 0);
+  g.nb = take(4 * g.slots * g.Np);
   g.err = take(16);
   g.row_slot = take(contract ? 0 : 4 * M);
   g.clear_end = at;
@@ -713,7 +763,8 @@ struct TensorRun {
   uint8_t* ws;
   TensorLayout g;
   uint8_t *planes_a, *planes_b;
-  int *sa, *sb, *ca, *cb, *err, *row_slot;
+  int *sa, *sb, *ca, *cb, *na, *nb, *err, *row_slot;
+  float *pa, *pb;
   RaggedCrt crt;
   RaggedGemm gemm;
 };
@@ -729,6 +780,10 @@ TensorRun tensor_run(const RaggedProblem& q, const RaggedPlan& p, const TensorLa
   r.sb = ints(g.sb);
   r.ca = ints(g.ca);
   r.cb = ints(g.cb);
+  r.na = ints(g.na);
+  r.nb = ints(g.nb);
+  r.pa = reinterpret_cast<float*>(r.ws + g.pa);
+  r.pb = reinterpret_cast<float*>(r.ws + g.pb);
   r.err = ints(g.err);
   r.row_slot = ints(g.row_slot);
   const CrtConsts& cc = crt_consts();
@@ -748,6 +803,8 @@ TensorRun tensor_run(const RaggedProblem& q, const RaggedPlan& p, const TensorLa
   r.crt.cres = r.ws + g.c;
   r.crt.sa = r.sa;
   r.crt.sb = r.sb;
+  r.crt.pa = r.pa;
+  r.crt.pb = r.pb;
   r.crt.row_slot = r.row_slot;
   r.crt.err = r.err;
   r.crt.fix_count = r.err + 1;
@@ -801,32 +858,32 @@ int ragged_tensor_dot(const RaggedProblem& q, const RaggedPlan& p, void* workspa
       ProfileScope prof("ozaki_split", s);
       DSB_CUDA_TRY(cudaMemsetAsync(r.ws + g.clear, 0, g.clear_end - g.clear, s));
       const unsigned threads = static_cast<unsigned>(split_rows_threads(K));
-      DSB_CUDA_TRY(launch_dependent(ragged_split_rows_kernel, dim3(tiles, kTensorTile),
-                                    dim3(threads), s, a, q.M, K, g.Mp, Kp, P, p, r.planes_a, r.sa,
-                                    r.row_slot));
+      const RowSplit rows{a, q.M, K, g.Mp, Kp, P, r.planes_a, r.sa, r.row_slot, r.pa};
+      const ColumnMax cols{b, q.N, K, g.Np, r.cb, r.nb};
       const unsigned slots = static_cast<unsigned>(g.slots);
+      const unsigned cgx = static_cast<unsigned>(g.Np / kColTileR);
+      const unsigned cgy = static_cast<unsigned>((K + kColmaxSlab - 1) / kColmaxSlab);
+      DSB_CUDA_TRY(launch_dependent(ragged_split_rows_kernel, dim3(tiles, kTensorTile),
+                                    dim3(threads), s, rows, p));
       if (q.rhs_t) {
         DSB_CUDA_TRY(launch_dependent(ragged_split_matrix_rows_kernel,
                                       dim3(static_cast<unsigned>(g.Np), slots), dim3(threads), s,
-                                      b, q.N, K, g.Np, Kp, g.slots, P, p, r.planes_b, r.sb));
+                                      b, q.N, K, g.Np, Kp, g.slots, P, p, r.planes_b, r.sb, r.pb));
       } else {
-        DSB_CUDA_TRY(launch_dependent(
-            ragged_colmax_kernel,
-            dim3(static_cast<unsigned>(g.Np / kColTileR),
-                 static_cast<unsigned>((K + kColmaxSlab - 1) / kColmaxSlab), slots),
-            dim3(256), s, b, q.N, K, g.Np, p, r.cb));
+        DSB_CUDA_TRY(launch_dependent(ragged_colmax_kernel, dim3(cgx, cgy, slots), dim3(256), s,
+                                      cols, p));
         const int64_t cx = (g.Np + kMnRows - 1) / kMnRows;
         int64_t ky = (2 * static_cast<int64_t>(sm_count()) + cx - 1) / cx;
         ky = ky > Kp / 16 ? Kp / 16 : ky;
         const dim3 grid(static_cast<unsigned>(cx), grid_y(ky), slots);
         if (q.rhs.f64)
           DSB_CUDA_TRY(launch_dependent(ragged_split_matrix_kernel<false>, grid, dim3(256), s, b,
-                                        q.N, K, g.Np, Kp, g.slots, P, p, r.cb, r.planes_b,
-                                        r.sb));
+                                        q.N, K, g.Np, Kp, g.slots, P, p, r.cb, r.nb, r.planes_b,
+                                        r.sb, r.pb));
         else
           DSB_CUDA_TRY(launch_dependent(ragged_split_matrix_kernel<true>, grid, dim3(256), s, b,
-                                        q.N, K, g.Np, Kp, g.slots, P, p, r.cb, r.planes_b,
-                                        r.sb));
+                                        q.N, K, g.Np, Kp, g.slots, P, p, r.cb, r.nb, r.planes_b,
+                                        r.sb, r.pb));
       }
     }
     r.gemm.stages = static_cast<int>((Kp / kTileK + kSub2 - 1) / kSub2);
@@ -856,22 +913,22 @@ int ragged_tensor_contract(const RaggedProblem& q, const RaggedPlan& p, bool add
   {
     ProfileScope prof("ozaki_split", s);
     DSB_CUDA_TRY(cudaMemsetAsync(r.ws + g.clear, 0, g.clear_end - g.clear, s));
-    auto split = [&](const DotOperand& o, int64_t F, int64_t Fp, int* codes, uint8_t* planes,
-                     int* shifts) -> int {
+    auto split = [&](const DotOperand& o, int64_t F, int64_t Fp, int* codes, int* norms,
+                     uint8_t* planes, int* shifts, float* part) -> int {
       DSB_CUDA_TRY(launch_dependent(ragged_tile_colmax_kernel,
                                     dim3(static_cast<unsigned>(Fp / kColTileR), 2 * tiles),
-                                    dim3(256), s, o, F, Fp, p, codes));
+                                    dim3(256), s, o, F, Fp, p, codes, norms));
       const dim3 grid(static_cast<unsigned>((Fp + kMnRows - 1) / kMnRows), 8, tiles);
       if (o.f64)
         DSB_CUDA_TRY(launch_dependent(ragged_split_tiles_kernel<false>, grid, dim3(256), s, o, F,
-                                      Fp, g.Kp, p, codes, planes, shifts));
+                                      Fp, g.Kp, p, codes, norms, planes, shifts, part));
       else
         DSB_CUDA_TRY(launch_dependent(ragged_split_tiles_kernel<true>, grid, dim3(256), s, o, F,
-                                      Fp, g.Kp, p, codes, planes, shifts));
+                                      Fp, g.Kp, p, codes, norms, planes, shifts, part));
       return DS_OK;
     };
-    if (int st = split(q.lhs, q.K, g.Mp, r.ca, r.planes_a, r.sa)) return st;
-    if (int st = split(q.rhs, q.N, g.Np, r.cb, r.planes_b, r.sb)) return st;
+    if (int st = split(q.lhs, q.K, g.Mp, r.ca, r.na, r.planes_a, r.sa, r.pa)) return st;
+    if (int st = split(q.rhs, q.N, g.Np, r.cb, r.nb, r.planes_b, r.sb, r.pb)) return st;
   }
   r.gemm.tiles_m = static_cast<int>(g.Mp / 256);
   if (int st = launch_gemm(ragged_contract_gemm_kernel, clusters, ta, tb, r.gemm, r.err, s))
