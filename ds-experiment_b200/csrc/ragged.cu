@@ -805,23 +805,20 @@ int splits_of(int64_t M, int64_t K, int64_t N, int64_t G) {
 // time is below the FP64 path's.  In microseconds, from measurements on one B200:
 // the FP64 path does 26 TFLOP/s; the tensor-core product has launches of 60 (80)
 // us, splits a value in 6.4 to 8.3 (7) ps, multiplies at 3 POPS of its 28
-// operations per product (a contraction's short units take at least 0.76 us per
-// 256 x 256 outputs), and rebuilds an output in 9 ps.  Measured with / without:
+// operations per product but takes at least 0.76 us per 256 x 256 outputs (short
+// contractions), and rebuilds an output in 9 ps.  Measured with / without:
 // 2048 x 1024 x 1024 in 4 groups 140 / 190 us (contraction 191 / 175), 4096 x 1024
 // x 1024 in 8 groups 224 / 337 (286 / 323), 2048 x 2048 x 2048 in 4 groups 300 /
 // 646 (423 / 624), 8192 x 512 x 512 in 8 groups 198 / 179 (171 / 173).
 bool tensor_allowed(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
   if (M < tensor_rows(contract) || K < 64 || N < 64) return false;
   const double m = M, k = K, n = N, slots = static_cast<double>(ragged_slots(M, G, contract));
-  const double macs = m * k * n, matrices = slots * k * n;
+  const double macs = m * k * n, matrices = slots * k * n, outputs = contract ? matrices : m * n;
   const double plain = 7.7e-8 * macs;
-  double tensor;
-  if (contract) {
-    const double gemm = 9.3e-9 * macs, least = 1.15e-5 * matrices;
-    tensor = 80 + 7e-6 * m * (k + n) + (gemm > least ? gemm : least) + 9e-6 * matrices;
-  } else {
-    tensor = 60 + 6.4e-6 * m * k + 8.3e-6 * matrices + 9.3e-9 * macs + 9e-6 * m * n;
-  }
+  const double gemm = 9.3e-9 * macs, least = 1.15e-5 * outputs;
+  const double split = contract ? 7e-6 * m * (k + n) : 6.4e-6 * m * k + 8.3e-6 * matrices;
+  const double tensor = (contract ? 80 : 60) + split + (gemm > least ? gemm : least) +
+                        9e-6 * outputs;
   return tensor < plain && ragged_tensor_fits(M, K, N, G, contract);
 }
 
