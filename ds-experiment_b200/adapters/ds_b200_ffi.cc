@@ -1,7 +1,8 @@
 // XLA-FFI handlers for libds_b200: the reference's custom-call targets
 // (cpp/*.cpp and cpp/*.cu of rcast915/ds-experiment) re-pointed at the B200
 // library, plus the new targets its retargeted DS pass emits (reduce,
-// dot_general, fused elementwise regions).
+// dot_general, fused elementwise regions), and the recurrence along a sequence
+// and the products grouped by expert with their gradients.
 //
 // Built by adapters/CMakeLists.txt when the XLA-FFI headers are present
 // (jax.ffi.include_dir()); this repository's image has no JAX, so here the
@@ -395,6 +396,168 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(DsDotGeneralF64, DsDotGeneralF64Impl,
                                   .Attr<ffi::Span<const int64_t>>("rhs_contracting_dimensions")
                                   .Attr<int32_t>("algorithm")
                                   .Ret<ffi::Buffer<ffi::F64>>());
+
+// ---- linear recurrence along a sequence, and its gradient ------------------------
+//
+// A custom_vjp rule pairs the two: (a, b, h0) -> h, and (a, h, grad_h, h0) ->
+// (grad_a, grad_b, grad_h0).
+
+using RecurrenceFn = int (*)(const ds_buffer*, const ds_buffer*, const ds_buffer*,
+                             const ds_buffer*, void*, size_t, void*);
+using RecurrenceVjpFn = int (*)(const ds_buffer*, const ds_buffer*, const ds_buffer*,
+                                const ds_buffer*, const ds_buffer*, const ds_buffer*,
+                                const ds_buffer*, void*, size_t, void*);
+
+template <ffi::DataType T, int32_t kType, RecurrenceFn kFn>
+static ffi::Error DsLinearRecurrenceImpl(cudaStream_t s, ffi::ScratchAllocator alloc,
+                                         ffi::Buffer<T> a, ffi::Buffer<T> b, ffi::Buffer<T> h0,
+                                         ffi::ResultBuffer<T> h) {
+  View A(a), B(b), H0(h0), H(*h);
+  const size_t need = ds_linear_recurrence_workspace_size(A.get(), kType);
+  auto ws = scratch(alloc, need);
+  if (!ws) return no_scratch("ds_linear_recurrence");
+  return status(kFn(A.get(), B.get(), H0.get(), H.get(), *ws, need, s));
+}
+
+template <ffi::DataType T, int32_t kType, RecurrenceVjpFn kFn>
+static ffi::Error DsLinearRecurrenceVjpImpl(cudaStream_t s, ffi::ScratchAllocator alloc,
+                                            ffi::Buffer<T> a, ffi::Buffer<T> h,
+                                            ffi::Buffer<T> grad_h, ffi::Buffer<T> h0,
+                                            ffi::ResultBuffer<T> grad_a,
+                                            ffi::ResultBuffer<T> grad_b,
+                                            ffi::ResultBuffer<T> grad_h0) {
+  View A(a), H(h), G(grad_h), H0(h0), GA(*grad_a), GB(*grad_b), GH(*grad_h0);
+  const size_t need = ds_linear_recurrence_workspace_size(A.get(), kType);
+  auto ws = scratch(alloc, need);
+  if (!ws) return no_scratch("ds_linear_recurrence_vjp");
+  return status(kFn(A.get(), H.get(), G.get(), H0.get(), GA.get(), GB.get(), GH.get(), *ws, need,
+                    s));
+}
+
+#define DS_RECURRENCE_HANDLERS(Name, T, kType, fn, vjp_fn)                                    \
+  XLA_FFI_DEFINE_HANDLER_SYMBOL(DsLinearRecurrence##Name,                                     \
+                                (DsLinearRecurrenceImpl<T, kType, fn>),                       \
+                                ffi::Ffi::Bind()                                              \
+                                    .Ctx<ffi::PlatformStream<cudaStream_t>>()                 \
+                                    .Ctx<ffi::ScratchAllocator>()                             \
+                                    .Arg<ffi::Buffer<T>>()                                    \
+                                    .Arg<ffi::Buffer<T>>()                                    \
+                                    .Arg<ffi::Buffer<T>>()                                    \
+                                    .Ret<ffi::Buffer<T>>());                                  \
+  XLA_FFI_DEFINE_HANDLER_SYMBOL(DsLinearRecurrenceVjp##Name,                                  \
+                                (DsLinearRecurrenceVjpImpl<T, kType, vjp_fn>),                \
+                                ffi::Ffi::Bind()                                              \
+                                    .Ctx<ffi::PlatformStream<cudaStream_t>>()                 \
+                                    .Ctx<ffi::ScratchAllocator>()                             \
+                                    .Arg<ffi::Buffer<T>>()                                    \
+                                    .Arg<ffi::Buffer<T>>()                                    \
+                                    .Arg<ffi::Buffer<T>>()                                    \
+                                    .Arg<ffi::Buffer<T>>()                                    \
+                                    .Ret<ffi::Buffer<T>>()                                    \
+                                    .Ret<ffi::Buffer<T>>()                                    \
+                                    .Ret<ffi::Buffer<T>>())
+
+DS_RECURRENCE_HANDLERS(F64, ffi::F64, DS_FUSED_F64, ds_linear_recurrence_f64,
+                       ds_linear_recurrence_vjp_f64);
+DS_RECURRENCE_HANDLERS(F32, ffi::F32, DS_FUSED_F32, ds_linear_recurrence_f32,
+                       ds_linear_recurrence_vjp_f32);
+DS_RECURRENCE_HANDLERS(Packed, ffi::F32, DS_FUSED_PACKED, ds_linear_recurrence_packed,
+                       ds_linear_recurrence_vjp_packed);
+
+// ---- products grouped by expert (jax.lax.ragged_dot's form) ------------------------
+
+static ffi::Error DsRaggedDotF64Impl(cudaStream_t s, ffi::ScratchAllocator alloc,
+                                     ffi::Buffer<ffi::F64> lhs, ffi::Buffer<ffi::F64> rhs,
+                                     ffi::Buffer<ffi::S32> group_sizes, int32_t rhs_contracting,
+                                     ffi::ResultBuffer<ffi::F64> out) {
+  View L(lhs), R(rhs), G(group_sizes), O(*out);
+  const size_t need = ds_ragged_dot_workspace_size(L.get(), R.get(), rhs_contracting);
+  auto ws = scratch(alloc, need);
+  if (!ws) return no_scratch("ds_ragged_dot_f64");
+  return status(
+      ds_ragged_dot_f64(L.get(), R.get(), G.get(), rhs_contracting, O.get(), *ws, need, s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(DsRaggedDotF64, DsRaggedDotF64Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Ctx<ffi::ScratchAllocator>()
+                                  .Arg<ffi::Buffer<ffi::F64>>()
+                                  .Arg<ffi::Buffer<ffi::F64>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Attr<int32_t>("rhs_contracting")
+                                  .Ret<ffi::Buffer<ffi::F64>>());
+
+static ffi::Error DsRaggedDotImpl(cudaStream_t s, ffi::ScratchAllocator alloc,
+                                  ffi::Buffer<ffi::F32> lhs_hi, ffi::Buffer<ffi::F32> lhs_lo,
+                                  ffi::Buffer<ffi::F32> rhs_hi, ffi::Buffer<ffi::F32> rhs_lo,
+                                  ffi::Buffer<ffi::S32> group_sizes, int32_t rhs_contracting,
+                                  ffi::ResultBuffer<ffi::F32> out_hi,
+                                  ffi::ResultBuffer<ffi::F32> out_lo) {
+  View LH(lhs_hi), LL(lhs_lo), RH(rhs_hi), RL(rhs_lo), G(group_sizes), OH(*out_hi), OL(*out_lo);
+  const size_t need = ds_ragged_dot_workspace_size(LH.get(), RH.get(), rhs_contracting);
+  auto ws = scratch(alloc, need);
+  if (!ws) return no_scratch("ds_ragged_dot");
+  return status(ds_ragged_dot(LH.get(), LL.get(), RH.get(), RL.get(), G.get(), rhs_contracting,
+                              OH.get(), OL.get(), *ws, need, s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(DsRaggedDot, DsRaggedDotImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Ctx<ffi::ScratchAllocator>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Attr<int32_t>("rhs_contracting")
+                                  .Ret<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
+
+static ffi::Error DsRaggedDotContractF64Impl(cudaStream_t s, ffi::ScratchAllocator alloc,
+                                             ffi::Buffer<ffi::F64> lhs, ffi::Buffer<ffi::F64> rhs,
+                                             ffi::Buffer<ffi::S32> group_sizes,
+                                             ffi::ResultBuffer<ffi::F64> out) {
+  View L(lhs), R(rhs), G(group_sizes), O(*out);
+  const size_t need = ds_ragged_dot_contract_workspace_size(L.get(), R.get(), G.get());
+  auto ws = scratch(alloc, need);
+  if (!ws) return no_scratch("ds_ragged_dot_contract_f64");
+  return status(ds_ragged_dot_contract_f64(L.get(), R.get(), G.get(), O.get(), *ws, need, s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(DsRaggedDotContractF64, DsRaggedDotContractF64Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Ctx<ffi::ScratchAllocator>()
+                                  .Arg<ffi::Buffer<ffi::F64>>()
+                                  .Arg<ffi::Buffer<ffi::F64>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Ret<ffi::Buffer<ffi::F64>>());
+
+static ffi::Error DsRaggedDotContractImpl(cudaStream_t s, ffi::ScratchAllocator alloc,
+                                          ffi::Buffer<ffi::F32> lhs_hi,
+                                          ffi::Buffer<ffi::F32> lhs_lo,
+                                          ffi::Buffer<ffi::F32> rhs_hi,
+                                          ffi::Buffer<ffi::F32> rhs_lo,
+                                          ffi::Buffer<ffi::S32> group_sizes,
+                                          ffi::ResultBuffer<ffi::F32> out_hi,
+                                          ffi::ResultBuffer<ffi::F32> out_lo) {
+  View LH(lhs_hi), LL(lhs_lo), RH(rhs_hi), RL(rhs_lo), G(group_sizes), OH(*out_hi), OL(*out_lo);
+  const size_t need = ds_ragged_dot_contract_workspace_size(LH.get(), RH.get(), G.get());
+  auto ws = scratch(alloc, need);
+  if (!ws) return no_scratch("ds_ragged_dot_contract");
+  return status(ds_ragged_dot_contract(LH.get(), LL.get(), RH.get(), RL.get(), G.get(), OH.get(),
+                                       OL.get(), *ws, need, s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(DsRaggedDotContract, DsRaggedDotContractImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<cudaStream_t>>()
+                                  .Ctx<ffi::ScratchAllocator>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
 
 // ---- fused elementwise regions (one kernel per region) --------------------------
 //

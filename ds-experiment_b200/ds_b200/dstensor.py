@@ -13,6 +13,8 @@ torch f64/f32 tensors and Python numbers build an expression, and the
 expression runs as ONE generated kernel (`ds_b200.fuse`) when the value is
 needed -- `packed`, `to_f64()`, `to_f32()`, `sum()`, `matmul()` -- with the
 same DS operations, in the same order, as one target call per operation.
+`linear_recurrence` and `ragged_matmul` take the recurrence along a sequence
+and the products grouped by expert.
 
     a = DSTensor.from_f64(x)
     b = (a + y) * a - 0.1          # nothing runs yet
@@ -193,6 +195,23 @@ class DSTensor:
         return DSTensor.from_f64(ops.ds_matmul_f64(self.to_f64(), other.to_f64()))
 
     __matmul__ = matmul
+
+    def ragged_matmul(self, other: "DSTensor", group_sizes: torch.Tensor) -> "DSTensor":
+        """Rows of consecutive groups, each times its group's matrix: self [M, K],
+        other [G, K, N], int32 group_sizes [G] on the device (ds_ragged_dot)."""
+        if not isinstance(other, DSTensor):
+            raise TypeError("ragged_matmul takes a DSTensor")
+        return DSTensor.from_f64(ops.ds_ragged_dot_f64(self.to_f64(), other.to_f64(),
+                                                       group_sizes))
+
+    def linear_recurrence(self, b: "DSTensor", h0: "DSTensor" = None) -> "DSTensor":
+        """h_t = a_t h_{t-1} + b_t along dim -2, self = a [..., T, D], from the
+        state h0 [..., D] (default zeros), the pairs kept throughout
+        (ds_linear_recurrence_packed)."""
+        if not isinstance(b, DSTensor) or not isinstance(h0, (DSTensor, type(None))):
+            raise TypeError("linear_recurrence takes DSTensors")
+        return DSTensor(ops.ds_linear_recurrence_packed(self.packed, b.packed,
+                                                        None if h0 is None else h0.packed))
 
 
 def _as_operand(x, device):

@@ -177,3 +177,17 @@ def test_host_loops_agree_with_each_other():
             d = (f[0] - f[1]) * 2.0 ** 7
             # the loss's values are below 1000 here: 2^-53 of them over 2^-7
             assert abs(d - float(grads[which][at])) <= 1000 * 2.0 ** -44
+
+
+def test_adapters_have_a_handler_for_every_new_target():
+    """ds_b200_ffi.cc, read as text: one XLA-FFI handler per target."""
+    import os
+    import re
+    from conftest import ROOT
+    from ds_b200 import ffi
+    text = open(os.path.join(ROOT, "ds-experiment_b200", "adapters", "ds_b200_ffi.cc")).read()
+    symbols = set(re.findall(r"XLA_FFI_DEFINE_HANDLER_SYMBOL\((\w+),", text))
+    for name in re.findall(r"^DS_RECURRENCE_HANDLERS\((\w+),", text, re.M):
+        symbols |= {f"DsLinearRecurrence{name}", f"DsLinearRecurrenceVjp{name}"}
+    for target in ffi.SEQUENCE_TARGETS:
+        assert "".join(p[:1].upper() + p[1:] for p in target.split("_")) in symbols, target

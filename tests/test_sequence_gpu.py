@@ -136,7 +136,7 @@ def test_non_finite_stays_in_its_sequence(shape):
     assert np.array_equal(np.isfinite(got), fine)
     assert fine.any() and not fine.all()
     bound = ref.recurrence_bound(mag, "f64", np.where(fine, want, 0).astype(np.float64))
-    assert np.all(np.abs(got - want)[fine] <= bound[fine])
+    assert np.all(np.abs(got[fine] - want[fine]) <= bound[fine])
 
 
 def test_products_that_overflow_meet_a_zero_state():
@@ -256,6 +256,51 @@ def test_other_device():
     want = host(forward("f64")(cu(a), cu(b), cu(h0)))
     got = forward("f64")(*(torch.from_numpy(x).to("cuda:1") for x in (a, b, h0)))
     assert np.array_equal(got.cpu().numpy(), want)
+
+
+def test_ds_tensors_keep_their_pairs():
+    """DSTensor's recurrence and grouped product are the packed and f64 targets on
+    its pairs; a pending expression enters as its pairs."""
+    from ds_b200 import ops
+    from ds_b200.dstensor import DSTensor
+    (a, _), (b, _), _, (h0, _) = inputs((2, 40, 6), 13, "f64")
+    A, B, H = (DSTensor.from_f64(cu(x)) for x in (a, b, h0))
+    h = A.linear_recurrence(B * 2.0, H)
+    want = ops.ds_linear_recurrence_packed(A.packed, (B * 2.0).packed, H.packed)
+    assert torch.equal(h.packed, want) and h.shape == (2, 40, 6)
+    assert torch.equal(A.linear_recurrence(B).packed,
+                       ops.ds_linear_recurrence_packed(A.packed, B.packed))
+    w = np.random.default_rng(0).standard_normal((3, 6, 5))
+    s = torch.tensor([10, 0, 30], dtype=torch.int32, device="cuda")
+    W, X = DSTensor.from_f64(cu(w)), DSTensor.from_f64(cu(a[0]))
+    got = X.ragged_matmul(W, s)
+    want = ops.ds_from_f64(ops.ds_ragged_dot_f64(X.to_f64(), W.to_f64(), s))
+    assert torch.equal(got.packed, want)
+    with pytest.raises(TypeError, match="DSTensor"):
+        A.linear_recurrence(cu(b))
+    with pytest.raises(TypeError, match="DSTensor"):
+        X.ragged_matmul(cu(w), s)
+
+
+def test_calls_through_the_registry():
+    """ffi_call by target name gives what ops gives, with and without h0."""
+    from ds_b200 import ffi, ops
+    (a, _), (b, _), (g, _), (h0, _) = inputs((2, 70, 6), 14, "f64")
+    ta, tb, tg, th = cu(a), cu(b), cu(g), cu(h0)
+    spec = ffi.ShapeDtypeStruct(ta.shape, torch.float64)
+    state = ffi.ShapeDtypeStruct(th.shape, torch.float64)
+    h = ops.ds_linear_recurrence_f64(ta, tb, th)
+    for _ in range(2):
+        assert torch.equal(ffi.ffi_call("ds_linear_recurrence_f64", spec)(ta, tb, th), h)
+    assert torch.equal(ffi.ffi_call("ds_linear_recurrence_f64", spec)(ta, tb, None),
+                       ops.ds_linear_recurrence_f64(ta, tb))
+    got = ffi.ffi_call("ds_linear_recurrence_vjp_f64", (spec, spec, state))(ta, h, tg, th)
+    want = ops.ds_linear_recurrence_vjp_f64(ta, h, tg, th)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    with pytest.raises(ValueError, match="output shape"):
+        ffi.ffi_call("ds_linear_recurrence_f64", state)(ta, tb, th)
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        ffi.ffi_call("ds_linear_recurrence_f64", spec)(ta, None, th)
 
 
 def test_refusals_on_device():
