@@ -10,13 +10,14 @@ platform="CUDA")`` binds a target name to a libds_b200 entry point, and
 raises on a non-OK status.  Every reference target name is registered at
 import.  Scratch for ds_reduce / ds_dot_general comes from torch's caching
 allocator (the role XLA's scratch allocator plays for an FFI handler); small
-scratch is kept per stream and reused, and a reduce's scratch size is asked
-once per shape.
+scratch is kept per stream and host thread and reused, and a reduce's scratch
+size is asked once per shape.
 """
 from __future__ import annotations
 
 import array
 import ctypes
+import threading
 from dataclasses import dataclass
 from typing import Dict, Tuple
 
@@ -169,9 +170,11 @@ def _buf(t):
 
 
 # Workspaces up to _CACHED_WORKSPACE_MAX (reduce partials, the residue
-# planes of products up to about 1100 x 1100) are kept per (device, stream)
-# and reused: calls on one stream run in order, so one buffer serves them
-# all, and a call skips an allocation.  The buffer starts at 1 MiB and grows
+# planes of products up to about 1100 x 1100) are kept per (device, stream,
+# host thread) and reused: one thread's calls on one stream run in order, so one
+# buffer serves them all, and a call skips an allocation.  (Two threads that
+# launch on one stream take turns launch by launch, and a call has several.)
+# The buffer starts at 1 MiB and grows
 # to the next power of two a request needs; the one it replaces was
 # allocated on the same stream, so torch's allocator hands its memory out
 # again only to work ordered after the calls that used it.  Larger ones come
@@ -186,7 +189,7 @@ def _workspace(nbytes: int, device, stream: int = 0) -> torch.Tensor:
     nbytes = max(int(nbytes), 1)
     if nbytes > _CACHED_WORKSPACE_MAX or torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, stream)
+    key = (device.index, stream, threading.get_ident())
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         if ws is None and len(_workspaces) > 64:

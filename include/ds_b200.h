@@ -485,10 +485,12 @@ DS_API int ds_linear_recurrence_vjp_packed(const ds_buffer* a, const ds_buffer* 
    no rows does not read its matrix.
    Operands are f64, or DS pairs as hi / lo tensors of one shape; the result
    is rounded once from f64 accumulations (CUDA-core and small groups) or
-   from the exact integer products of ds_dot_general's tensor-core path.  Row
-   i depends on the group sizes only through the group it lies in and that
-   group's size.  `out` must not overlap operands.  Workspace: the query's
-   bytes, 256-byte aligned. */
+   from the exact integer products of ds_dot_general's tensor-core path, whose
+   uncertified outputs are summed again in double-length arithmetic.  Row i
+   depends on the group sizes only through the group it lies in and that
+   group's size (a call with more than 2^20 uncertified outputs sums every
+   output of its large groups again).  `out` must not overlap operands.
+   Workspace: the query's bytes, 256-byte aligned. */
 DS_API size_t ds_ragged_dot_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
                                            int32_t rhs_contracting);
 DS_API int ds_ragged_dot(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,

@@ -191,3 +191,17 @@ def test_adapters_have_a_handler_for_every_new_target():
         symbols |= {f"DsLinearRecurrence{name}", f"DsLinearRecurrenceVjp{name}"}
     for target in ffi.SEQUENCE_TARGETS:
         assert "".join(p[:1].upper() + p[1:] for p in target.split("_")) in symbols, target
+
+
+def test_threads_have_workspaces_of_their_own(monkeypatch):
+    import threading
+    import torch
+    from ds_b200 import ffi
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(ffi, "_workspaces", {})
+    got = []
+    here = ffi._workspace(100, torch.device("cpu"), 7)
+    t = threading.Thread(target=lambda: got.append(ffi._workspace(100, torch.device("cpu"), 7)))
+    t.start()
+    t.join()
+    assert got[0] is not here and ffi._workspace(100, torch.device("cpu"), 7) is here

@@ -258,6 +258,28 @@ def test_other_device():
     assert np.array_equal(got.cpu().numpy(), want)
 
 
+def test_threads_on_one_stream():
+    """Two host threads launch on one stream in any order: their calls do not
+    meet in a workspace."""
+    from concurrent.futures import ThreadPoolExecutor
+    from ds_b200 import ops
+    values = [inputs((1, 5000, 12), 20 + i, "f64") for i in range(2)]
+    seqs = [(cu(v[0][0]), cu(v[1][0])) for v in values]
+    rng = np.random.default_rng(5)
+    rows = [cu(rng.standard_normal((9, 1024))) for _ in range(2)]
+    W = cu(rng.standard_normal((4, 1024, 96)))
+    s = torch.tensor([2, 0, 3, 1], dtype=torch.int32, device="cuda")
+
+    def run(i):
+        return (ops.ds_linear_recurrence_f64(*seqs[i]), ops.ds_ragged_dot_f64(rows[i], W, s))
+    want = [run(i) for i in range(2)]
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(2) as pool:
+        for i, got in enumerate(pool.map(lambda i: [run(i) for _ in range(100)], range(2))):
+            for g in got:
+                assert all(torch.equal(x, y) for x, y in zip(g, want[i]))
+
+
 def test_ds_tensors_keep_their_pairs():
     """DSTensor's recurrence and grouped product are the packed and f64 targets on
     its pairs; a pending expression enters as its pairs."""
