@@ -15,7 +15,6 @@
 // its own scale, and every group the bits its own length allows.
 //
 // A contraction longer than 32768 runs in chunks whose results are added.
-#include <cstring>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -296,16 +295,57 @@ ragged_contract_gemm_kernel(const __grid_constant__ CUtensorMap ta,
 
 // ---- reconstruction ----------------------------------------------------------------
 
-struct RaggedCrt {
+// The modular sum of an output's 14 residues. A residue byte r becomes the f64
+// 4096 + r by one byte permutation (byte 1 of the high word of 2^12), and the
+// weights W_l, each less the modulus product M where that keeps the running sums
+// of the weights within M / 2, sum to 1: the 4096s leave 4096 times 1, which
+// the sums start below zero. In limbs of 70 bits (hi rounded to nearest) the high
+// sum stays below 2^51.5 in magnitude and is exact; the low one's partial sums
+// stay below 2^86, so its 15 roundings lose at most 2^37 together.
+struct CrtSum {
   double w[kL][2];
+  double start[2];
   double mlimb[2];
-  double inv_m;
+  double inv_m;  // 2^70 / M
+};
+
+CrtSum crt_sum() {
+  CrtSum c{};
+  using i128 = __int128;
+  i128 M = 1, sum = 0, sum_hi = 0;
+  for (int l = 0; l < kL; ++l) M *= mod_of(l);
+  const i128 unit = static_cast<i128>(1) << kCrtSplit;
+  for (int l = 0; l < kL; ++l) {
+    const i128 Ml = M / mod_of(l);
+    int inv = 1;
+    while (static_cast<int>(Ml % mod_of(l)) * inv % mod_of(l) != 1) ++inv;
+    i128 w = Ml * inv;
+    if (sum + w > M / 2) w -= M;
+    sum += w;
+    // floor(w / 2^70 + 1/2)
+    const i128 hi = (w + unit / 2) >> kCrtSplit;
+    sum_hi += hi;
+    c.w[l][0] = static_cast<double>(static_cast<int64_t>(hi));
+    c.w[l][1] = static_cast<double>(w - hi * unit);
+  }
+  c.start[0] = -4096.0 * static_cast<double>(static_cast<int64_t>(sum_hi));
+  c.start[1] = -4096.0 * static_cast<double>(sum - sum_hi * unit);
+  c.mlimb[0] = crt_consts().mlimb[0];
+  c.mlimb[1] = crt_consts().mlimb[1];
+  c.inv_m = crt_consts().inv_m * 0x1p70;
+  return c;
+}
+
+struct RaggedCrt {
+  CrtSum sum;
   RaggedPlan p;
   DotOperand a, b;
   DotResult c;
   int64_t M, K, N;       // rows; products: contraction; contraction: rows of a matrix
   int64_t Mp, Np, slots;
   int P;                 // products
+  uint32_t blocks_n;     // of columns, and (contraction) of a slot's rows, of
+  uint32_t blocks_m;     // ragged_crt_kernel
   const uint8_t* cres;
   const int* sa;
   const int* sb;
@@ -325,12 +365,11 @@ struct RowView {
   int64_t residues;      // row of the residue planes
   int64_t out;           // row of the result
   int64_t a, b, K;       // first elements and length of the contraction
-  double part;           // of the certificate: without the column's
 };
 
 // The certificate's K / 4 and the low limb's rounding.
-__device__ __forceinline__ double certify_rest(int64_t K) {
-  return (0.25 * static_cast<double>(K) + 0x1p35) * pow2_normal(kCertifyBits);
+__device__ __forceinline__ float certify_rest(int64_t K) {
+  return __double2float_ru((0.25 * static_cast<double>(K) + 0x1p37) * pow2_normal(kCertifyBits));
 }
 
 template <bool kContract>
@@ -365,92 +404,212 @@ __device__ __forceinline__ RowView view(const RaggedCrt& p, int64_t row) {
     v.P = p.P;
     v.sa = p.sa[row];
   }
-  v.part = certify_rest(v.K) + static_cast<double>(p.pa[v.residues]);
   return v;
 }
 
-// As crt_kernel in dot_ozaki.cu: kCols consecutive columns per thread over
-// rows blockIdx.y, + gridDim.y, ...
+// C from an output's residues: the modular sum, less the multiple of M that
+// brings it within M / 4 (so near that the high sum alone tells which).
+__device__ __forceinline__ double crt_value(const CrtSum& k, double s_hi, double s_lo) {
+  const double qt = rint(s_hi * k.inv_m);
+  const double t_hi = __fma_rn(-qt, k.mlimb[0], s_hi);
+  const double t_lo = __fma_rn(-qt, k.mlimb[1], s_lo);
+  return __fma_rn(t_hi, 0x1p70, t_lo);
+}
+
+// bytes of the high word: 0, byte q of `word`, 0xb0, 0x40
+__device__ __forceinline__ double biased_byte(uint32_t word, int q) {
+  return __hiloint2double(static_cast<int>(__byte_perm(word, 0x40b00000u, 0x7604u | (q << 4))), 0);
+}
+
+__device__ __forceinline__ bool scales_ordinary(int sa, int sb) {
+  return shift_ordinary(sa) && shift_ordinary(sb);
+}
+__device__ __forceinline__ bool in_range(int s) { return s <= 1022 && s >= -1023; }
+
+// Outputs of one row at four columns that ragged_crt_kernel leaves out of its
+// loop: scales whose sum leaves the f64 range, and (the IEEE sum of the products)
+// non-finite operands.
+struct SpecialRow {
+  const uint8_t* residues;
+  int64_t a, b, K;  // first elements of the row and of the column, and length
+  int64_t out;
+  int columns, sa;
+};
+
+__device__ __noinline__ void special_outputs(const RaggedCrt& p, const SpecialRow& r,
+                                             const int* sb_of, size_t plane) {
+  for (int q = 0; q < r.columns; ++q) {
+    const int sa = r.sa, sb = sb_of[q];
+    double out = 0.0;
+    if (scales_ordinary(sa, sb)) {
+      if (in_range(sa + sb)) continue;
+      double s_hi = p.sum.start[0], s_lo = p.sum.start[1];
+      for (int l = 0; l < kL; ++l) {
+        const double x = biased_byte(r.residues[l * plane + q], 0);
+        s_hi = __fma_rn(x, p.sum.w[l][0], s_hi);
+        s_lo = __fma_rn(x, p.sum.w[l][1], s_lo);
+      }
+      out = scale2(scale2(crt_value(p.sum, s_hi, s_lo), -sa), -sb);
+    } else {
+      if (sa != kShiftNonFinite && sb != kShiftNonFinite) continue;
+      for (int64_t k = 0; k < r.K; ++k)
+        out += op_value(p.a, r.a + k * p.a.s_k) *
+               op_value(p.b, r.b + q * p.b.s_r + k * p.b.s_k);
+    }
+    put_result(p.c, r.out + q, out);
+  }
+}
+
+// A block takes kCrtRows rows of one group x 512 columns, each thread kCols
+// consecutive columns, whose scales and certificate parts it keeps.  14 bytes in
+// and 8 out per output: bound by HBM once enough rows are on their way, which
+// the loop's own loads (64 to 126 registers, 20 to 32 warps) did not reach.  Each
+// warp copies its rows to shared memory three ahead: 16.8 million outputs of
+// 2048 x 2048 matrices take 63 us (5.9 TB/s), with loads in the loop and a
+// residue's bias subtracted 117; 33.5 million of a contraction 113 and 226.
+// 8 or 32 rows, or 4 or 6 blocks per SM, are within 1%, and so is five rows ahead.
 constexpr int kRaggedCrtThreads = 128, kCols = 4;
+constexpr int kCrtRows = 16, kCrtAhead = 3, kWarpCols = 32 * kCols;
+static_assert(kCrtRows <= 32, "a lane per row");
 
 template <bool kContract>
-__global__ void __launch_bounds__(kRaggedCrtThreads, 8)
+__global__ void __launch_bounds__(kRaggedCrtThreads, 5)
 ragged_crt_kernel(const __grid_constant__ RaggedCrt p) {
   wait_previous_grid();
+  const uint32_t bm = blockIdx.x / p.blocks_n, bn = blockIdx.x - bm * p.blocks_n;
+  int64_t row0;
+  int rows;
+  if constexpr (kContract) {
+    const uint32_t slot = bm / p.blocks_m;
+    if (slot >= static_cast<uint32_t>(slots_of(p.p))) return;
+    const int64_t i = static_cast<int64_t>(bm - slot * p.blocks_m) * kCrtRows;
+    row0 = slot * p.K + i;
+    rows = p.K - i < kCrtRows ? static_cast<int>(p.K - i) : kCrtRows;
+  } else {
+    constexpr uint32_t kParts = kTensorTile / kCrtRows;
+    if (bm / kParts >= static_cast<uint32_t>(p.p.tensor_start[p.p.groups])) return;
+    const RaggedTile x = p.p.tensor[bm / kParts];
+    const int i = static_cast<int>(bm % kParts) * kCrtRows, left = x.rows - i;
+    row0 = x.row + i;
+    rows = left < kCrtRows ? left : kCrtRows;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t w0 = (static_cast<int64_t>(bn) * (kRaggedCrtThreads / 32) + warp) * kWarpCols;
+  const int64_t j0 = w0 + lane * kCols;
+  if (rows <= 0 || w0 >= p.N) return;  // the whole warp
+  const RowView v = view<kContract>(p, row0);
   const size_t plane = static_cast<size_t>(kContract ? p.slots : 1) * p.Mp * p.Np;
+  // the warp's columns of the 14 planes of a row, kCrtAhead rows ahead
+  __shared__ __align__(16) uint8_t s_rows[kRaggedCrtThreads / 32][kCrtAhead + 1][kL * kWarpCols];
+  const uint8_t* from = p.cres + v.residues * p.Np + w0 + lane / 8 * plane + lane % 8 * 16;
+  auto copy_row = [&](int r) {
+    if (r < rows) {
+      const uint32_t to = smem_u32(&s_rows[warp][r % (kCrtAhead + 1)][lane * 16]);
+#pragma unroll
+      for (int i = 0; i < (kL + 3) / 4; ++i)
+        if (4 * i + lane / 8 < kL)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * 512),
+                       "l"(from + 4 * i * plane)
+                       : "memory");
+      from += p.Np;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int r = 0; r < kCrtAhead; ++r) copy_row(r);
+  // row r's scale and certificate part in lane r
+  const int sa_of = lane < rows ? p.sa[v.residues + lane] : 0;
+  const float pa_of = lane < rows ? p.pa[v.residues + lane] : 0.0f;
   const bool failed = *p.err != 0;
-  const int64_t j0 = (static_cast<int64_t>(blockIdx.x) * kRaggedCrtThreads + threadIdx.x) * kCols;
-  if (j0 >= p.N) return;
-  const int64_t rows = rows_of<kContract>(p);
-  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-    const RowView v = view<kContract>(p, row);
-    if (!v.live) continue;
-    const uint8_t* src = p.cres + v.residues * p.Np + j0;
+  const int4 sbv = *reinterpret_cast<const int4*>(p.sb + v.slot * p.Np + j0);
+  const int sb[kCols] = {sbv.x, sbv.y, sbv.z, sbv.w};
+  const float4 pbv = *reinterpret_cast<const float4*>(p.pb + v.slot * p.Np + j0);
+  const float pb[kCols] = {pbv.x, pbv.y, pbv.z, pbv.w};
+  int sb_min = sb[0], sb_max = sb[0];
+  bool plain = !failed && j0 + kCols <= p.N;
+#pragma unroll
+  for (int q = 0; q < kCols; ++q) {
+    plain &= shift_ordinary(sb[q]);
+    sb_min = sb[q] < sb_min ? sb[q] : sb_min;
+    sb_max = sb[q] > sb_max ? sb[q] : sb_max;
+  }
+  const float rest = certify_rest(v.K);
+  const bool words =
+      p.c.f64 && (p.N & 1) == 0 && (reinterpret_cast<uintptr_t>(p.c.f64) & 15) == 0;
+  int64_t at = v.out * p.N + j0;
+  uint32_t special = 0;  // rows with outputs for special_outputs
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r, at += p.N) {
+    const int sa = __shfl_sync(0xffffffffu, sa_of, r);
+    const float part = __fadd_ru(rest, __shfl_sync(0xffffffffu, pa_of, r));
+    asm volatile("cp.async.wait_group %0;" ::"n"(kCrtAhead - 1) : "memory");
+    __syncwarp();
+    copy_row(r + kCrtAhead);
+    const uint32_t* row = reinterpret_cast<const uint32_t*>(s_rows[warp][r % (kCrtAhead + 1)]);
     uint32_t cur[kL];
 #pragma unroll
-    for (int l = 0; l < kL; ++l)
-      cur[l] = __ldcs(reinterpret_cast<const unsigned int*>(src + l * plane));
+    for (int l = 0; l < kL; ++l) cur[l] = row[l * (kWarpCols / 4) + lane];
     double s_hi[kCols], s_lo[kCols];
 #pragma unroll
-    for (int q = 0; q < kCols; ++q) s_hi[q] = s_lo[q] = 0.0;
+    for (int q = 0; q < kCols; ++q) {
+      s_hi[q] = p.sum.start[0];
+      s_lo[q] = p.sum.start[1];
+    }
 #pragma unroll
     for (int l = 0; l < kL; ++l) {
-      const double w_hi = p.w[l][0], w_lo = p.w[l][1];
+      const double w_hi = p.sum.w[l][0], w_lo = p.sum.w[l][1];
 #pragma unroll
       for (int q = 0; q < kCols; ++q) {
-        const double r = byte_to_f64(cur[l], q);
-        s_hi[q] = __fma_rn(r, w_hi, s_hi[q]);  // exact
-        s_lo[q] = __fma_rn(r, w_lo, s_lo[q]);
+        const double x = biased_byte(cur[l], q);
+        s_hi[q] = __fma_rn(x, w_hi, s_hi[q]);  // exact
+        s_lo[q] = __fma_rn(x, w_lo, s_lo[q]);
       }
     }
-    const int4 sbv = *reinterpret_cast<const int4*>(p.sb + v.slot * p.Np + j0);
-    const int sb[kCols] = {sbv.x, sbv.y, sbv.z, sbv.w};
-    const float4 pbv = *reinterpret_cast<const float4*>(p.pb + v.slot * p.Np + j0);
-    const float pb[kCols] = {pbv.x, pbv.y, pbv.z, pbv.w};
-    double out[kCols];
-    bool put[kCols], all = j0 + kCols <= p.N;
+    double c[kCols];
+    bool sure[kCols];
 #pragma unroll
     for (int q = 0; q < kCols; ++q) {
-      put[q] = j0 + q < p.N;
-      if (failed) {
-        out[q] = __longlong_as_double(0x7ff8000000000000LL);
-      } else if (shift_ordinary(v.sa) && shift_ordinary(sb[q])) {
-        const double approx = __fma_rn(s_hi[q], 0x1p70, s_lo[q]);
-        const double qt = rint(approx * p.inv_m);
-        const double t_hi = __fma_rn(-qt, p.mlimb[0], s_hi[q]);
-        const double t_lo = __fma_rn(-qt, p.mlimb[1], s_lo[q]);
-        const double c = __fma_rn(t_hi, 0x1p70, t_lo);
-        if (put[q] && !(fabs(c) >= v.part + static_cast<double>(pb[q]))) {
-          // uncertified: listed for ragged_fix_kernel, which writes this output
-          put[q] = false;
-          const int at = atomicAdd(p.fix_count, 1);
-          if (at < p.fix_cap) p.fix_list[at] = static_cast<uint64_t>(row * p.N + j0 + q);
-        }
-        const int e = -(v.sa + sb[q]);
-        out[q] = (e >= -1022 && e <= 1023) ? c * pow2_normal(e) : scale2(scale2(c, -v.sa), -sb[q]);
-      } else if (v.sa == kShiftNonFinite || sb[q] == kShiftNonFinite) {
-        // a non-finite operand: the IEEE sum of the products
-        double s = 0.0;
-        if (put[q])
-          for (int64_t k = 0; k < v.K; ++k)
-            s += op_value(p.a, v.a + k * p.a.s_k) *
-                 op_value(p.b, v.b + (j0 + q) * p.b.s_r + k * p.b.s_k);
-        out[q] = s;
-      } else {
-        out[q] = 0.0;  // a row or column of zeros
-      }
-      all &= put[q];
+      c[q] = crt_value(p.sum, s_hi[q], s_lo[q]);
+      // the high word of the bound as an f64, rounded down, against c's
+      const int bound = (__float_as_int(__fadd_ru(part, pb[q])) >> 3) + (896 << 20);
+      sure[q] = (__double2hiint(c[q]) & 0x7fffffff) > bound;
+      const uint32_t e = 1023u - static_cast<uint32_t>(sa) - static_cast<uint32_t>(sb[q]);
+      c[q] = __dmul_rn(c[q], __hiloint2double(static_cast<int>(e << 20), 0));
     }
-    const int64_t at = v.out * p.N + j0;
-    double* dst = p.c.f64 ? p.c.f64 + at : nullptr;
-    if (all && dst && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-      reinterpret_cast<double2*>(dst)[0] = make_double2(out[0], out[1]);
-      reinterpret_cast<double2*>(dst)[1] = make_double2(out[2], out[3]);
-    } else {
+    if (words && plain && shift_ordinary(sa) && in_range(sa + sb_max) && in_range(sa + sb_min) &&
+        sure[0] && sure[1] && sure[2] && sure[3]) {
+      double2* dst = reinterpret_cast<double2*>(p.c.f64 + at);
+      dst[0] = make_double2(c[0], c[1]);
+      dst[1] = make_double2(c[2], c[3]);
+      continue;
+    }
 #pragma unroll
-      for (int q = 0; q < kCols; ++q)
-        if (put[q]) put_result(p.c, at + q, out[q]);
+    for (int q = 0; q < kCols; ++q) {
+      if (j0 + q >= p.N) continue;
+      if (failed) {
+        c[q] = __longlong_as_double(0x7ff8000000000000LL);
+      } else if (!scales_ordinary(sa, sb[q])) {
+        c[q] = 0.0;  // a row or column of zeros
+        if (sa == kShiftNonFinite || sb[q] == kShiftNonFinite) special |= 1u << r;
+      } else if (!sure[q]) {
+        // uncertified: listed for ragged_fix_kernel, which writes this output
+        const int n = atomicAdd(p.fix_count, 1);
+        if (n < p.fix_cap) p.fix_list[n] = static_cast<uint64_t>((row0 + r) * p.N + j0 + q);
+        continue;
+      } else if (!in_range(sa + sb[q])) {
+        special |= 1u << r;
+      }
+      put_result(p.c, at + q, c[q]);
     }
+  }
+  while (special != 0) {
+    const int r = __ffs(special) - 1;
+    special &= special - 1;
+    const int left = p.N - j0 < kCols ? static_cast<int>(p.N - j0) : kCols;
+    const SpecialRow x{p.cres + (v.residues + r) * p.Np + j0,
+                       v.a + r * (kContract ? 1 : p.a.s_r), v.b + j0 * p.b.s_r, v.K,
+                       (v.out + r) * p.N + j0, left, p.sa[v.residues + r]};
+    special_outputs(p, x, p.sb + v.slot * p.Np + j0, plane);
   }
 }
 
@@ -732,11 +891,10 @@ template <bool kContract>
 int launch_rebuild(const RaggedCrt& c, int64_t rows, const DotResult* add_to, cudaStream_t s) {
   {
     ProfileScope prof("ozaki_crt", s);
-    const int64_t gx = (c.N + kRaggedCrtThreads * kCols - 1) / (kRaggedCrtThreads * kCols);
-    int64_t gy = (static_cast<int64_t>(sm_count()) * 16 + gx - 1) / gx;
-    if (gy > rows) gy = rows;
+    const int64_t parts =
+        kContract ? c.slots * c.blocks_m : c.p.tensor_cap * (kTensorTile / kCrtRows);
     DSB_CUDA_TRY(launch_dependent(ragged_crt_kernel<kContract>,
-                                  dim3(static_cast<unsigned>(gx), grid_y(gy)),
+                                  dim3(static_cast<unsigned>(parts * c.blocks_n)),
                                   dim3(kRaggedCrtThreads), s, c));
   }
   ProfileScope prof("ozaki_fix", s);
@@ -786,10 +944,11 @@ TensorRun tensor_run(const RaggedProblem& q, const RaggedPlan& p, const TensorLa
   r.pb = reinterpret_cast<float*>(r.ws + g.pb);
   r.err = ints(g.err);
   r.row_slot = ints(g.row_slot);
-  const CrtConsts& cc = crt_consts();
-  std::memcpy(r.crt.w, cc.w, sizeof(r.crt.w));
-  std::memcpy(r.crt.mlimb, cc.mlimb, sizeof(r.crt.mlimb));
-  r.crt.inv_m = cc.inv_m;
+  static const CrtSum sum = crt_sum();
+  r.crt.sum = sum;
+  constexpr int64_t kBlockN = kRaggedCrtThreads * kCols;
+  r.crt.blocks_n = static_cast<uint32_t>((q.N + kBlockN - 1) / kBlockN);
+  r.crt.blocks_m = static_cast<uint32_t>((q.K + kCrtRows - 1) / kCrtRows);
   r.crt.p = p;
   r.crt.a = q.lhs;
   r.crt.b = q.rhs;
@@ -829,6 +988,10 @@ bool ragged_tensor_fits(int64_t M, int64_t K, int64_t N, int64_t G, bool contrac
   const TensorLayout g = tensor_layout(M, K, N, G, contract);
   const int64_t most = (1LL << 31) - 1;  // TMA coordinates and tile numbers are int32
   if (g.total > kRaggedTensorBytes) return false;
+  // blocks of ragged_crt_kernel
+  const int64_t rows = contract ? g.slots * pad(K, kCrtRows)
+                                : ragged_tensor_tiles(M, G, false) * kTensorTile;
+  if (rows / kCrtRows * (N / (kRaggedCrtThreads * kCols) + 1) > most) return false;
   if (contract) return g.slots * g.Mp <= most && g.Np <= most;
   return kL * g.Mp <= most && kL * g.slots * g.Np <= most && g.slots <= 65535;
 }
