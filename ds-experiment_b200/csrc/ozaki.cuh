@@ -330,25 +330,19 @@ __host__ __device__ constexpr int split_rows_threads(int64_t K) {
   return K > 4096 && K <= 16 * kSplitRowsMaxThreads ? kSplitRowsMaxThreads : 256;
 }
 
-//
-// kNorm: norm[b rows_pad + r] also takes the row's part of the certificate
-// (certify_part).
-template <bool kNorm = false>
 __device__ __forceinline__ void split_rows_body(const DotOperand& o, int64_t rows, int64_t K,
                                                 int64_t rows_pad, int64_t Kp, int64_t batch,
                                                 int P, uint8_t* __restrict__ planes,
-                                                int* __restrict__ shifts, int64_t r, int64_t b,
-                                                float* norm = nullptr) {
+                                                int* __restrict__ shifts, int64_t r, int64_t b) {
   __shared__ double s_max[kSplitRowsMaxThreads / 32];
   __shared__ int s_bad[kSplitRowsMaxThreads / 32];
-  __shared__ double s_sum[kNorm ? kSplitRowsMaxThreads / 32 : 1];
   const bool live = r < rows;
   const int64_t base = b * o.s_b + r * o.s_r;
   const bool vec = o.f64 && o.s_k == 1 && (reinterpret_cast<uintptr_t>(o.f64 + base) & 15) == 0;
   const int64_t group = 4 * static_cast<int64_t>(blockDim.x);  // k covered by one group
   const bool in_regs = vec && K <= 4 * group;
   double v[16];
-  double mx = 0.0, sum = 0.0;
+  double mx = 0.0;
   bool bad = false;
   if (in_regs) {
 #pragma unroll
@@ -371,26 +365,22 @@ __device__ __forceinline__ void split_rows_body(const DotOperand& o, int64_t row
     for (int j = 0; j < 16; ++j) {
       bad |= !isfinite(v[j]);
       mx = fmax(mx, fabs(v[j]));
-      if constexpr (kNorm) sum += fabs(v[j]);
     }
   } else if (live) {
     for (int64_t k = threadIdx.x; k < K; k += blockDim.x) {
       const double x = op_value(o, base + k * o.s_k);
       bad |= !isfinite(x);
       mx = fmax(mx, fabs(x));
-      if constexpr (kNorm) sum += fabs(x);
     }
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
     mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, d));
     bad |= __shfl_xor_sync(0xffffffffu, static_cast<int>(bad), d) != 0;
-    if constexpr (kNorm) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   }
   if ((threadIdx.x & 31) == 0) {
     s_max[threadIdx.x >> 5] = mx;
     s_bad[threadIdx.x >> 5] = bad;
-    if constexpr (kNorm) s_sum[threadIdx.x >> 5] = sum;
   }
   __syncthreads();
   mx = 0.0;
@@ -400,14 +390,7 @@ __device__ __forceinline__ void split_rows_body(const DotOperand& o, int64_t row
     bad |= s_bad[w] != 0;
   }
   const int shift = live ? shift_for(mx, bad, P) : 0;
-  if (threadIdx.x == 0) {
-    shifts[b * rows_pad + r] = shift;
-    if constexpr (kNorm) {
-      double all = 0.0;
-      for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) all += s_sum[w];
-      norm[b * rows_pad + r] = certify_part(all, shift, K);
-    }
-  }
+  if (threadIdx.x == 0) shifts[b * rows_pad + r] = shift;
   const bool zero = !live || shift == kShiftNonFinite || shift == kShiftZero;
   const int sh = zero ? 0 : shift;
   const size_t plane_stride = static_cast<size_t>(batch) * rows_pad * Kp;

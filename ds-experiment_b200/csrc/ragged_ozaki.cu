@@ -44,9 +44,108 @@ __device__ __forceinline__ int slots_of(const RaggedPlan& p) { return p.slot[p.g
 
 // ---- split ---------------------------------------------------------------------
 
+// Values k .. k + 7 of the row that starts at `base` (contiguous in k), zeros
+// from K on.
+__device__ __forceinline__ void load_8(const DotOperand& o, int64_t base, bool words, int64_t k,
+                                       int64_t K, double (&v)[8]) {
+  if (words && k + 8 <= K) {
+    const double2* p = reinterpret_cast<const double2*>(o.f64 + base + k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double2 d = __ldg(p + j);
+      v[2 * j] = d.x;
+      v[2 * j + 1] = d.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k + j < K ? op_value(o, base + k + j) : 0.0;
+  }
+}
+
+// A row's largest magnitude (as high and, where that is 0, low word: its exponent
+// is all that counts) and 1-norm.
+struct RowStats {
+  int high = 0;
+  uint32_t low = 0;
+  double sum = 0.0;
+  __device__ __forceinline__ void add(const double (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int h = __double2hiint(v[j]) & 0x7fffffff;
+      high = h > high ? h : high;
+      low |= static_cast<uint32_t>(__double2loint(v[j]));
+      sum += fabs(v[j]);
+    }
+  }
+};
+
+// One row into its planes by one block, eight values per thread, modulus and
+// 8-byte store.  The first 2048 values stay in registers, later ones are read
+// twice.
+//
+// Bound by the instructions of 14 residues per value (119 in all): 16.8 million
+// values in rows of 2048 take 88 us (22 bytes per value, 4.2 TB/s).  With four
+// values per thread and store, the maximum taken in f64 and all values read twice
+// it was 109 us.  Blocks of eight rows that load the next one early keep the
+// residues' constants in registers and spill: within 1% of this either way.
+constexpr int kSplitThreads = 256;
+
+__device__ __forceinline__ void split_row(const DotOperand& o, int64_t base, int64_t K, int64_t Kp,
+                                          int P, uint8_t* __restrict__ out, size_t plane_stride,
+                                          int* shift_to, float* part_to) {
+  __shared__ int s_high[kSplitThreads / 32];
+  __shared__ uint32_t s_low[kSplitThreads / 32];
+  __shared__ double s_sum[kSplitThreads / 32];
+  const bool words = o.f64 && (reinterpret_cast<uintptr_t>(o.f64 + base) & 15) == 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int64_t kStep = 8 * kSplitThreads;
+  const int64_t first = 8 * static_cast<int64_t>(threadIdx.x);
+  double v[8];
+  load_8(o, base, words, first, K, v);
+  RowStats stats;
+  stats.add(v);
+  for (int64_t k = first + kStep; k < K; k += kStep) {
+    double w[8];
+    load_8(o, base, words, k, K, w);
+    stats.add(w);
+  }
+  int high = __reduce_max_sync(0xffffffffu, stats.high);
+  uint32_t low = __reduce_or_sync(0xffffffffu, stats.low);
+  double sum = stats.sum;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) {
+    s_high[warp] = high;
+    s_low[warp] = low;
+    s_sum[warp] = sum;
+  }
+  __syncthreads();
+  constexpr int kWarps = kSplitThreads / 32;
+  high = __reduce_max_sync(0xffffffffu, s_high[lane % kWarps]);
+  low = __reduce_or_sync(0xffffffffu, s_low[lane % kWarps]);
+  const int shift = shift_for(__hiloint2double(high, high == 0 ? static_cast<int>(low) : 0),
+                              high >= 0x7ff00000, P);
+  if (threadIdx.x == 0) {
+    sum = 0.0;
+    for (int w = 0; w < kWarps; ++w) sum += s_sum[w];
+    *shift_to = shift;
+    *part_to = certify_part(sum, shift, K);
+  }
+  const bool zero = !shift_ordinary(shift);
+  const int sh = zero ? 0 : shift;
+#pragma unroll 1
+  for (int64_t k = first; k < Kp; k += kStep) {
+    if (k != first) load_8(o, base, words, k, K, v);
+    Limbs x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = limbs_of(quantise(zero ? 0.0 : v[j], sh));
+    store_planes_n<8, true>(x, out + k, plane_stride);
+  }
+}
+
 struct RowSplit {
   DotOperand o;
-  int64_t M, K, Mp, Kp;
+  int64_t K, Mp, Kp;
   int P;
   uint8_t* planes;
   int* shifts;
@@ -57,7 +156,7 @@ struct RowSplit {
 // Rows of the large groups, one block each: blockIdx.y is the row in tile
 // blockIdx.x.  (In one launch with the column maxima of the matrices, their
 // blocks interleaved, it took as long as both.)
-__global__ void __launch_bounds__(kSplitRowsMaxThreads, 2)
+__global__ void __launch_bounds__(kSplitThreads, 4)
 ragged_split_rows_kernel(RowSplit r, RaggedPlan p) {
   wait_previous_grid();
   if (static_cast<int>(blockIdx.x) >= p.tensor_start[p.groups]) return;
@@ -65,20 +164,21 @@ ragged_split_rows_kernel(RowSplit r, RaggedPlan p) {
   if (static_cast<int>(blockIdx.y) >= t.rows) return;
   const int64_t at = t.row + static_cast<int64_t>(blockIdx.y);
   if (threadIdx.x == 0) r.row_slot[at] = t.slot + 1;
-  split_rows_body<true>(r.o, r.M, r.K, r.Mp, r.Kp, 1, r.P, r.planes, r.shifts, at, 0, r.part);
+  split_row(r.o, at * r.o.s_r, r.K, r.Kp, r.P, r.planes + at * r.Kp,
+            static_cast<size_t>(r.Mp) * r.Kp, r.shifts + at, r.part + at);
 }
 
 // Matrices with K contiguous ([G, N, K]): column blockIdx.x of slot blockIdx.y.
-__global__ void __launch_bounds__(kSplitRowsMaxThreads, 2)
-ragged_split_matrix_rows_kernel(DotOperand o, int64_t N, int64_t K, int64_t Np, int64_t Kp,
-                                int64_t slots, int P, RaggedPlan p, uint8_t* __restrict__ planes,
+__global__ void __launch_bounds__(kSplitThreads, 4)
+ragged_split_matrix_rows_kernel(DotOperand o, int64_t K, int64_t Np, int64_t Kp, int64_t slots,
+                                int P, RaggedPlan p, uint8_t* __restrict__ planes,
                                 int* __restrict__ shifts, float* __restrict__ part) {
   wait_previous_grid();
   const int slot = blockIdx.y;
   if (slot >= slots_of(p)) return;
-  DotOperand x = moved(o, p.slot_group[slot] * o.s_b);
-  x.s_b = 0;
-  split_rows_body<true>(x, N, K, Np, Kp, slots, P, planes, shifts, blockIdx.x, slot, part);
+  const int64_t at = slot * Np + blockIdx.x;
+  split_row(o, p.slot_group[slot] * o.s_b + blockIdx.x * o.s_r, K, Kp, P, planes + at * Kp,
+            static_cast<size_t>(slots) * Np * Kp, shifts + at, part + at);
 }
 
 struct ColumnMax {
@@ -1020,18 +1120,18 @@ int ragged_tensor_dot(const RaggedProblem& q, const RaggedPlan& p, void* workspa
     {
       ProfileScope prof("ozaki_split", s);
       DSB_CUDA_TRY(cudaMemsetAsync(r.ws + g.clear, 0, g.clear_end - g.clear, s));
-      const unsigned threads = static_cast<unsigned>(split_rows_threads(K));
-      const RowSplit rows{a, q.M, K, g.Mp, Kp, P, r.planes_a, r.sa, r.row_slot, r.pa};
+      const RowSplit rows{a, K, g.Mp, Kp, P, r.planes_a, r.sa, r.row_slot, r.pa};
       const ColumnMax cols{b, q.N, K, g.Np, r.cb, r.nb};
       const unsigned slots = static_cast<unsigned>(g.slots);
       const unsigned cgx = static_cast<unsigned>(g.Np / kColTileR);
       const unsigned cgy = static_cast<unsigned>((K + kColmaxSlab - 1) / kColmaxSlab);
       DSB_CUDA_TRY(launch_dependent(ragged_split_rows_kernel, dim3(tiles, kTensorTile),
-                                    dim3(threads), s, rows, p));
+                                    dim3(kSplitThreads), s, rows, p));
       if (q.rhs_t) {
         DSB_CUDA_TRY(launch_dependent(ragged_split_matrix_rows_kernel,
-                                      dim3(static_cast<unsigned>(g.Np), slots), dim3(threads), s,
-                                      b, q.N, K, g.Np, Kp, g.slots, P, p, r.planes_b, r.sb, r.pb));
+                                      dim3(static_cast<unsigned>(q.N), slots),
+                                      dim3(kSplitThreads), s, b, K, g.Np, Kp, g.slots, P, p,
+                                      r.planes_b, r.sb, r.pb));
       } else {
         DSB_CUDA_TRY(launch_dependent(ragged_colmax_kernel, dim3(cgx, cgy, slots), dim3(256), s,
                                       cols, p));
