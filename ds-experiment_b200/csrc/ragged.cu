@@ -803,22 +803,24 @@ int splits_of(int64_t M, int64_t K, int64_t N, int64_t G) {
 
 // Whether the tensor-core product takes the large groups: where its estimated
 // time is below the FP64 path's.  In microseconds, from measurements on one B200:
-// the FP64 path does 26 TFLOP/s; the tensor-core product has launches of 60 (80)
-// us, splits a value in 6.4 to 8.3 (7) ps, multiplies at 3 POPS of its 28
-// operations per product but takes at least 0.76 us per 256 x 256 outputs (short
-// contractions), and rebuilds an output in 9 ps.  Measured with / without:
-// 2048 x 1024 x 1024 in 4 groups 140 / 190 us (contraction 191 / 175), 4096 x 1024
-// x 1024 in 8 groups 224 / 337 (286 / 323), 2048 x 2048 x 2048 in 4 groups 300 /
-// 646 (423 / 624), 8192 x 512 x 512 in 8 groups 198 / 179 (171 / 173).
+// the FP64 path takes 12 us and does 26 TFLOP/s; the tensor-core product has
+// launches of 60 (contraction: 80) us, splits a value in 5.5 to 7.2 (6.5) ps,
+// multiplies at 3 POPS of its 28 operations per product but takes at least 0.76 us
+// per 256 x 256 outputs (short contractions), and rebuilds an output in 5.5 ps.
+// Measured with / without: 2048 x 1024 x 1024 in 4 groups 132 / 190 us
+// (contraction 173 / 169), 4096 x 1024 x 1024 in 8 groups 208 / 333 (232 / 318),
+// 2048 x 2048 x 2048 in 4 groups 286 / 646 (368 / 624), 8192 x 512 x 512 in 8 groups
+// 175 / 177 (159 / 183), 1024 x 1024 x 1024 in one 90 / 106 (128 / 97), 4096 x 256 x
+// 2048 in 4 groups 208 / 173 (177 / 183).
 bool tensor_allowed(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
   if (M < tensor_rows(contract) || K < 64 || N < 64) return false;
   const double m = M, k = K, n = N, slots = static_cast<double>(ragged_slots(M, G, contract));
   const double macs = m * k * n, matrices = slots * k * n, outputs = contract ? matrices : m * n;
-  const double plain = 7.7e-8 * macs;
+  const double plain = 12 + 7.7e-8 * macs;
   const double gemm = 9.3e-9 * macs, least = 1.15e-5 * outputs;
-  const double split = contract ? 7e-6 * m * (k + n) : 6.4e-6 * m * k + 8.3e-6 * matrices;
+  const double split = contract ? 6.5e-6 * m * (k + n) : 5.5e-6 * m * k + 7.2e-6 * matrices;
   const double tensor = (contract ? 80 : 60) + split + (gemm > least ? gemm : least) +
-                        9e-6 * outputs;
+                        5.5e-6 * outputs;
   return tensor < plain && ragged_tensor_fits(M, K, N, G, contract);
 }
 

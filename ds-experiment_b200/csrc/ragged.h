@@ -15,9 +15,10 @@ constexpr int kSmallTile = 64;    // rows of a small group's tile
 constexpr int kTensorTile = 256;  // rows of a tile of the tensor-core product
 // Groups of at least this many rows are large: the tensor-core product takes
 // them.  Its fixed costs are a matrix's split (products) or rebuilding (contraction):
-// 32 groups of 128 rows, 2048 x 2048 matrices, take 1.21 ms with it and 1.36
-// without as products, 1.77 and 1.39 as a contraction; 16 of 256 rows 0.79 and
-// 1.28, 1.28 and 1.28.
+// 32 groups of 96 rows, 2048 x 2048 matrices, take 1.18 ms with it and 1.11 without
+// as products, of 128 rows 1.20 and 1.43; as a contraction 32 of 192 rows 1.96 and
+// 1.96, of 256 2.06 and 2.53 (1024 x 1024 matrices: of 192 0.58 and 0.50, of 256 0.64
+// and 0.65).
 constexpr int64_t tensor_rows(bool contract) { return contract ? 256 : 128; }
 // Longest contraction over rows that is taken at once.
 constexpr int64_t kRaggedWindow = 1 << 15;
