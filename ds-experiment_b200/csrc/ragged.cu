@@ -81,7 +81,9 @@ __device__ __forceinline__ int64_t owner_of(const int32_t* start, int64_t G, int
 // A group's rows inside [begin, end) of the call's rows, given its first row and
 // number (a negative one counts as 0; no group passes row M), and its tiles.
 struct GroupShape {
-  int32_t row, end, small, tensor;  // tiles of its kind; 0 of the other
+  int32_t row, end;
+  int32_t full, tail;  // small: tiles of kSmallTile rows, and rows of one more (or 0)
+  int32_t tensor;      // large: tiles
   bool large;
 };
 
@@ -96,17 +98,31 @@ __device__ __forceinline__ GroupShape shape_of(int64_t first, int64_t n, int64_t
   g.row = static_cast<int32_t>(lo);
   g.end = static_cast<int32_t>(hi);
   g.large = rows >= p.tensor_rows;
-  g.small = g.large ? 0 : static_cast<int32_t>((rows + kSmallTile - 1) / kSmallTile);
+  g.full = g.large ? 0 : static_cast<int32_t>(rows / kSmallTile);
+  g.tail = g.large ? 0 : static_cast<int32_t>(rows % kSmallTile);
   g.tensor = g.large ? static_cast<int32_t>((rows + kTensorTile - 1) / kTensorTile) : 0;
   return g;
 }
 
-// Writes group g's places, given the small tiles, large tiles and large groups
-// before it.
+// Small tiles stand in falling order of the work they take (full ones, then
+// tails by the accumulators that small_kernel gives them), so that the last units
+// of a call are its short ones: 0 .. 3, or 4 for no tail.
+constexpr int kTailKinds = 4;
+__device__ __forceinline__ int tail_kind(int tail) {
+  return tail == 0 ? kTailKinds : tail <= 8 ? 3 : tail <= 16 ? 2 : tail <= 32 ? 1 : 0;
+}
+
+__device__ __forceinline__ void put_tail(const RaggedPlan& p, int64_t g, int32_t end, int32_t tail,
+                                         int64_t at) {
+  p.small[at] = RaggedTile{static_cast<int32_t>(g), end - tail, tail, 0};
+}
+
+// Writes group g's places, given the full small tiles, large tiles and large
+// groups before it.
 __device__ __forceinline__ void put_group(const RaggedPlan& p, int64_t g, const GroupShape& x,
-                                          int64_t small, int64_t tensor, int64_t slot) {
+                                          int64_t full, int64_t tensor, int64_t slot) {
   p.row[g] = x.row;
-  p.small_start[g] = static_cast<int32_t>(small);
+  p.small_start[g] = static_cast<int32_t>(full);
   p.tensor_start[g] = static_cast<int32_t>(tensor);
   p.slot[g] = static_cast<int32_t>(slot);
   if (x.large) {
@@ -117,16 +133,16 @@ __device__ __forceinline__ void put_group(const RaggedPlan& p, int64_t g, const 
   }
   if (g == p.groups - 1) {
     p.row[g + 1] = x.end;
-    p.small_start[g + 1] = static_cast<int32_t>(small + x.small);
+    p.small_start[g + 1] = static_cast<int32_t>(full + x.full);
     p.tensor_start[g + 1] = static_cast<int32_t>(tensor + x.tensor);
     p.slot[g + 1] = static_cast<int32_t>(slot + x.large);
   }
 }
 
-// The tile tables and the groups' order, from what put_group wrote.
+// The tables of whole tiles and the groups' order, from what put_group wrote.
 __device__ void put_tables(const RaggedPlan& p, int64_t G, int64_t tid, int64_t threads) {
-  // the groups by falling number of rows
-  if (p.order) {
+  // a contraction's groups by falling number of rows
+  if (!p.small) {
     for (int64_t g = tid; g < G; g += threads) {
       const int32_t n = p.row[g + 1] - p.row[g];
       int32_t rank = static_cast<int32_t>(g);
@@ -160,6 +176,7 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
   wait_previous_grid();
   const int64_t tid = threadIdx.x;
   int64_t rows_before = 0, tiles_before = 0, slots_before = 0;
+  int64_t tails_before = 0;  // 16 bits for each kind
   for (int64_t g0 = 0; g0 < G; g0 += kPrepThreads) {
     const int64_t g = g0 + tid;
     const int64_t n = g < G && sizes[g] > 0 ? sizes[g] : 0;
@@ -167,16 +184,37 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
     const GroupShape x = shape_of(rows_before + block_scan(n, rows), n, M, begin, end, p);
     // both counts stay below 2^31
     const int64_t both =
-        tiles_before + block_scan(static_cast<int64_t>(x.small) << 32 | x.tensor, tiles);
+        tiles_before + block_scan(static_cast<int64_t>(x.full) << 32 | x.tensor, tiles);
     const int64_t slot = slots_before + block_scan(x.large, slots);
     rows_before += rows;
     tiles_before += tiles;
     slots_before += slots;
     if (g < G) put_group(p, g, x, both >> 32, both & 0xffffffff, slot);
+    if (p.small) {
+      int64_t tails;
+      const int kind = tail_kind(x.tail);
+      const int64_t one = kind < kTailKinds ? 1ll << (16 * kind) : 0;
+      const int64_t before = tails_before + block_scan(one, tails);
+      tails_before += tails;
+      // the tail's number among its kind
+      if (one) p.order[g] = static_cast<int32_t>(before >> (16 * kind) & 0xffff);
+    }
   }
   if (G == 0 && tid == 0) p.row[0] = p.small_start[0] = p.tensor_start[0] = p.slot[0] = 0;
   __syncthreads();
   put_tables(p, G, tid, kPrepThreads);
+  if (!p.small) return;
+  int64_t kinds[kTailKinds + 1] = {tiles_before >> 32};
+#pragma unroll
+  for (int k = 0; k < kTailKinds; ++k) kinds[k + 1] = kinds[k] + (tails_before >> (16 * k) & 0xffff);
+  for (int64_t g = tid; g < G; g += kPrepThreads) {
+    const int32_t end = p.row[g + 1], rows = end - p.row[g];
+    const int kind = tail_kind(rows >= p.tensor_rows ? 0 : rows % kSmallTile);
+#pragma unroll
+    for (int k = 0; k < kTailKinds; ++k)
+      if (kind == k) put_tail(p, g, end, rows % kSmallTile, kinds[k] + p.order[g]);
+  }
+  if (tid == 0) p.small_start[G + 1] = static_cast<int32_t>(kinds[kTailKinds]);
 }
 
 // The same for at most 32 groups, by one warp's shuffles (3.6 us instead of 5.3).
@@ -199,9 +237,21 @@ prep_few_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t
       return x - v;
     };
     const GroupShape x = shape_of(before(n), n, M, begin, end, p);
-    const int64_t both = before(static_cast<int64_t>(x.small) << 32 | x.tensor);
-    const int slot = __popc(__ballot_sync(0xffffffffu, x.large) & ((1u << lane) - 1u));
+    const int64_t both = before(static_cast<int64_t>(x.full) << 32 | x.tensor);
+    const uint32_t earlier = (1u << lane) - 1u;
+    const int slot = __popc(__ballot_sync(0xffffffffu, x.large) & earlier);
     if (lane < G) put_group(p, lane, x, both >> 32, both & 0xffffffff, slot);
+    if (p.small) {
+      int at = __shfl_sync(0xffffffffu, static_cast<int>(both >> 32) + x.full, 31);
+      const int kind = tail_kind(x.tail);
+#pragma unroll
+      for (int k = 0; k < kTailKinds; ++k) {
+        const uint32_t same = __ballot_sync(0xffffffffu, kind == k);
+        if (kind == k) put_tail(p, lane, x.end, x.tail, at + __popc(same & earlier));
+        at += __popc(same);
+      }
+      if (lane == 0) p.small_start[G + 1] = at;
+    }
     if (G == 0 && lane == 0) p.row[0] = p.small_start[0] = p.tensor_start[0] = p.slot[0] = 0;
   }
   __syncthreads();
@@ -450,7 +500,7 @@ struct SmallUnit {
 
 __device__ __forceinline__ uint32_t units_of(const SmallArgs& a) {
   if (a.contract) return static_cast<uint32_t>(a.q.G) * a.tiles_k * a.tiles_n;
-  return static_cast<uint32_t>(a.p.small_start[a.q.G]) * a.tiles_n * a.splits;
+  return static_cast<uint32_t>(a.p.small_start[a.q.G + 1]) * a.tiles_n * a.splits;
 }
 
 // False for a unit that belongs to the tensor-core product, or that adds
@@ -468,12 +518,12 @@ __device__ __forceinline__ bool unit_at(const SmallArgs& a, uint32_t u, SmallUni
     x.split = 0;
     if (x.k1 - x.k0 >= a.p.tensor_rows || (a.add && x.k1 == x.k0)) return false;
   } else {
-    const uint32_t n = a.p.small_start[a.q.G], rest = u / n, tn = rest / a.splits;
-    const RaggedTile t = a.p.small[u - rest * n];
+    const uint32_t per = a.tiles_n * a.splits, at = u / per, r = u - at * per, tn = r / a.splits;
+    const RaggedTile t = a.p.small[at];
     x.g = t.group;
     x.row = t.row;
     x.rows = t.rows;
-    x.split = static_cast<int>(rest - tn * a.splits);
+    x.split = static_cast<int>(r - tn * a.splits);
     x.col = static_cast<int64_t>(tn) * kTN;
     x.k0 = x.split * a.split_k;
     x.k1 = x.k0 + a.split_k < a.q.K ? x.k0 + a.split_k : a.q.K;
@@ -655,11 +705,10 @@ small_kernel(const __grid_constant__ SmallArgs a) {
       put(a.q.out, i, 0.0);
   }
   const uint32_t units = units_of(a);
-  // the block's units: every gridDim.x-th; a contraction's fall in size and are
-  // taken there and back, so that every block gets about as much
+  // the block's units: every gridDim.x-th.  They fall in size and are taken there
+  // and back, so that every block gets about as much
   auto unit_number = [&](uint32_t step) {
-    const bool back = a.contract && (step & 1);
-    return step * gridDim.x + (back ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    return step * gridDim.x + (step & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
   };
   auto next_unit = [&](uint32_t step, SmallUnit& x) {
     while (step * gridDim.x < units) {
@@ -764,7 +813,7 @@ small_kernel(const __grid_constant__ SmallArgs a) {
 __global__ void __launch_bounds__(kThreads)
 small_sum_kernel(const __grid_constant__ SmallArgs a) {
   wait_previous_grid();
-  if (static_cast<int>(blockIdx.y) >= a.p.small_start[a.q.G]) return;
+  if (static_cast<int>(blockIdx.y) >= a.p.small_start[a.q.G + 1]) return;
   const RaggedTile t = a.p.small[blockIdx.y];
   const int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (c >= a.q.N) return;
@@ -849,10 +898,10 @@ Layout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
   }
   l.splits = contract ? 1 : splits_of(M, K, N, G);
   l.row = take((G + 1) * 4);
-  l.small_start = take((G + 1) * 4);
+  l.small_start = take((G + 2) * 4);
   l.tensor_start = take((G + 1) * 4);
   l.slot = take((G + 1) * 4);
-  l.order = take(contract ? G * 4 : 0);
+  l.order = take(G * 4);
   l.small = take(l.small_cap * sizeof(RaggedTile));
   l.tensor = take(l.tensor_cap * sizeof(RaggedTile));
   l.slot_group = take(l.slots * 4);
@@ -894,8 +943,8 @@ RaggedPlan plan_at(const Layout& l, int64_t G, bool contract, uint8_t* ws, bool 
   p.small_start = ints(l.small_start);
   p.tensor_start = ints(l.tensor_start);
   p.slot = ints(l.slot);
-  p.order = contract ? ints(l.order) : nullptr;
-  p.small = l.small_cap ? reinterpret_cast<RaggedTile*>(ws + l.small) : nullptr;
+  p.order = ints(l.order);
+  p.small = contract ? nullptr : reinterpret_cast<RaggedTile*>(ws + l.small);
   p.tensor = l.tensor_cap ? reinterpret_cast<RaggedTile*>(ws + l.tensor) : nullptr;
   p.slot_group = ints(l.slot_group);
   p.slot_bits = ints(l.slot_bits);

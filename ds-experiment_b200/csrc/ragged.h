@@ -47,11 +47,13 @@ constexpr int kBitsLimits = 6;
 struct RaggedPlan {
   int64_t groups;
   int32_t* row;           // [G + 1] first row of each group, then the end of the last
-  int32_t* small_start;   // [G + 1] first tile of each small group, then their number
+  int32_t* small_start;   // [G + 2] full tiles of the small groups before each, then their
+                          // number, then that of all small tiles
   int32_t* tensor_start;  // [G + 1] the same of the large ones
   int32_t* slot;          // [G + 1] large groups before each, then their number
-  int32_t* order;         // [G] the groups by falling number of rows (null: not wanted)
-  RaggedTile* small;      // null: not wanted
+  int32_t* order;         // [G] contraction: the groups by falling number of rows; products:
+                          // prep_kernel's own
+  RaggedTile* small;      // [small_cap] products; null: contraction
   RaggedTile* tensor;
   int32_t* slot_group;    // of each large group: its number among all,
   int32_t* slot_bits;     // and the bits its rows allow as a contraction
