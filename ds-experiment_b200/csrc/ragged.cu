@@ -217,13 +217,12 @@ prep_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t beg
   if (tid == 0) p.small_start[G + 1] = static_cast<int32_t>(kinds[kTailKinds]);
 }
 
-// The same for at most 32 groups, by one warp's shuffles (3.6 us instead of 5.3).
+// The same for at most kFewGroups, by one warp's shuffles (3.6 us instead of 5.3).
+constexpr int kFewGroups = 32;
 constexpr int kPrepFewThreads = 128;
 
-__global__ void __launch_bounds__(kPrepFewThreads)
-prep_few_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t begin,
-                int64_t end, RaggedPlan p) {
-  wait_previous_grid();
+__device__ __forceinline__ void prep_few(const int32_t* __restrict__ sizes, int64_t G, int64_t M,
+                                         int64_t begin, int64_t end, const RaggedPlan& p) {
   const int lane = threadIdx.x;
   if (lane < 32) {
     const int64_t n = lane < G && sizes[lane] > 0 ? sizes[lane] : 0;
@@ -255,7 +254,14 @@ prep_few_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t
     if (G == 0 && lane == 0) p.row[0] = p.small_start[0] = p.tensor_start[0] = p.slot[0] = 0;
   }
   __syncthreads();
-  put_tables(p, G, threadIdx.x, kPrepFewThreads);
+  put_tables(p, G, threadIdx.x, blockDim.x);
+}
+
+__global__ void __launch_bounds__(kPrepFewThreads)
+prep_few_kernel(const int32_t* __restrict__ sizes, int64_t G, int64_t M, int64_t begin,
+                int64_t end, RaggedPlan p) {
+  wait_previous_grid();
+  prep_few(sizes, G, M, begin, end, p);
 }
 
 // ---- small groups: FP64 matrix instructions ---------------------------------------
@@ -488,7 +494,33 @@ struct SmallArgs {
   int64_t split_k;
   double* partial;   // [splits][M][N]
   int vec_a, vec_b;  // DS pairs per copy
+  bool own_plan;     // each block makes the plan (of at most kFewGroups) for itself
 };
+
+// A block's own plan: of calls without large groups and with few tiles, which are
+// short enough for the launch before them to count ([16] x [16, 1024, 2048]: 35 us
+// with prep_few_kernel, 32.5 without).
+constexpr int kOwnTiles = 96;
+
+struct OwnPlan {
+  int32_t row[kFewGroups + 1], small_start[kFewGroups + 2], tensor_start[kFewGroups + 1];
+  int32_t slot[kFewGroups + 1], order[kFewGroups];
+  RaggedTile small[kOwnTiles];
+};
+
+__device__ __forceinline__ void make_own_plan(const SmallArgs& a, OwnPlan& own) {
+  RaggedPlan p = a.p;
+  p.row = own.row;
+  p.small_start = own.small_start;
+  p.tensor_start = own.tensor_start;
+  p.slot = own.slot;
+  p.order = own.order;
+  p.small = a.contract ? nullptr : own.small;
+  prep_few(a.q.group_sizes, a.q.G, a.q.M, 0, a.q.M, p);
+  __syncthreads();
+  // small_sum_kernel asks for the last group's end
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.p.row[a.q.G] = own.row[a.q.G];
+}
 
 // A unit of work: an output tile over a range of the contraction.
 struct SmallUnit {
@@ -498,28 +530,31 @@ struct SmallUnit {
   int split;
 };
 
-__device__ __forceinline__ uint32_t units_of(const SmallArgs& a) {
+__device__ __forceinline__ uint32_t units_of(const SmallArgs& a, const OwnPlan& own) {
   if (a.contract) return static_cast<uint32_t>(a.q.G) * a.tiles_k * a.tiles_n;
-  return static_cast<uint32_t>(a.p.small_start[a.q.G + 1]) * a.tiles_n * a.splits;
+  const int tiles = (a.own_plan ? own.small_start : a.p.small_start)[a.q.G + 1];
+  return static_cast<uint32_t>(tiles) * a.tiles_n * a.splits;
 }
 
 // False for a unit that belongs to the tensor-core product, or that adds
 // nothing.
-__device__ __forceinline__ bool unit_at(const SmallArgs& a, uint32_t u, SmallUnit& x) {
+__device__ __forceinline__ bool unit_at(const SmallArgs& a, const OwnPlan& own, uint32_t u,
+                                        SmallUnit& x) {
   if (a.contract) {
     const uint32_t per = a.tiles_k * a.tiles_n, at = u / per, r = u - at * per;
-    const uint32_t tk = r / a.tiles_n, g = a.p.order[at];
+    const uint32_t tk = r / a.tiles_n, g = (a.own_plan ? own.order : a.p.order)[at];
+    const int32_t* rows = (a.own_plan ? own.row : a.p.row) + g;
     x.g = static_cast<int>(g);
     x.row = static_cast<int64_t>(tk) * kSmallTile;
     x.col = static_cast<int64_t>(r - tk * a.tiles_n) * kTN;
-    x.k0 = a.p.row[g];
-    x.k1 = a.p.row[g + 1];
+    x.k0 = rows[0];
+    x.k1 = rows[1];
     x.rows = a.q.K - x.row < kSmallTile ? static_cast<int>(a.q.K - x.row) : kSmallTile;
     x.split = 0;
     if (x.k1 - x.k0 >= a.p.tensor_rows || (a.add && x.k1 == x.k0)) return false;
   } else {
     const uint32_t per = a.tiles_n * a.splits, at = u / per, r = u - at * per, tn = r / a.splits;
-    const RaggedTile t = a.p.small[at];
+    const RaggedTile t = (a.own_plan ? own.small : a.p.small)[at];
     x.g = t.group;
     x.row = t.row;
     x.rows = t.rows;
@@ -695,16 +730,18 @@ __global__ void __launch_bounds__(kThreads, 2)
 small_kernel(const __grid_constant__ SmallArgs a) {
   using St = Stages<kRows>;
   extern __shared__ __align__(16) double stage[];
+  __shared__ OwnPlan own;
   wait_previous_grid();
+  if (a.own_plan) make_own_plan(a, own);
   // rows behind the last group
   if (!a.contract) {
     const int64_t end = a.q.M * a.q.N;
-    for (int64_t i = a.p.row[a.q.G] * a.q.N + static_cast<int64_t>(blockIdx.x) * kThreads +
+    for (int64_t i = (a.own_plan ? own.row : a.p.row)[a.q.G] * a.q.N + static_cast<int64_t>(blockIdx.x) * kThreads +
                      threadIdx.x;
          i < end; i += static_cast<int64_t>(gridDim.x) * kThreads)
       put(a.q.out, i, 0.0);
   }
-  const uint32_t units = units_of(a);
+  const uint32_t units = units_of(a, own);
   // the block's units: every gridDim.x-th.  They fall in size and are taken there
   // and back, so that every block gets about as much
   auto unit_number = [&](uint32_t step) {
@@ -713,7 +750,7 @@ small_kernel(const __grid_constant__ SmallArgs a) {
   auto next_unit = [&](uint32_t step, SmallUnit& x) {
     while (step * gridDim.x < units) {
       const uint32_t u = unit_number(step);
-      if (u < units && unit_at(a, u, x)) return step;
+      if (u < units && unit_at(a, own, u, x)) return step;
       ++step;
     }
     return kNoUnit;
@@ -809,12 +846,21 @@ small_kernel(const __grid_constant__ SmallArgs a) {
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// The splits of every small tile (blockIdx.y) added up in order.
+// The splits of every small tile (blockIdx.y) added up in order; where the blocks
+// made the plan themselves all rows are small groups' and blockIdx.y stands for
+// kSmallTile of them.
 __global__ void __launch_bounds__(kThreads)
 small_sum_kernel(const __grid_constant__ SmallArgs a) {
   wait_previous_grid();
-  if (static_cast<int>(blockIdx.y) >= a.p.small_start[a.q.G + 1]) return;
-  const RaggedTile t = a.p.small[blockIdx.y];
+  RaggedTile t;
+  if (a.own_plan) {
+    t.row = static_cast<int>(blockIdx.y) * kSmallTile;
+    t.rows = a.p.row[a.q.G] - t.row;
+    t.rows = t.rows < kSmallTile ? t.rows : kSmallTile;
+  } else {
+    if (static_cast<int>(blockIdx.y) >= a.p.small_start[a.q.G + 1]) return;
+    t = a.p.small[blockIdx.y];
+  }
   const int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (c >= a.q.N) return;
   const int64_t plane = a.q.M * a.q.N;
@@ -996,10 +1042,11 @@ int launch_small(const SmallArgs& a, int64_t most_units, cudaStream_t s) {
   cfg.numAttrs = 1;
   DSB_CUDA_TRY(cudaLaunchKernelEx(&cfg, small_kernel<kPair, kA, kB, kRows>, a));
   if (a.splits > 1) {
-    const int64_t rows = a.q.M < 8 ? a.q.M : 8;
+    const int64_t most = a.own_plan ? kSmallTile : 8, rows = a.q.M < most ? a.q.M : most;
     DSB_CUDA_TRY(launch_dependent(small_sum_kernel,
                                   dim3(static_cast<unsigned>(ceil_div(a.q.N, kThreads)),
-                                       static_cast<unsigned>(a.p.small_cap),
+                                       static_cast<unsigned>(
+                                           a.own_plan ? ceil_div(a.q.M, kSmallTile) : a.p.small_cap),
                                        static_cast<unsigned>(rows)),
                                   dim3(kThreads), s, a));
   }
@@ -1019,7 +1066,7 @@ int launch_products(const SmallArgs& a, int64_t units, cudaStream_t s) {
 
 int launch_prep(const RaggedProblem& q, int64_t begin, int64_t end, const RaggedPlan& p,
                 cudaStream_t s) {
-  if (q.G <= 32)
+  if (q.G <= kFewGroups)
     DSB_CUDA_TRY(launch_dependent(prep_few_kernel, dim3(1), dim3(kPrepFewThreads), s,
                                   q.group_sizes, q.G, q.M, begin, end, p));
   else
@@ -1050,7 +1097,9 @@ int ragged_dot(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) 
   a.partial = reinterpret_cast<double*>(ws + l.partial);
   a.vec_a = copy_width(q.lhs, q.K, q.lhs.s_r, 0);
   a.vec_b = copy_width(q.rhs, q.rhs_t ? q.K : q.N, q.rhs_t ? q.rhs.s_r : q.rhs.s_k, q.rhs.s_b);
-  if (int st = launch_prep(q, 0, q.M, a.p, s)) return st;
+  a.own_plan = clusters == 0 && q.G <= kFewGroups && l.small_cap <= kOwnTiles;
+  if (!a.own_plan)
+    if (int st = launch_prep(q, 0, q.M, a.p, s)) return st;
   if (clusters > 0)
     if (int st = ragged_tensor_dot(q, a.p, ws + l.tensor_ws, clusters, s)) return st;
   ProfileScope prof("ragged_small", s);
@@ -1078,12 +1127,14 @@ int ragged_contract(const RaggedProblem& q, void* workspace, size_t, cudaStream_
   a.splits = 1;
   a.vec_a = copy_width(q.lhs, q.K, q.lhs.s_k, 0);
   a.vec_b = copy_width(q.rhs, q.N, q.rhs.s_k, 0);
+  a.own_plan = clusters == 0 && q.G <= kFewGroups;
   const int64_t units = q.G * a.tiles_k * a.tiles_n;
   // without the tensor-core product one window takes all rows
   const int64_t window = clusters > 0 ? kRaggedWindow : q.M + 1;
   for (int64_t begin = 0; begin == 0 || begin < q.M; begin += window) {
     a.add = begin > 0;
-    if (int st = launch_prep(q, begin, begin + window, a.p, s)) return st;
+    if (!a.own_plan)
+      if (int st = launch_prep(q, begin, begin + window, a.p, s)) return st;
     if (clusters > 0)
       if (int st = ragged_tensor_contract(q, a.p, a.add, ws + l.tensor_ws, clusters, s)) return st;
     ProfileScope prof("ragged_small", s);

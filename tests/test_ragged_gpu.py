@@ -89,6 +89,22 @@ def test_contraction(case):
     check(ref.value_of(host(torch.stack([hi, lo], -1))), want, bound)
 
 
+@pytest.mark.parametrize("M,K,G", [(4096, 24, 32), (4160, 24, 32), (900, 40, 33), (9000, 12, 1300),
+                                   (70, 700, 5), (40, 1030, 40)])
+def test_tiles_of_every_kind(M, K, G):
+    """Groups of 0 to 200 rows, so that tails of every size stand behind the full
+    tiles; as many groups and tiles as a block plans for itself, one more, and
+    more than a pass of the planning kernel takes; contractions in several parts."""
+    from ds_b200 import ops
+    rng = np.random.default_rng(M + G)
+    sizes = rng.integers(0, max(2, min(200, 2 * M // G)), G).tolist()
+    x, w, y, _ = make((M, K, 30, sizes), 3)
+    want, bound = ref.ragged_dot(x, w, sizes)
+    check(host(ops.ds_ragged_dot_f64(cu(x), cu(w), sz(sizes))), want, bound)
+    want, bound = ref.ragged_contract(x, y, sizes)
+    check(host(ops.ds_ragged_dot_contract_f64(cu(x), cu(y), sz(sizes))), want, bound)
+
+
 @pytest.mark.parametrize("M,K,N,G", [(0, 4, 5, 3), (6, 0, 5, 3), (6, 4, 0, 3), (6, 4, 5, 0)])
 def test_empty(M, K, N, G):
     """No rows, columns or groups: nothing; no contraction or no group: zeros."""
