@@ -898,24 +898,31 @@ int splits_of(int64_t M, int64_t K, int64_t N, int64_t G) {
 
 // Whether the tensor-core product takes the large groups: where its estimated
 // time is below the FP64 path's.  In microseconds, from measurements on one B200:
-// the FP64 path takes 12 us and does 26 TFLOP/s; the tensor-core product has
-// launches of 60 (contraction: 80) us, splits a value in 5.5 to 7.2 (6.5) ps,
-// multiplies at 3 POPS of its 28 operations per product but takes at least 0.76 us
-// per 256 x 256 outputs (short contractions), and rebuilds an output in 5.5 ps.
-// Measured with / without: 2048 x 1024 x 1024 in 4 groups 132 / 190 us
-// (contraction 173 / 169), 4096 x 1024 x 1024 in 8 groups 208 / 333 (232 / 318),
+// the FP64 path takes 9 us and does 26 TFLOP/s; the tensor-core product has
+// launches of 60 us (50 with K-contiguous matrices) for each 32768 of K, as a
+// contraction 80, splits a value in 5 to 7.2 ps, multiplies at 3 POPS of its 28
+// operations per product but takes at least 0.76 us per 256 x 256 outputs (short
+// contractions), and rebuilds an output in 5.5 ps; a matrix counts with whole tiles
+// of 256 columns.  Measured with / without: 2048 x 1024 x 1024 in 4 groups 132 /
+// 190 us (contraction 173 / 169), 4096 x 1024 x 1024 in 8 groups 208 / 333 (232 / 318),
 // 2048 x 2048 x 2048 in 4 groups 286 / 646 (368 / 624), 8192 x 512 x 512 in 8 groups
 // 175 / 177 (159 / 183), 1024 x 1024 x 1024 in one 90 / 106 (128 / 97), 4096 x 256 x
-// 2048 in 4 groups 208 / 173 (177 / 183).
-bool tensor_allowed(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
+// 2048 in 4 groups 208 / 173 (177 / 183), 494 x 1910 x 1292 in one 109 / 104
+// (K-contiguous 91 / 105), 700 x 33041 x 300 in 3 groups 966 / 630, 33041 rows of 300
+// x 400 contracted in 2 groups 608 / 788, in 5 545 / 550.
+bool tensor_allowed(int64_t M, int64_t K, int64_t N, int64_t G, bool contract, bool rhs_t) {
   if (M < tensor_rows(contract) || K < 64 || N < 64) return false;
   const double m = M, k = K, n = N, slots = static_cast<double>(ragged_slots(M, G, contract));
   const double macs = m * k * n, matrices = slots * k * n, outputs = contract ? matrices : m * n;
-  const double plain = 12 + 7.7e-8 * macs;
-  const double gemm = 9.3e-9 * macs, least = 1.15e-5 * outputs;
-  const double split = contract ? 6.5e-6 * m * (k + n) : 5.5e-6 * m * k + 7.2e-6 * matrices;
-  const double tensor = (contract ? 80 : 60) + split + (gemm > least ? gemm : least) +
-                        5.5e-6 * outputs;
+  const double padded = static_cast<double>(ceil_div(N, 256) * 256) / n;
+  const double plain = 9 + 7.7e-8 * macs;
+  const double chunks = static_cast<double>(ceil_div(K, kRaggedWindow));
+  const double launches = contract ? 80 : (rhs_t ? 50 : 60) * chunks;
+  const double split =
+      contract ? 6.5e-6 * m * (k + n)
+               : 5.5e-6 * m * k + (rhs_t ? 5e-6 : 7.2e-6) * matrices * padded;
+  const double gemm = 9.3e-9 * macs * padded, least = 1.15e-5 * outputs;
+  const double tensor = launches + split + (gemm > least ? gemm : least) + 5.5e-6 * outputs;
   return tensor < plain && ragged_tensor_fits(M, K, N, G, contract);
 }
 
@@ -926,7 +933,7 @@ struct Layout {
   bool tensor_ok;
 };
 
-Layout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
+Layout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract, bool rhs_t) {
   Layout l{};
   size_t at = 0;
   auto take = [&at](size_t bytes) {
@@ -935,7 +942,7 @@ Layout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract) {
     return here;
   };
   const int64_t groups = G < M ? G : M;  // with rows
-  l.tensor_ok = tensor_allowed(M, K, N, G, contract);
+  l.tensor_ok = tensor_allowed(M, K, N, G, contract, rhs_t);
   l.small_cap = contract ? 0 : M / kSmallTile + groups;
   if (l.tensor_ok) {
     const int64_t rows = contract && M > kRaggedWindow ? kRaggedWindow : M;
@@ -1077,13 +1084,13 @@ int launch_prep(const RaggedProblem& q, int64_t begin, int64_t end, const Ragged
 
 }  // namespace
 
-size_t ragged_dot_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, bool) {
-  return layout_of(M, K, N, G, false).total;
+size_t ragged_dot_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, bool rhs_t) {
+  return layout_of(M, K, N, G, false, rhs_t).total;
 }
 
 int ragged_dot(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) {
   if (q.M == 0 || q.N == 0) return ok();
-  const Layout l = layout_of(q.M, q.K, q.N, q.G, false);
+  const Layout l = layout_of(q.M, q.K, q.N, q.G, false, q.rhs_t);
   int clusters = 0;
   if (l.tensor_ok)
     if (int st = ragged_tensor_clusters(&clusters)) return st;
@@ -1108,12 +1115,12 @@ int ragged_dot(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) 
 }
 
 size_t ragged_contract_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G) {
-  return layout_of(M, K, N, G, true).total;
+  return layout_of(M, K, N, G, true, false).total;
 }
 
 int ragged_contract(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) {
   if (q.G == 0 || q.K == 0 || q.N == 0) return ok();
-  const Layout l = layout_of(q.M, q.K, q.N, q.G, true);
+  const Layout l = layout_of(q.M, q.K, q.N, q.G, true, false);
   int clusters = 0;
   if (l.tensor_ok)
     if (int st = ragged_tensor_clusters(&clusters)) return st;

@@ -474,13 +474,22 @@ def test_long_contractions():
     n = 33000 + 41
     x, w = on_gpu(700, n, seed=19), on_gpu(3, n, 300, seed=20)
     wt = w.transpose(1, 2).contiguous()
-    with Reached():
-        out = ops.ds_ragged_dot_f64(x, w, sz([400, 40, 250]))
-        outt = ops.ds_ragged_dot_f64(x, wt, sz([400, 40, 250]), rhs_contracting=2)
+    out = ops.ds_ragged_dot_f64(x, w, sz([400, 40, 250]))
+    outt = ops.ds_ragged_dot_f64(x, wt, sz([400, 40, 250]), rhs_contracting=2)
     for g, b, e in ref.spans([400, 40, 250], 700):
         within(out[b:e], *expect(x[b:e], w[g]))
         within(outt[b:e], *expect(x[b:e], w[g]))
     assert not out[690:].any()
+    x, w = on_gpu(1100, n, seed=23), on_gpu(2, n, 500, seed=24)
+    wt = w.transpose(1, 2).contiguous()
+    with Reached():
+        out = ops.ds_ragged_dot_f64(x, w, sz([600, 490]))
+    with Reached():
+        outt = ops.ds_ragged_dot_f64(x, wt, sz([600, 490]), rhs_contracting=2)
+    for g, b, e in ref.spans([600, 490], 1100):
+        within(out[b:e], *expect(x[b:e], w[g]))
+        within(outt[b:e], *expect(x[b:e], w[g]))
+    assert not out[1090:].any()
     x, y = on_gpu(n, 300, seed=21), on_gpu(n, 400, seed=22)
     for sizes in ([n - 3, 3], [100, 32700, 241], [0, 32768, 0, 273], [32500, 541],
                   [32768 - 100, 100, 273]):
