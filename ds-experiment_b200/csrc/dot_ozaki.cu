@@ -21,7 +21,8 @@
 // quantised to 49 bits relative to its row (column) maximum, i.e. at least
 // the precision of the DS input itself; the products and sums add no error.
 //
-// GEMM kernel (step 2): persistent, one CTA per SM, warp-specialised.
+// GEMM kernel (step 2): persistent, one CTA per SM, warp-specialised.  The CTA-pair
+// form (ozaki.cuh) is the default, this the one without clusters:
 //   warp 0      TMA producer: 128x128 (A) and 256x128 (B) int8 tiles, 128B
 //               swizzle, 4-stage mbarrier ring (48 KB per stage);
 //   warp 1      TMEM allocator and MMA issuer: one thread issues

@@ -565,8 +565,8 @@ __device__ __noinline__ void special_outputs(const RaggedCrt& p, const SpecialRo
 // and 8 out per output: bound by HBM once enough rows are on their way, which
 // the loop's own loads (64 to 126 registers, 20 to 32 warps) did not reach.  Each
 // warp copies its rows to shared memory three ahead: 16.8 million outputs of
-// 2048 x 2048 matrices take 63 us (5.9 TB/s), with loads in the loop and a
-// residue's bias subtracted 117; 33.5 million of a contraction 113 and 226.
+// 2048 x 2048 matrices take 68 us (5.4 TB/s), with loads in the loop and a
+// residue's bias subtracted 117; 33.5 million of a contraction 114 and 226.
 // 8 or 32 rows, or 4 or 6 blocks per SM, are within 1%, and so is five rows ahead.
 constexpr int kRaggedCrtThreads = 128, kCols = 4;
 constexpr int kCrtRows = 16, kCrtAhead = 3, kWarpCols = 32 * kCols;
