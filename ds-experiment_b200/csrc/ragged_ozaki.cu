@@ -549,7 +549,7 @@ __device__ __noinline__ void special_outputs(const RaggedCrt& p, const SpecialRo
         s_hi = __fma_rn(x, p.sum.w[l][0], s_hi);
         s_lo = __fma_rn(x, p.sum.w[l][1], s_lo);
       }
-      out = scale2(scale2(crt_value(p.sum, s_hi, s_lo), -sa), -sb);
+      out = scale2(crt_value(p.sum, s_hi, s_lo), -(sa + sb));
     } else {
       if (sa != kShiftNonFinite && sb != kShiftNonFinite) continue;
       for (int64_t k = 0; k < r.K; ++k)
@@ -752,7 +752,7 @@ __device__ double ragged_dot2(const RaggedCrt& p, const RowView& v, int64_t j, i
   if (threadIdx.x == 0) {
     Dot2 d = s_warp[0];
     for (int w = 1; w < kRaggedFixThreads / 32; ++w) dot2_merge(d, s_warp[w]);
-    r = scale2(scale2(__dadd_rn(d.p, d.s), -da), -db);
+    r = scale2(__dadd_rn(d.p, d.s), -(da + db));  // at once: in two steps it may underflow
   }
   __syncthreads();  // s_warp is reused
   return r;
@@ -816,8 +816,7 @@ __device__ void ragged_dot2_tile(const RaggedCrt& p, int64_t row0, int rows, int
       const int c = tx + 16 * w;
       if (shift_ordinary(sShA[r]) && shift_ordinary(sShB[c]))
         put_result(p.c, (v.out + r) * p.N + j0 + c,
-                   scale2(scale2(__dadd_rn(acc[u][w].p, acc[u][w].s), v.P - sShA[r]),
-                          v.P - sShB[c]));
+                   scale2(__dadd_rn(acc[u][w].p, acc[u][w].s), 2 * v.P - sShA[r] - sShB[c]));
     }
   }
   __syncthreads();

@@ -436,6 +436,54 @@ def test_large_zero_rows_columns_and_wide_range():
                 within(got, p @ q, (p.shape[1] + 2) * 4 * ref.U * terms + 2.0 ** -24 * got.abs())
 
 
+def test_large_scales_beyond_the_range():
+    """Rows times 2^-800 and columns times 2^-200: their scale exponents together
+    leave the f64 range, the results (about 2^-1000) do not, and scaling by powers
+    of two changes no bit of them."""
+    from ds_b200 import ops
+    M, K, N, sizes = 4100, 700, 1000, [1500, 0, 2000, 300]
+    x, w, y = on_gpu(M, K, seed=30), on_gpu(4, K, N, seed=31), on_gpu(M, N, seed=32)
+    s = sz(sizes)
+
+    def scale(n, e):
+        return torch.where(torch.arange(n, device="cuda") % 3 == 0, 2.0 ** e, 1.0).double()
+    rows, feats, cols = scale(M, -800), scale(K, -800), scale(N, -200)
+    cases = (
+        (lambda a, b: ops.ds_ragged_dot_f64(a, b, s), x, w, rows[:, None], cols,
+         rows[:, None] * cols),
+        (lambda a, b: ops.ds_ragged_dot_f64(a, b.transpose(1, 2).contiguous(), s,
+                                            rhs_contracting=2), x, w, rows[:, None], cols,
+         rows[:, None] * cols),
+        (lambda a, b: ops.ds_ragged_dot_contract_f64(a, b, s), x, y, feats, cols,
+         feats[:, None] * cols))
+    for f, a, b, sa, sb, want in cases:
+        with Reached():
+            base, got = f(a, b), f(a * sa, b * sb)
+        far = base.abs() > 2.0 ** -20  # those below may become subnormal
+        assert torch.equal(got[far], (base * want)[far]) and bool(far.any())
+        assert bool(((got - base * want).abs() <= 2.0 ** -1073).all())
+
+
+def test_large_subnormal_rows():
+    """Rows and matrices whose every value is subnormal, with nothing in its high
+    word, keep all their bits: integers times the smallest f64."""
+    from ds_b200 import ops
+    M, K, N, sizes = 4100, 700, 1000, [1500, 0, 2000, 300]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(40)
+
+    def ints(*shape):
+        return torch.randint(-2 ** 20, 2 ** 20, shape, generator=g, device="cuda").double()
+    x, w, s = ints(M, K), ints(4, K, N), sz(sizes)
+    tiny, back = 2.0 ** -1074, 2.0 ** 500
+    with Reached():
+        base = ops.ds_ragged_dot_f64(x, w, s)
+        rows = ops.ds_ragged_dot_f64(x * tiny, w * back, s)
+        wt = (w * tiny).transpose(1, 2).contiguous()
+        cols = ops.ds_ragged_dot_f64(x * back, wt, s, rhs_contracting=2)
+    assert torch.equal(rows, base * 2.0 ** -574) and torch.equal(cols, rows) and bool(base.any())
+
+
 def test_large_graph_replayed_with_other_sizes():
     """One captured graph for every split of the rows: groups change kind."""
     from ds_b200 import ops
