@@ -381,7 +381,8 @@ _SCAN_TYPES = {"f64": _lib.DS_FUSED_F64, "f32": _lib.DS_FUSED_F32, "packed": _li
 class _Plan:
     """What a recurrence or grouped product of given shapes needs of each call:
     built on its first call, read-only afterwards."""
-    __slots__ = ("fn", "dtypes", "present", "dims", "specs", "workspace", "attr", "keep")
+    __slots__ = ("fn", "dtypes", "present", "specs", "like", "table", "offsets", "workspace",
+                 "attr", "keep")
 
 
 # (entry point, device index, rhs_contracting, operand shapes...) -> _Plan
@@ -409,16 +410,24 @@ def _make_plan(sym, conv, args, specs, contracting):
     L = _lib.lib()
     plan.dtypes = conv.args
     plan.present = tuple(t is not None for t in args)
-    plan.keep, plan.dims = [], []
+    plan.keep, plan.table, plan.offsets = [], array.array("Q"), []
     for shape in [None if t is None else tuple(t.shape) for t in args] + [s.shape for s in specs]:
+        plan.offsets.append(None if shape is None else 8 * len(plan.table))
         if shape is None:
-            plan.dims.append(None)
+            plan.table.extend((0, 0, 0))
             continue
         _, d = _lib.make_buffer(0, shape)
         plan.keep.append(d)  # the dims the plan's addresses point into
-        plan.dims.append((ctypes.addressof(d), len(shape)))
+        plan.table.extend((0, ctypes.addressof(d), len(shape)))
     plan.specs = [(s.shape, s.dtype) for s in specs]
+    # the operand that a result is made like (cheaper than from its shape)
+    plan.like = [next((i for i, t in enumerate(args)
+                       if t is not None and tuple(t.shape) == s.shape and t.dtype == s.dtype), None)
+                 for s in specs]
+    n = len(plan.offsets)
     plan.attr = contracting if conv.kind == "ragged" else None
+    if plan.attr is not None:
+        plan.offsets.insert(len(args), None)
 
     def ref(t):
         b, d = _lib.make_buffer(t.data_ptr(), t.shape)
@@ -433,7 +442,7 @@ def _make_plan(sym, conv, args, specs, contracting):
     else:
         plan.workspace = L.ds_ragged_dot_contract_workspace_size(ref(args[0]), ref(args[-2]),
                                                                  ref(args[-1]))
-    plan.fn = _fast_fn(sym, conv.kind, len(plan.dims))
+    plan.fn = _fast_fn(sym, conv.kind, n)
     return plan
 
 
@@ -463,25 +472,28 @@ def _plan_key(sym, index, contracting, args):
 
 def _run_plan(target_name, plan, args, index, out):
     if out is None:
-        first = args[0]
-        out = [first.new_empty(shape, dtype=dtype) for shape, dtype in plan.specs]
-    words = []
-    for t, d in zip((*args, *out), plan.dims):
-        if d is None:
-            words += (0, 0, 0)
-        else:
-            words += (t.data_ptr(), d[0], d[1])
-    table = array.array("Q", words)
-    at = table.buffer_info()[0]
-    pointers = [at + 24 * i if d is not None else None for i, d in enumerate(plan.dims)]
+        out = [torch.empty_like(args[i]) if i is not None else
+               args[0].new_empty(shape, dtype=dtype)
+               for i, (shape, dtype) in zip(plan.like, plan.specs)]
+    table = plan.table[:]  # the call's own: (data, dims, rank) of each buffer
+    at = 0
+    for t in args:
+        if t is not None:
+            table[at] = t.data_ptr()
+        at += 3
+    for t in out:
+        table[at] = t.data_ptr()
+        at += 3
+    base = table.buffer_info()[0]
+    words = [None if o is None else base + o for o in plan.offsets]
     if plan.attr is not None:
-        pointers.insert(len(args), plan.attr)
+        words[len(args)] = plan.attr
     stream = _lib.current_stream_ptr(index)
     ws, wsp = None, None
     if plan.workspace:
         ws = _workspace(plan.workspace, args[0].device, stream)
         wsp = ws.data_ptr()
-    _lib.check(plan.fn(*pointers, wsp, plan.workspace, stream), target_name)
+    _lib.check(plan.fn(*words, wsp, plan.workspace, stream), target_name)
     return out
 
 
