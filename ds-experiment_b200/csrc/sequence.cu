@@ -32,6 +32,12 @@
 // always some block's current one, so the chain moves; each wait is bounded
 // (about 2 s), after which the unit works with NaN.
 //
+// A composed map is not the steps where a product of coefficients leaves the f64
+// range and the states do not.  Such a channel's chunk is stepped through, thread
+// after thread, and hands on the state at its end in place of its map (see tiny):
+// with every chunk stepped [8, 2048, 1024] of f64 takes 119 us instead of 69,
+// [1, 65536, 250], whose chunks then wait for one another, 2.7 ms instead of 110 us.
+//
 // Measured on one B200 (cold L2, launch included): f64 [8, 2048, 1024] 80 us =
 // 5.0 TB/s, its gradient 129 us = 5.2 TB/s, [1, 65536, 250] 112 us, f32 [4, 4096,
 // 2048] 90 us.  A plain kernel that reads two arrays of that size and writes a
@@ -150,23 +156,43 @@ __device__ __forceinline__ bool not_finite(double v) {
   return (__double2hiint(v) & 0x7ff00000) == 0x7ff00000;
 }
 
-// A zero state stays out of the product, so that coefficients whose product
-// has overflowed do not turn it into NaN (a coefficient that is itself NaN or
-// infinite has made s NaN already).  Looked at only where the result is not
-// finite: 0 p + s is s for a finite p, and a comparison in f64 costs as much as
-// the step.
 __device__ __forceinline__ double apply(const Map& m, double state) {
-  const double r = __fma_rn(m.p, state, m.s);
-  if (not_finite(r) && state == 0.0) return m.s;
-  return r;
+  return __fma_rn(m.p, state, m.s);
 }
 
 // first, then second.
 __device__ __forceinline__ Map compose(const Map& first, const Map& second) {
-  double p = __dmul_rn(second.p, first.p);
-  if (not_finite(p) && first.p == 0.0) p = 0.0;
-  return Map{p, apply(second, first.s)};
+  return Map{__dmul_rn(second.p, first.p), apply(second, first.s)};
 }
+
+// Products of coefficients may leave the f64 range where no state does: one that
+// overflows meets a tiny state, or a coefficient of zero (inf 0 is NaN, the state
+// is 0); one that underflows meets a large state, or coefficients that make it
+// large again.  So a channel's chunk is stepped through one step after another, as
+// the loop does, where
+//   a map of its threads or of their composition is not finite,
+//   a product is below the normal range (tiny) and a coefficient of the chunk is
+//   above 1, or
+//   a tiny product meets a state above 2^64.
+// Elsewhere a tiny product is below 2^-1021 and off by at most 2^-1075 in each of
+// up to 1024 roundings, and the state that it is multiplied with is at most 2^71
+// (a thread's is at most 2^64): a result is off by at most 2^-994.
+__device__ __forceinline__ bool tiny(double p) {
+  return (__double2hiint(p) & 0x7ff00000) == 0;
+}
+__device__ __forceinline__ bool beyond(double state) {
+  return (__double2hiint(state) & 0x7fffffff) >= (1023 + 64) << 20;
+}
+__device__ __forceinline__ bool large(double state) {
+  return beyond(state) && !not_finite(state);
+}
+
+// Bit 30 is set for |a| >= 1 + 2^-20 (1024 factors below that are 2^0.002), also
+// in the bitwise or of several.  A NaN may not set it; it is not finite.
+__device__ __forceinline__ uint32_t growth_bits(double a) {
+  return static_cast<uint32_t>(__double2hiint(a)) + 0xfffffu;
+}
+__device__ __forceinline__ bool grows(uint32_t bits) { return (bits & 0x40000000u) != 0; }
 
 template <class E>
 struct ChunkArgs {
@@ -247,6 +273,24 @@ __device__ __forceinline__ double wait_state(const uint64_t* at, uint32_t* err) 
   return __longlong_as_double(static_cast<long long>(v));
 }
 
+// The state at the end of a chunk that was stepped through, in place of its map: an
+// infinite product says so.
+constexpr uint64_t kEnd = 0x7ff0000000000000ull;
+__device__ __forceinline__ void put_end(ulonglong2* at, double end) {
+  put_map(at, Map{__longlong_as_double(static_cast<long long>(kEnd)), end});
+}
+
+// The state after the chunk whose message at `at` was m, from the one before it.
+// A tiny product and a large state: that chunk gives its end after its map.
+__device__ __forceinline__ double pass(const ulonglong2* at, const Map& m, double state,
+                                       uint32_t* err) {
+  if (not_finite(m.p)) return m.s;
+  if (!(tiny(m.p) && large(state))) return apply(m, state);
+  ulonglong2 v;
+  if (!poll([&] { return (v = look_at_map(at)).x == kEnd; }, err)) v.y = 0x7ff8000000000000ull;
+  return __longlong_as_double(static_cast<long long>(v.y));
+}
+
 // V neighbouring channels, moved as one word.
 template <class E, int V>
 struct alignas(sizeof(E) * V) Word {
@@ -265,27 +309,28 @@ __device__ __forceinline__ void copy_async(W* dst, const void* src) {
 }
 
 // One thread's part of a unit: R steps of V channels.
+template <int V, int CT, int R>
 struct Part {
+  static constexpr int N = CT / V, S = kThreads / N;
   uint32_t chunk, tile;
-  int64_t c;     // first channel
-  int64_t p0;    // first step (gradient: counted from the end)
-  int64_t row;   // element of the first step's row
-  int n;         // steps it has
+  int64_t row;  // element of the first step's row
+  int n;        // steps it has
+  // first channel, and first step (gradient: counted from the end)
+  __device__ __forceinline__ uint32_t c() const { return tile * CT + threadIdx.x % N * V; }
+  __device__ __forceinline__ int64_t p0() const {
+    return (static_cast<int64_t>(chunk) * S + threadIdx.x / N) * R;
+  }
 };
 
 template <class E, int V, int CT, int R, bool kGrad>
-__device__ __forceinline__ Part part_of(const ChunkArgs<E>& p, uint32_t unit) {
-  constexpr int N = CT / V, S = kThreads / N;
-  Part q;
+__device__ __forceinline__ Part<V, CT, R> part_of(const ChunkArgs<E>& p, uint32_t unit) {
+  Part<V, CT, R> q;
   q.chunk = unit / p.tiles;
   q.tile = unit - q.chunk * p.tiles;
-  const uint32_t c = q.tile * CT + threadIdx.x % N * V;
-  const uint32_t seq = c / p.D;
-  q.c = c;
-  q.p0 = (static_cast<int64_t>(q.chunk) * S + threadIdx.x / N) * R;
-  const int64_t left = c < p.C ? p.T - q.p0 : 0;
+  const uint32_t c = q.c(), seq = c / p.D;
+  const int64_t p0 = q.p0(), left = c < p.C ? p.T - p0 : 0;
   q.n = left < 0 ? 0 : left < R ? static_cast<int>(left) : R;
-  q.row = (seq * p.T + (kGrad ? p.T - 1 - q.p0 : q.p0)) * p.D + (c - seq * p.D);
+  q.row = (seq * p.T + (kGrad ? p.T - 1 - p0 : p0)) * p.D + (c - seq * p.D);
   return q;
 }
 
@@ -302,8 +347,8 @@ struct Slots {
 };
 
 // Values of a part on their way.  kFull: it has all R steps.
-template <bool kFull, class E, int V, int R, bool kGrad>
-__device__ __forceinline__ void issue_part(const ChunkArgs<E>& p, const Part& q,
+template <bool kFull, class E, int V, int CT, int R, bool kGrad>
+__device__ __forceinline__ void issue_part(const ChunkArgs<E>& p, const Part<V, CT, R>& q,
                                            const Slots<E, V, R>& s) {
   const int64_t dir = kGrad ? -static_cast<int64_t>(p.D) : static_cast<int64_t>(p.D);
   const E* x = p.x + q.row;
@@ -316,9 +361,9 @@ __device__ __forceinline__ void issue_part(const ChunkArgs<E>& p, const Part& q,
     if constexpr (kGrad) {
       // the last step in time has no coefficient after it, the first one the
       // state h0 before it
-      if (i > 0 || q.p0 > 0) copy_async(s.a + i * kThreads, a);
-      if ((kFull && i < R - 1) || q.p0 + i < p.T - 1) copy_async(s.h + i * kThreads, h);
-      else if (p.h0) copy_async(s.h + i * kThreads, p.h0 + q.c);
+      if (i > 0 || q.p0() > 0) copy_async(s.a + i * kThreads, a);
+      if ((kFull && i < R - 1) || q.p0() + i < p.T - 1) copy_async(s.h + i * kThreads, h);
+      else if (p.h0) copy_async(s.h + i * kThreads, p.h0 + q.c());
       h += dir;
     } else {
       copy_async(s.a + i * kThreads, a);
@@ -328,23 +373,25 @@ __device__ __forceinline__ void issue_part(const ChunkArgs<E>& p, const Part& q,
   }
 }
 
-template <class E, int V, int R, bool kGrad>
-__device__ __forceinline__ void issue(const ChunkArgs<E>& p, const Part& q,
+template <class E, int V, int CT, int R, bool kGrad>
+__device__ __forceinline__ void issue(const ChunkArgs<E>& p, const Part<V, CT, R>& q,
                                       const Slots<E, V, R>& s) {
-  if (q.n == R) issue_part<true, E, V, R, kGrad>(p, q, s);
-  else if (q.n > 0) issue_part<false, E, V, R, kGrad>(p, q, s);
+  if (q.n == R) issue_part<true, E, V, CT, R, kGrad>(p, q, s);
+  else if (q.n > 0) issue_part<false, E, V, CT, R, kGrad>(p, q, s);
 }
 
-// A part's values, widened once: a conversion costs a quarter of the FP64 rate.
-template <int V, int R, bool kGrad>
+// A part's values, those used twice widened once: a conversion costs a quarter of
+// the FP64 rate.
+template <class E, int V, int R, bool kGrad>
 struct Values {
-  double a[R][V], x[R][V], h[kGrad ? R : 1][V];
+  double a[R][V], x[R][V];
+  E h[kGrad ? R : 1][V];
 };
 
 // Steps that the part does not have do nothing: s -> 1 s + 0.
-template <class E, int V, int R, bool kGrad>
-__device__ __forceinline__ void read(const ChunkArgs<E>& p, const Part& q, const Slots<E, V, R>& s,
-                                     Values<V, R, kGrad>& v) {
+template <class E, int V, int CT, int R, bool kGrad>
+__device__ __forceinline__ void read(const ChunkArgs<E>& p, const Part<V, CT, R>& q,
+                                     const Slots<E, V, R>& s, Values<E, V, R, kGrad>& v) {
   using IO = SeqIO<E>;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -357,14 +404,14 @@ __device__ __forceinline__ void read(const ChunkArgs<E>& p, const Part& q, const
     if constexpr (kGrad) {
       const Word<E, V> h = s.h[i * kThreads];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v.h[i][j] = IO::value(h.v[j]);
+      for (int j = 0; j < V; ++j) v.h[i][j] = h.v[j];
     }
   }
-  if (kGrad && q.p0 == 0) {
+  if (kGrad && q.p0() == 0) {
 #pragma unroll
     for (int j = 0; j < V; ++j) v.a[0][j] = 1.0;
   }
-  if (q.n == R && !(kGrad && !p.h0 && q.p0 + R == p.T)) return;
+  if (q.n == R && !(kGrad && !p.h0 && q.p0() + R == p.T)) return;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
 #pragma unroll
@@ -374,16 +421,16 @@ __device__ __forceinline__ void read(const ChunkArgs<E>& p, const Part& q, const
         v.a[i][j] = 1.0;
       }
       if constexpr (kGrad) {
-        if (!p.h0 && q.p0 + i == p.T - 1) v.h[i][j] = 0.0;
+        if (!p.h0 && q.p0() + i == p.T - 1) v.h[i][j] = IO::zero();
       }
     }
   }
 }
 
 // The steps from `state` on, stored.
-template <bool kFull, class E, int V, int R, bool kGrad>
-__device__ __forceinline__ void run_part(const ChunkArgs<E>& p, const Part& q,
-                                         const Values<V, R, kGrad>& v, double (&state)[V]) {
+template <bool kFull, class E, int V, int CT, int R, bool kGrad>
+__device__ __forceinline__ void run_part(const ChunkArgs<E>& p, const Part<V, CT, R>& q,
+                                         const Values<E, V, R, kGrad>& v, double (&state)[V]) {
   using IO = SeqIO<E>;
   const int64_t dir = kGrad ? -static_cast<int64_t>(p.D) : static_cast<int64_t>(p.D);
   E* out = p.out + q.row;
@@ -395,21 +442,28 @@ __device__ __forceinline__ void run_part(const ChunkArgs<E>& p, const Part& q,
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       state[j] = __fma_rn(v.a[i][j], state[j], v.x[i][j]);
-      if constexpr (kGrad) g[j] = __dmul_rn(state[j], v.h[i][j]);
+      if constexpr (kGrad) g[j] = __dmul_rn(state[j], IO::value(v.h[i][j]));
     }
     IO::template put<V>(out, state);
     out += dir;
     if constexpr (kGrad) {
       IO::template put<V>(ga, g);
       ga += dir;
-      if ((!kFull || i == R - 1) && q.p0 + i == p.T - 1) {
+      if ((!kFull || i == R - 1) && q.p0() + i == p.T - 1) {
         const E* a0 = p.a + q.row + i * dir;
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          IO::store(p.gh0 + q.c + j, __dmul_rn(IO::value(IO::load(a0 + j)), state[j]));
+          IO::store(p.gh0 + q.c() + j, __dmul_rn(IO::value(IO::load(a0 + j)), state[j]));
       }
     }
   }
+}
+
+// The state before the first step of channel threadIdx.x of a tile.
+template <class E, int CT, bool kGrad>
+__device__ __forceinline__ double state_h0(const ChunkArgs<E>& p, uint32_t tile) {
+  const uint32_t c = tile * CT + threadIdx.x;
+  return !kGrad && p.h0 && c < p.C ? SeqIO<E>::value(SeqIO<E>::load(p.h0 + c)) : 0.0;
 }
 
 template <class E, int V, int CT, int R, bool kGrad>
@@ -417,7 +471,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 scan_chunk_kernel(const __grid_constant__ ChunkArgs<E> p) {
   constexpr int N = CT / V;         // threads across the channels
   constexpr int S = kThreads / N;   // and along the steps
-  using IO = SeqIO<E>;
+  // Whether a thread's smallest product is kept from step to step, or found by a
+  // second pass where a coefficient is above 1.  The pass costs most threads nothing
+  // (f32 [4, 4096, 2048] 86 us, kept 87), but spills with the more steps of V = 1
+  // (f64 [8, 2048, 1023] 83 us, kept 80).
+  constexpr bool kTrack = V == 1;
   extern __shared__ __align__(16) uint8_t smem[];
   Slots<E, V, R> slots;
   slots.a = reinterpret_cast<Word<E, V>*>(smem) + threadIdx.x;
@@ -427,6 +485,13 @@ scan_chunk_kernel(const __grid_constant__ ChunkArgs<E> p) {
   __shared__ Map s_before[kMaxRound][CT];
   __shared__ double s_start[CT];
   __shared__ uint32_t s_unit[2];
+  // the last of the block's units in which a channel has a
+  // coefficient above 1, has a tiny product, and is stepped through
+  __shared__ uint32_t s_grows[CT], s_tiny[CT], s_stepped[CT];
+  // the last one with a coefficient above 1 or a state beyond 2^64 in a thread's
+  // map, with a channel that is stepped through, and with a map from another block
+  // that is not an ordinary one
+  __shared__ uint32_t s_careful, s_any_stepped, s_special;
   const int tid = threadIdx.x, cl = tid % N * V, sub = tid / N;
 
   wait_previous_grid();
@@ -436,52 +501,92 @@ scan_chunk_kernel(const __grid_constant__ ChunkArgs<E> p) {
     if (u + p.tiles < p.units) return u + p.tiles;
     return u % p.tiles + gridDim.x < p.tiles ? u % p.tiles + gridDim.x : p.units;
   };
-  if (p.counter) {
-    if (tid == 0) s_unit[0] = atomicAdd(p.counter, 1u) + 1u;
-    __syncthreads();
-    unit = s_unit[0];
-  }
+  if (tid < CT) s_grows[tid] = s_tiny[tid] = s_stepped[tid] = ~0u;
+  if (tid == 0) s_careful = s_any_stepped = s_special = ~0u;
+  if (p.counter && tid == 0) s_unit[0] = atomicAdd(p.counter, 1u) + 1u;
+  __syncthreads();
+  if (p.counter) unit = s_unit[0];
   if (unit >= p.units) return;
-  Part q = part_of<E, V, CT, R, kGrad>(p, unit);
-  issue<E, V, R, kGrad>(p, q, slots);
+  Part<V, CT, R> q = part_of<E, V, CT, R, kGrad>(p, unit);
+  issue<E, V, CT, R, kGrad>(p, q, slots);
   int turn = 0;
   for (;;) {
     turn ^= 1;
     if (p.counter && tid == 0) s_unit[turn] = atomicAdd(p.counter, 1u) + 1u;
+    if (!p.counter && tid < CT && q.chunk == 0)
+      s_start[tid] = state_h0<E, CT, kGrad>(p, q.tile);
     asm volatile("cp.async.wait_all;" ::: "memory");
-    Values<V, R, kGrad> val;
-    read<E, V, R, kGrad>(p, q, slots, val);
+    Values<E, V, R, kGrad> val;
+    read<E, V, CT, R, kGrad>(p, q, slots, val);
     // the slots are this thread's own: the next unit's values may come
-    const Part cur = q;
+    const Part<V, CT, R> cur = q;
     uint32_t next = p.units;
     if (!p.counter) {
       next = after(unit);
       if (next < p.units) {
         q = part_of<E, V, CT, R, kGrad>(p, next);
-        issue<E, V, R, kGrad>(p, q, slots);
+        issue<E, V, CT, R, kGrad>(p, q, slots);
       }
     }
     Map m[V];
+    uint32_t growth[V];
+    int lowest[V];  // high word of the smallest product
 #pragma unroll
-    for (int j = 0; j < V; ++j) m[j] = Map{1.0, 0.0};
+    for (int j = 0; j < V; ++j) {
+      m[j] = Map{1.0, 0.0};
+      growth[j] = 0;
+      lowest[j] = 0x7fffffff;
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         m[j].s = __fma_rn(val.a[i][j], m[j].s, val.x[i][j]);
         m[j].p = __dmul_rn(m[j].p, val.a[i][j]);
+        growth[j] |= growth_bits(val.a[i][j]);
+        if constexpr (kTrack) lowest[j] = min(lowest[j], __double2hiint(m[j].p) & 0x7fffffff);
       }
     }
+    bool low[V], steps[V];  // a product is tiny; the channel is to be stepped through
     // inclusive scan over the S threads of a channel
     int buf = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) s_map[0][sub][j * N + tid % N] = m[j];
+    for (int j = 0; j < V; ++j) {
+      steps[j] = false;
+      s_map[0][sub][j * N + tid % N] = m[j];
+      low[j] = kTrack ? lowest[j] < 0x00100000 : tiny(m[j].p);
+      if (grows(growth[j])) {
+        s_grows[cl + j] = s_careful = unit;
+        if constexpr (!kTrack) {
+          double product = 1.0;
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            product = __dmul_rn(product, val.a[i][j]);
+            low[j] |= tiny(product);
+          }
+        }
+      }
+      if (beyond(m[j].s)) s_careful = unit;
+    }
     __syncthreads();
     if (p.counter) {
       next = s_unit[turn];
       if (next < p.units) {
         q = part_of<E, V, CT, R, kGrad>(p, next);
-        issue<E, V, R, kGrad>(p, q, slots);
+        issue<E, V, CT, R, kGrad>(p, q, slots);
+      }
+    }
+    // Without a coefficient above 1 and a state beyond 2^64 in a thread's map no
+    // product or state of a composition passes 2^71, and one that is tiny makes
+    // those after it tiny.
+    const bool careful = s_careful == unit;
+    if (careful) {
+      // a product with a coefficient of zero is exact
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (!low[j]) continue;
+#pragma unroll
+        for (int i = 0; i < R; ++i) low[j] &= val.a[i][j] != 0.0;
       }
     }
 #pragma unroll
@@ -489,23 +594,42 @@ scan_chunk_kernel(const __grid_constant__ ChunkArgs<E> p) {
       buf ^= 1;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (sub >= d) m[j] = compose(s_map[buf ^ 1][sub - d][j * N + tid % N], m[j]);
+        if (sub >= d) {
+          const Map first = s_map[buf ^ 1][sub - d][j * N + tid % N];
+          const bool zero = m[j].p == 0.0 || first.p == 0.0;
+          if (careful) steps[j] |= tiny(m[j].p) && large(first.s);
+          m[j] = compose(first, m[j]);
+          if (careful) low[j] |= tiny(m[j].p) && !zero;
+        }
         s_map[buf][sub][j * N + tid % N] = m[j];
       }
-      __syncthreads();
+      if (2 * d < S) __syncthreads();
     }
-    // the state at the chunk's start, by one thread per channel (cs)
-    const int cs = tid;
-    const int64_t channel = static_cast<int64_t>(cur.tile) * CT + cs;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (careful)
+        steps[j] |= not_finite(m[j].p) || not_finite(m[j].s) ||
+                    (low[j] && s_grows[cl + j] == unit);
+      low[j] |= tiny(m[j].p);
+      if (low[j]) {
+        steps[j] |= !p.counter && large(s_start[cl + j]);
+        s_tiny[cl + j] = unit;
+      }
+      if (steps[j]) s_stepped[cl + j] = s_any_stepped = unit;
+    }
+    __syncthreads();
+    bool any_stepped = s_any_stepped == unit;
+    auto stepped = [&](int c) { return any_stepped && s_stepped[c] == unit; };
     if (p.counter) {
       const int64_t slot = static_cast<int64_t>(cur.chunk) * p.tiles + cur.tile;
       const uint32_t rnd = cur.chunk / p.round;
       const int idx = static_cast<int>(cur.chunk - rnd * p.round);
       const bool last = cur.chunk == p.chunks - 1, ends = idx == static_cast<int>(p.round) - 1;
       // a later chunk of the round reads it
-      if (!last && !ends && sub == S - 1) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) put_map(p.maps + slot * CT + cl + j, m[j]);
+      for (int j = 0; j < V; ++j) {
+        steps[j] = stepped(cl + j);
+        if (!last && !ends && sub == S - 1 && !steps[j]) put_map(p.maps + slot * CT + cl + j, m[j]);
       }
       // the round's earlier maps, spread over all threads
       const ulonglong2* maps = p.maps + (slot - static_cast<int64_t>(idx) * p.tiles) * CT;
@@ -519,37 +643,78 @@ scan_chunk_kernel(const __grid_constant__ ChunkArgs<E> p) {
           if (i + u * Q < idx) v[u] = look_at_map(maps + (i + u * Q) * step + cm);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if (i + u * Q < idx)
-            s_before[i + u * Q][cm] = wait_map(maps + (i + u * Q) * step + cm, v[u], p.err);
+          if (i + u * Q < idx) {
+            const Map b = wait_map(maps + (i + u * Q) * step + cm, v[u], p.err);
+            s_before[i + u * Q][cm] = b;
+            if (not_finite(b.p) || tiny(b.p)) s_special = unit;
+          }
       }
       __syncthreads();
+      // the state at the chunk's start, by one thread per channel (cs)
+      const int cs = tid;
       if (cs < CT) {
-        double start = 0.0;
+        double start;
         if (rnd > 0)
           start = wait_state(
               p.states + (static_cast<int64_t>(rnd - 1) * p.tiles + cur.tile) * CT + cs, p.err);
-        else if (!kGrad && p.h0 && channel < p.C)
-          start = IO::value(IO::load(p.h0 + channel));
-        for (int i = 0; i < idx; ++i) start = apply(s_before[i][cs], start);
+        else
+          start = state_h0<E, CT, kGrad>(p, cur.tile);
+        if (s_special != unit)
+          for (int i = 0; i < idx; ++i) start = apply(s_before[i][cs], start);
+        else
+          for (int i = 0; i < idx; ++i)
+            start = pass(maps + i * step + cs, s_before[i][cs], start, p.err);
         s_start[cs] = start;
-        if (!last && ends)
+        const bool late = s_tiny[cs] == unit && large(start);
+        if (late) s_stepped[cs] = s_any_stepped = unit;
+        if (!last && ends && !late && !stepped(cs))
           put_state(p.states + (static_cast<int64_t>(rnd) * p.tiles + cur.tile) * CT + cs,
                     apply(s_map[buf][S - 1][cs % V * N + cs / V], start));
       }
-    } else if (cs < CT && cur.chunk == 0) {
-      s_start[cs] = !kGrad && p.h0 && channel < p.C ? IO::value(IO::load(p.h0 + channel)) : 0.0;
+      __syncthreads();
+      any_stepped = s_any_stepped == unit;
     }
-    if (p.counter || cur.chunk == 0) __syncthreads();
     double state[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       state[j] = s_start[cl + j];
       if (sub > 0) state[j] = apply(s_map[buf][sub - 1][j * N + tid % N], state[j]);
     }
-    if (cur.n == R) run_part<true, E, V, R, kGrad>(p, cur, val, state);
-    else if (cur.n > 0) run_part<false, E, V, R, kGrad>(p, cur, val, state);
+    if (any_stepped) {
+      // thread after thread, the state in s_start
+#pragma unroll 1
+      for (int k = 0; k < S; ++k) {
+        if (sub == k) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            if (!stepped(cl + j)) continue;
+            double s = state[j] = s_start[cl + j];
+#pragma unroll
+            for (int i = 0; i < R; ++i) s = __fma_rn(val.a[i][j], s, val.x[i][j]);
+            s_start[cl + j] = s;
+          }
+        }
+        __syncthreads();
+      }
+      if (p.counter && cur.chunk != p.chunks - 1 && sub == S - 1) {
+        const uint32_t rnd = cur.chunk / p.round;
+        const bool ends = cur.chunk - rnd * p.round == p.round - 1;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (!stepped(cl + j)) continue;
+          const double end = s_start[cl + j];
+          // a map that was given already counts unless its product is tiny
+          if (ends)
+            put_state(p.states + (static_cast<int64_t>(rnd) * p.tiles + cur.tile) * CT + cl + j, end);
+          else if (steps[j] || tiny(s_map[buf][S - 1][j * N + tid % N].p))
+            put_end(p.maps + (static_cast<int64_t>(cur.chunk) * p.tiles + cur.tile) * CT + cl + j, end);
+        }
+      }
+    }
+    if (cur.n == R) run_part<true, E, V, CT, R, kGrad>(p, cur, val, state);
+    else if (cur.n > 0) run_part<false, E, V, CT, R, kGrad>(p, cur, val, state);
     __syncthreads();  // s_map, s_before and s_start are written again
-    if (!p.counter && sub == S - 1) {
+    if (!p.counter && cur.chunk != p.chunks - 1 && sub == S - 1) {
       // where the tile's next chunk starts
 #pragma unroll
       for (int j = 0; j < V; ++j) s_start[cl + j] = state[j];

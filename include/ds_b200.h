@@ -430,9 +430,11 @@ DS_API int ds_fused_reduce_rows_compile_check(const ds_fused_op* ops, int32_t n_
    once to the output's type.  Long sequences are cut into chunks whose
    carries meet in an order fixed by the shape, so results are deterministic.
    A NaN or infinite state stays non-finite for the rest of its sequence, as
-   in the step-by-step loop; products of up to a chunk's coefficients are
-   formed, so a state that would leave the f64 range and come back inside a
-   chunk may differ from that loop.
+   in the step-by-step loop, and a_t = 0 starts a new one exactly whatever
+   finite state stood before.  Where the products of a chunk's coefficients
+   leave the f64 range (which no state need do) its channel is stepped through
+   as in that loop, at a lower speed; what a product below 2^-1022 leaves of a
+   state up to 2^64 counts as zero to within 2^-994.
    Outputs must not overlap operands.  The workspace
    (ds_linear_recurrence_workspace_size bytes, 256-byte aligned; `type` is
    DS_FUSED_F64, DS_FUSED_F32 or DS_FUSED_PACKED) serves one call at a time. */
