@@ -548,7 +548,7 @@ __device__ __forceinline__ void crt_finish(const CrtParams& p, bool failed, int6
     const double c = __fma_rn(t_hi, 0x1p70, t_lo);
     if (!(fabs(c) >= p.certify_below)) {
       // uncertified: listed for fix_kernel, which writes this output
-      const int slot = atomicAdd(p.fix_count, 1);
+      const int64_t slot = list_place(p.fix_count, p.fix_cap);
       if (slot < p.fix_cap) p.fix_list[slot] = static_cast<uint64_t>(row * p.N + j);
       return;
     }
@@ -641,7 +641,7 @@ crt_kernel(CrtParams p) {
         all &= cert[q];
         if (!cert[q]) {
           // uncertified: listed for fix_kernel, which writes this output
-          const int slot = atomicAdd(p.fix_count, 1);
+          const int64_t slot = list_place(p.fix_count, p.fix_cap);
           if (slot < p.fix_cap) p.fix_list[slot] = static_cast<uint64_t>(row * p.N + j0 + q);
         }
         const int e = -(sa + sbv[q]);

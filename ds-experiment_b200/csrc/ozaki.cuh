@@ -298,6 +298,15 @@ __device__ __forceinline__ int shift_from_code(int code, int P) {
   return P - (code - kExpBias);
 }
 
+// Place of an uncertified output in the list of those to recompute: at least `cap`
+// where that is full.  A count past `cap` says so and is not raised further (a call
+// may have more than 2^31 such outputs): it stays within the resident threads of
+// cap + 1, as each looks before it adds one.
+__device__ __forceinline__ int64_t list_place(int* count, int64_t cap) {
+  if (*reinterpret_cast<volatile int*>(count) > cap) return cap;
+  return atomicAdd(count, 1);
+}
+
 // The certificate by the operands' own 1-norms (the products grouped by expert).
 // In units of C_int the quantisation error of an output is at most
 // (||a_int||_1 + ||b_int||_1) / 2 + K / 4, and ||a_int||_1 <= sum |a| 2^sa + K / 2.

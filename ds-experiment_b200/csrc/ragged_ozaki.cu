@@ -693,7 +693,7 @@ ragged_crt_kernel(const __grid_constant__ RaggedCrt p) {
         if (sa == kShiftNonFinite || sb[q] == kShiftNonFinite) special |= 1u << r;
       } else if (!sure[q]) {
         // uncertified: listed for ragged_fix_kernel, which writes this output
-        const int n = atomicAdd(p.fix_count, 1);
+        const int64_t n = list_place(p.fix_count, p.fix_cap);
         if (n < p.fix_cap) p.fix_list[n] = static_cast<uint64_t>((row0 + r) * p.N + j0 + q);
         continue;
       } else if (!in_range(sa + sb[q])) {
