@@ -911,7 +911,7 @@ int splits_of(int64_t M, int64_t K, int64_t N, int64_t G) {
 // (K-contiguous 91 / 105), 700 x 33041 x 300 in 3 groups 966 / 630, 33041 rows of 300
 // x 400 contracted in 2 groups 608 / 788, in 5 545 / 550.
 bool tensor_allowed(int64_t M, int64_t K, int64_t N, int64_t G, bool contract, bool rhs_t) {
-  if (M < tensor_rows(contract) || K < 64 || N < 64) return false;
+  if (G < 1 || M < tensor_rows(contract) || K < 64 || N < 64) return false;
   const double m = M, k = K, n = N, slots = static_cast<double>(ragged_slots(M, G, contract));
   const double macs = m * k * n, matrices = slots * k * n, outputs = contract ? matrices : m * n;
   const double padded = static_cast<double>(ceil_div(N, 256) * 256) / n;

@@ -644,3 +644,18 @@ def test_recurrent_experts_layer():
                       (ggate, lg.grad), (gh0, lh0.grad)):
         got, want = got.cpu(), want.detach()
         assert float((got - want).abs().max()) <= 2.0 ** -30 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("M,K,N", [(2048, 1024, 1024), (8192, 1024, 1024)])
+def test_no_groups_at_batch_size(M, K, N):
+    """Zeros, as of a few rows, for f64 and pairs and either layout."""
+    from ds_b200 import ops
+    x, s = on_gpu(M, K, seed=50), sz([])
+    for contracting, shape in ((1, (0, K, N)), (2, (0, N, K))):
+        w = torch.empty(shape, dtype=torch.float64, device="cuda")
+        out = torch.full((M, N), float("nan"), dtype=torch.float64, device="cuda")
+        ops.ds_ragged_dot_f64(x, w, s, rhs_contracting=contracting, out=out)
+        assert not out.any()
+        hi, lo = ops.ds_ragged_dot(*pair(x), w.float(), w.float(), s, rhs_contracting=contracting)
+        assert hi.shape == lo.shape == (M, N) and not hi.any() and not lo.any()
+    assert ops.ds_ragged_dot_contract_f64(x, on_gpu(M, N, seed=51), s).shape == (0, K, N)

@@ -205,3 +205,14 @@ def test_threads_have_workspaces_of_their_own(monkeypatch):
     t.start()
     t.join()
     assert got[0] is not here and ffi._workspace(100, torch.device("cpu"), 7) is here
+
+
+def test_no_groups_ask_for_no_planes(L):
+    """A product of batch size without groups is zeros: no tensor-core product, whose
+    planes would take hundreds of megabytes."""
+    b = Bufs(L)
+    q = L.lib().ds_ragged_dot_workspace_size
+    for contracting, w in ((1, b(0, 1024, 1024)), (2, b(0, 1024, 1024))):
+        assert 0 < q(R(b(8192, 1024)), R(w), contracting) <= 1 << 20
+    assert 0 < L.lib().ds_ragged_dot_contract_workspace_size(
+        R(b(8192, 1024)), R(b(8192, 1024)), R(b(0))) <= 1 << 20
