@@ -532,6 +532,13 @@ int linear_recurrence_vjp(const char* name, int type, const ds_buffer* a, const 
 constexpr int64_t kRaggedMax = (1LL << 31) - 1024;
 constexpr int64_t kRaggedMaxGroups = 65535;
 
+int ragged_algorithm(const std::string& op, int32_t algorithm, RaggedProblem& p) {
+  if (algorithm != DS_DOT_TENSOR_INT8 && algorithm != DS_DOT_CUDA_CORE)
+    return invalid(op + ": unknown algorithm");
+  p.tensor = algorithm == DS_DOT_TENSOR_INT8;
+  return DS_OK;
+}
+
 int ragged_geometry(const std::string& op, const ds_buffer* lhs, const ds_buffer* rhs,
                     int32_t rhs_contracting, RaggedProblem& p) {
   if (rhs_contracting != 1 && rhs_contracting != 2)
@@ -585,10 +592,11 @@ int ragged_workspace(const std::string& op, size_t need, void* workspace, size_t
 
 int ragged_dot_checked(const std::string& op, RaggedProblem& p, std::initializer_list<Named> ins,
                        std::initializer_list<Named> outs, const ds_buffer* group_sizes,
-                       int32_t rhs_contracting, void* workspace, size_t workspace_bytes,
-                       void* stream) {
+                       int32_t rhs_contracting, int32_t algorithm, void* workspace,
+                       size_t workspace_bytes, void* stream) {
   const ds_buffer* lhs = ins.begin()->b;
   const ds_buffer* rhs = (ins.end() - 2)->b;  // group_sizes is last
+  if (int st = ragged_algorithm(op, algorithm, p)) return st;
   if (int st = ragged_geometry(op, lhs, rhs, rhs_contracting, p)) return st;
   if (group_sizes->rank != 1 || group_sizes->dims[0] != p.G)
     return invalid(op + ": group_sizes must be [G]");
@@ -597,24 +605,25 @@ int ragged_dot_checked(const std::string& op, RaggedProblem& p, std::initializer
       return invalid(op + ": output shape mismatch");
   if (int st = check_overlap(op, ins, outs)) return st;
   p.group_sizes = static_cast<const int32_t*>(group_sizes->data);
-  const size_t need = ragged_dot_workspace_bytes(p.M, p.K, p.N, p.G, p.rhs_t);
+  const size_t need = ragged_dot_workspace_bytes(p);
   if (int st = ragged_workspace(op, need, workspace, workspace_bytes)) return st;
   return ragged_dot(p, workspace, workspace_bytes, as_stream(stream));
 }
 
 int ragged_contract_checked(const std::string& op, RaggedProblem& p,
                             std::initializer_list<Named> ins, std::initializer_list<Named> outs,
-                            const ds_buffer* group_sizes, void* workspace, size_t workspace_bytes,
-                            void* stream) {
+                            const ds_buffer* group_sizes, int32_t algorithm, void* workspace,
+                            size_t workspace_bytes, void* stream) {
   const ds_buffer* lhs = ins.begin()->b;
   const ds_buffer* rhs = (ins.end() - 2)->b;
+  if (int st = ragged_algorithm(op, algorithm, p)) return st;
   if (int st = contract_geometry(op, lhs, rhs, group_sizes, p)) return st;
   for (const Named& o : outs)
     if (o.b->rank != 3 || o.b->dims[0] != p.G || o.b->dims[1] != p.K || o.b->dims[2] != p.N)
       return invalid(op + ": output shape mismatch");
   if (int st = check_overlap(op, ins, outs)) return st;
   p.group_sizes = static_cast<const int32_t*>(group_sizes->data);
-  const size_t need = ragged_contract_workspace_bytes(p.M, p.K, p.N, p.G);
+  const size_t need = ragged_contract_workspace_bytes(p);
   if (int st = ragged_workspace(op, need, workspace, workspace_bytes)) return st;
   return ragged_contract(p, workspace, workspace_bytes, as_stream(stream));
 }
@@ -1073,19 +1082,65 @@ int ds_linear_recurrence_vjp_packed(const ds_buffer* a, const ds_buffer* h,
 
 size_t ds_ragged_dot_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
                                     int32_t rhs_contracting) {
-  if (!valid_buffer(lhs) || !valid_buffer(rhs) || bad_dims(lhs) || bad_dims(rhs)) return 0;
-  if (total_checked(lhs) < 0 || total_checked(rhs) < 0) return 0;
-  const std::string saved = g_last_error;
-  RaggedProblem p;
-  const int st = ragged_geometry("ds_ragged_dot", lhs, rhs, rhs_contracting, p);
-  g_last_error = saved;
-  return st == DS_OK ? ragged_dot_workspace_bytes(p.M, p.K, p.N, p.G, p.rhs_t) : 0;
+  return ds_ragged_dot_algorithm_workspace_size(lhs, rhs, rhs_contracting, DS_DOT_TENSOR_INT8);
 }
 
 int ds_ragged_dot(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo, const ds_buffer* rhs_hi,
                   const ds_buffer* rhs_lo, const ds_buffer* group_sizes, int32_t rhs_contracting,
                   const ds_buffer* out_hi, const ds_buffer* out_lo, void* workspace,
                   size_t workspace_bytes, void* stream) {
+  return ds_ragged_dot_algorithm(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes, rhs_contracting,
+                                 DS_DOT_TENSOR_INT8, out_hi, out_lo, workspace, workspace_bytes,
+                                 stream);
+}
+
+int ds_ragged_dot_f64(const ds_buffer* lhs, const ds_buffer* rhs, const ds_buffer* group_sizes,
+                      int32_t rhs_contracting, const ds_buffer* out, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  return ds_ragged_dot_algorithm_f64(lhs, rhs, group_sizes, rhs_contracting, DS_DOT_TENSOR_INT8,
+                                     out, workspace, workspace_bytes, stream);
+}
+
+size_t ds_ragged_dot_contract_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
+                                             const ds_buffer* group_sizes) {
+  return ds_ragged_dot_contract_algorithm_workspace_size(lhs, rhs, group_sizes,
+                                                         DS_DOT_TENSOR_INT8);
+}
+
+int ds_ragged_dot_contract(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
+                           const ds_buffer* rhs_hi, const ds_buffer* rhs_lo,
+                           const ds_buffer* group_sizes, const ds_buffer* out_hi,
+                           const ds_buffer* out_lo, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  return ds_ragged_dot_contract_algorithm(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes,
+                                          DS_DOT_TENSOR_INT8, out_hi, out_lo, workspace,
+                                          workspace_bytes, stream);
+}
+
+int ds_ragged_dot_contract_f64(const ds_buffer* lhs, const ds_buffer* rhs,
+                               const ds_buffer* group_sizes, const ds_buffer* out,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  return ds_ragged_dot_contract_algorithm_f64(lhs, rhs, group_sizes, DS_DOT_TENSOR_INT8, out,
+                                              workspace, workspace_bytes, stream);
+}
+
+size_t ds_ragged_dot_algorithm_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
+                                              int32_t rhs_contracting, int32_t algorithm) {
+  if (!valid_buffer(lhs) || !valid_buffer(rhs) || bad_dims(lhs) || bad_dims(rhs)) return 0;
+  if (total_checked(lhs) < 0 || total_checked(rhs) < 0) return 0;
+  const std::string saved = g_last_error;
+  RaggedProblem p;
+  int st = ragged_algorithm("ds_ragged_dot", algorithm, p);
+  if (st == DS_OK) st = ragged_geometry("ds_ragged_dot", lhs, rhs, rhs_contracting, p);
+  g_last_error = saved;
+  return st == DS_OK ? ragged_dot_workspace_bytes(p) : 0;
+}
+
+int ds_ragged_dot_algorithm(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
+                            const ds_buffer* rhs_hi, const ds_buffer* rhs_lo,
+                            const ds_buffer* group_sizes, int32_t rhs_contracting,
+                            int32_t algorithm, const ds_buffer* out_hi, const ds_buffer* out_lo,
+                            void* workspace, size_t workspace_bytes, void* stream) {
   const std::string op("ds_ragged_dot");
   const Named LH{lhs_hi, "lhs_hi", 4, 4}, LL{lhs_lo, "lhs_lo", 4, 4}, RH{rhs_hi, "rhs_hi", 4, 4},
       RL{rhs_lo, "rhs_lo", 4, 4}, GS{group_sizes, "group_sizes", 4, 4},
@@ -1101,12 +1156,13 @@ int ds_ragged_dot(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo, const ds_buf
   p.out.hi = static_cast<float*>(out_hi->data);
   p.out.lo = static_cast<float*>(out_lo->data);
   return ragged_dot_checked(op, p, {LH, LL, RH, RL, GS}, {OH, OL}, group_sizes, rhs_contracting,
-                            workspace, workspace_bytes, stream);
+                            algorithm, workspace, workspace_bytes, stream);
 }
 
-int ds_ragged_dot_f64(const ds_buffer* lhs, const ds_buffer* rhs, const ds_buffer* group_sizes,
-                      int32_t rhs_contracting, const ds_buffer* out, void* workspace,
-                      size_t workspace_bytes, void* stream) {
+int ds_ragged_dot_algorithm_f64(const ds_buffer* lhs, const ds_buffer* rhs,
+                                const ds_buffer* group_sizes, int32_t rhs_contracting,
+                                int32_t algorithm, const ds_buffer* out, void* workspace,
+                                size_t workspace_bytes, void* stream) {
   const std::string op("ds_ragged_dot_f64");
   const Named L{lhs, "lhs", 8, 8}, R{rhs, "rhs", 8, 8}, GS{group_sizes, "group_sizes", 4, 4},
       O{out, "out", 8, 8};
@@ -1115,27 +1171,29 @@ int ds_ragged_dot_f64(const ds_buffer* lhs, const ds_buffer* rhs, const ds_buffe
   p.lhs.f64 = f64p(lhs);
   p.rhs.f64 = f64p(rhs);
   p.out.f64 = static_cast<double*>(out->data);
-  return ragged_dot_checked(op, p, {L, R, GS}, {O}, group_sizes, rhs_contracting, workspace,
-                            workspace_bytes, stream);
+  return ragged_dot_checked(op, p, {L, R, GS}, {O}, group_sizes, rhs_contracting, algorithm,
+                            workspace, workspace_bytes, stream);
 }
 
-size_t ds_ragged_dot_contract_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
-                                             const ds_buffer* group_sizes) {
+size_t ds_ragged_dot_contract_algorithm_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
+                                                       const ds_buffer* group_sizes,
+                                                       int32_t algorithm) {
   if (!valid_buffer(lhs) || !valid_buffer(rhs) || !valid_buffer(group_sizes)) return 0;
   if (bad_dims(lhs) || bad_dims(rhs) || bad_dims(group_sizes)) return 0;
   if (total_checked(lhs) < 0 || total_checked(rhs) < 0) return 0;
   const std::string saved = g_last_error;
   RaggedProblem p;
-  const int st = contract_geometry("ds_ragged_dot_contract", lhs, rhs, group_sizes, p);
+  int st = ragged_algorithm("ds_ragged_dot_contract", algorithm, p);
+  if (st == DS_OK) st = contract_geometry("ds_ragged_dot_contract", lhs, rhs, group_sizes, p);
   g_last_error = saved;
-  return st == DS_OK ? ragged_contract_workspace_bytes(p.M, p.K, p.N, p.G) : 0;
+  return st == DS_OK ? ragged_contract_workspace_bytes(p) : 0;
 }
 
-int ds_ragged_dot_contract(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
-                           const ds_buffer* rhs_hi, const ds_buffer* rhs_lo,
-                           const ds_buffer* group_sizes, const ds_buffer* out_hi,
-                           const ds_buffer* out_lo, void* workspace, size_t workspace_bytes,
-                           void* stream) {
+int ds_ragged_dot_contract_algorithm(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
+                                     const ds_buffer* rhs_hi, const ds_buffer* rhs_lo,
+                                     const ds_buffer* group_sizes, int32_t algorithm,
+                                     const ds_buffer* out_hi, const ds_buffer* out_lo,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
   const std::string op("ds_ragged_dot_contract");
   const Named LH{lhs_hi, "lhs_hi", 4, 4}, LL{lhs_lo, "lhs_lo", 4, 4}, RH{rhs_hi, "rhs_hi", 4, 4},
       RL{rhs_lo, "rhs_lo", 4, 4}, GS{group_sizes, "group_sizes", 4, 4},
@@ -1150,13 +1208,14 @@ int ds_ragged_dot_contract(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
   p.rhs.lo = static_cast<const float*>(rhs_lo->data);
   p.out.hi = static_cast<float*>(out_hi->data);
   p.out.lo = static_cast<float*>(out_lo->data);
-  return ragged_contract_checked(op, p, {LH, LL, RH, RL, GS}, {OH, OL}, group_sizes, workspace,
-                                 workspace_bytes, stream);
+  return ragged_contract_checked(op, p, {LH, LL, RH, RL, GS}, {OH, OL}, group_sizes, algorithm,
+                                 workspace, workspace_bytes, stream);
 }
 
-int ds_ragged_dot_contract_f64(const ds_buffer* lhs, const ds_buffer* rhs,
-                               const ds_buffer* group_sizes, const ds_buffer* out,
-                               void* workspace, size_t workspace_bytes, void* stream) {
+int ds_ragged_dot_contract_algorithm_f64(const ds_buffer* lhs, const ds_buffer* rhs,
+                                         const ds_buffer* group_sizes, int32_t algorithm,
+                                         const ds_buffer* out, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
   const std::string op("ds_ragged_dot_contract_f64");
   const Named L{lhs, "lhs", 8, 8}, R{rhs, "rhs", 8, 8}, GS{group_sizes, "group_sizes", 4, 4},
       O{out, "out", 8, 8};
@@ -1165,8 +1224,8 @@ int ds_ragged_dot_contract_f64(const ds_buffer* lhs, const ds_buffer* rhs,
   p.lhs.f64 = f64p(lhs);
   p.rhs.f64 = f64p(rhs);
   p.out.f64 = static_cast<double*>(out->data);
-  return ragged_contract_checked(op, p, {L, R, GS}, {O}, group_sizes, workspace, workspace_bytes,
-                                 stream);
+  return ragged_contract_checked(op, p, {L, R, GS}, {O}, group_sizes, algorithm, workspace,
+                                 workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -148,10 +148,11 @@ struct RaggedProblem {
   const int32_t* group_sizes = nullptr;
   int64_t M = 0, K = 0, N = 0, G = 0;
   bool rhs_t = false;
+  bool tensor = true;  // large groups may take the tensor-core product
 };
-size_t ragged_dot_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, bool rhs_t);
+size_t ragged_dot_workspace_bytes(const RaggedProblem& p);
 int ragged_dot(const RaggedProblem& p, void* workspace, size_t workspace_bytes, cudaStream_t s);
-size_t ragged_contract_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G);
+size_t ragged_contract_workspace_bytes(const RaggedProblem& p);
 int ragged_contract(const RaggedProblem& p, void* workspace, size_t workspace_bytes,
                     cudaStream_t s);
 

@@ -933,7 +933,8 @@ struct Layout {
   bool tensor_ok;
 };
 
-Layout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract, bool rhs_t) {
+Layout layout_of(const RaggedProblem& q, bool contract) {
+  const int64_t M = q.M, K = q.K, N = q.N, G = q.G;
   Layout l{};
   size_t at = 0;
   auto take = [&at](size_t bytes) {
@@ -942,7 +943,7 @@ Layout layout_of(int64_t M, int64_t K, int64_t N, int64_t G, bool contract, bool
     return here;
   };
   const int64_t groups = G < M ? G : M;  // with rows
-  l.tensor_ok = tensor_allowed(M, K, N, G, contract, rhs_t);
+  l.tensor_ok = q.tensor && tensor_allowed(M, K, N, G, contract, q.rhs_t);
   l.small_cap = contract ? 0 : M / kSmallTile + groups;
   if (l.tensor_ok) {
     const int64_t rows = contract && M > kRaggedWindow ? kRaggedWindow : M;
@@ -1084,13 +1085,11 @@ int launch_prep(const RaggedProblem& q, int64_t begin, int64_t end, const Ragged
 
 }  // namespace
 
-size_t ragged_dot_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, bool rhs_t) {
-  return layout_of(M, K, N, G, false, rhs_t).total;
-}
+size_t ragged_dot_workspace_bytes(const RaggedProblem& q) { return layout_of(q, false).total; }
 
 int ragged_dot(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) {
   if (q.M == 0 || q.N == 0) return ok();
-  const Layout l = layout_of(q.M, q.K, q.N, q.G, false, q.rhs_t);
+  const Layout l = layout_of(q, false);
   int clusters = 0;
   if (l.tensor_ok)
     if (int st = ragged_tensor_clusters(&clusters)) return st;
@@ -1114,13 +1113,11 @@ int ragged_dot(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) 
   return q.rhs_t ? launch_products<false>(a, units, s) : launch_products<true>(a, units, s);
 }
 
-size_t ragged_contract_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G) {
-  return layout_of(M, K, N, G, true, false).total;
-}
+size_t ragged_contract_workspace_bytes(const RaggedProblem& q) { return layout_of(q, true).total; }
 
 int ragged_contract(const RaggedProblem& q, void* workspace, size_t, cudaStream_t s) {
   if (q.G == 0 || q.K == 0 || q.N == 0) return ok();
-  const Layout l = layout_of(q.M, q.K, q.N, q.G, true, false);
+  const Layout l = layout_of(q, true);
   int clusters = 0;
   if (l.tensor_ok)
     if (int st = ragged_tensor_clusters(&clusters)) return st;

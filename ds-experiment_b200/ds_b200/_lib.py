@@ -141,6 +141,16 @@ SIGNATURES = {
     "ds_ragged_dot_contract": ([_BUF, _BUF, _BUF, _BUF, _BUF, _BUF, _BUF, _VP, _SZ, _VP],
                                ctypes.c_int),
     "ds_ragged_dot_contract_f64": ([_BUF, _BUF, _BUF, _BUF, _VP, _SZ, _VP], ctypes.c_int),
+    "ds_ragged_dot_algorithm_workspace_size": ([_BUF, _BUF, _I32, _I32], _SZ),
+    "ds_ragged_dot_algorithm": ([_BUF, _BUF, _BUF, _BUF, _BUF, _I32, _I32, _BUF, _BUF, _VP, _SZ,
+                                 _VP], ctypes.c_int),
+    "ds_ragged_dot_algorithm_f64": ([_BUF, _BUF, _BUF, _I32, _I32, _BUF, _VP, _SZ, _VP],
+                                    ctypes.c_int),
+    "ds_ragged_dot_contract_algorithm_workspace_size": ([_BUF, _BUF, _BUF, _I32], _SZ),
+    "ds_ragged_dot_contract_algorithm": ([_BUF, _BUF, _BUF, _BUF, _BUF, _I32, _BUF, _BUF, _VP, _SZ,
+                                          _VP], ctypes.c_int),
+    "ds_ragged_dot_contract_algorithm_f64": ([_BUF, _BUF, _BUF, _I32, _BUF, _VP, _SZ, _VP],
+                                             ctypes.c_int),
     "ds_dot_tensor_plan": ([_I64, ctypes.POINTER(_I32), ctypes.POINTER(_I32)], ctypes.c_int),
     "ds_dot_tensor_kernel_info": ([ctypes.POINTER(_I32), ctypes.POINTER(_I32)], ctypes.c_int),
     "ds_profile_enable": ([ctypes.c_int], None),

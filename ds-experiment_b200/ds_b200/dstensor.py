@@ -196,13 +196,15 @@ class DSTensor:
 
     __matmul__ = matmul
 
-    def ragged_matmul(self, other: "DSTensor", group_sizes: torch.Tensor) -> "DSTensor":
+    def ragged_matmul(self, other: "DSTensor", group_sizes: torch.Tensor,
+                      algorithm: str = "tensor") -> "DSTensor":
         """Rows of consecutive groups, each times its group's matrix: self [M, K],
-        other [G, K, N], int32 group_sizes [G] on the device (ds_ragged_dot)."""
+        other [G, K, N], int32 group_sizes [G] on the device (ds_ragged_dot_f64,
+        with its algorithms)."""
         if not isinstance(other, DSTensor):
             raise TypeError("ragged_matmul takes a DSTensor")
         return DSTensor.from_f64(ops.ds_ragged_dot_f64(self.to_f64(), other.to_f64(),
-                                                       group_sizes))
+                                                       group_sizes, algorithm=algorithm))
 
     def linear_recurrence(self, b: "DSTensor", h0: "DSTensor" = None) -> "DSTensor":
         """h_t = a_t h_{t-1} + b_t along dim -2, self = a [..., T, D], from the

@@ -89,12 +89,14 @@ CONVENTIONS: Dict[str, _Convention] = {
     "ds_linear_recurrence_vjp_f64": _Convention((F64,) * 4, (), (F64,) * 3, "scan", (3,)),
     "ds_linear_recurrence_vjp_f32": _Convention((F32,) * 4, (), (F32,) * 3, "scan", (3,)),
     "ds_linear_recurrence_vjp_packed": _Convention((F32,) * 4, (), (F32,) * 3, "scan", (3,)),
-    "ds_ragged_dot": _Convention((F32, F32, F32, F32, S32), ("rhs_contracting",), (F32, F32),
-                                 "ragged"),
-    "ds_ragged_dot_f64": _Convention((F64, F64, S32), ("rhs_contracting",), (F64,), "ragged"),
-    "ds_ragged_dot_contract": _Convention((F32, F32, F32, F32, S32), (), (F32, F32),
+    "ds_ragged_dot": _Convention((F32, F32, F32, F32, S32), ("rhs_contracting", "algorithm"),
+                                 (F32, F32), "ragged"),
+    "ds_ragged_dot_f64": _Convention((F64, F64, S32), ("rhs_contracting", "algorithm"), (F64,),
+                                     "ragged"),
+    "ds_ragged_dot_contract": _Convention((F32, F32, F32, F32, S32), ("algorithm",), (F32, F32),
                                           "ragged_contract"),
-    "ds_ragged_dot_contract_f64": _Convention((F64, F64, S32), (), (F64,), "ragged_contract"),
+    "ds_ragged_dot_contract_f64": _Convention((F64, F64, S32), ("algorithm",), (F64,),
+                                              "ragged_contract"),
 }
 
 # The reference's target names, each bound to its replacement entry point.
@@ -382,30 +384,29 @@ class _Plan:
     """What a recurrence or grouped product of given shapes needs of each call:
     built on its first call, read-only afterwards."""
     __slots__ = ("fn", "dtypes", "present", "specs", "like", "table", "offsets", "workspace",
-                 "attr", "keep")
+                 "attrs", "keep")
 
 
-# (entry point, device index, rhs_contracting, operand shapes...) -> _Plan
+# (entry point, device index, rhs_contracting, algorithm, operand shapes...) -> _Plan
 _plans: Dict[tuple, _Plan] = {}
 _fast_fns: Dict[str, object] = {}
 
 
-def _fast_fn(sym, kind, n):
+def _fast_fn(entry, operands, attrs, results):
     """The entry point with every descriptor passed as an address: three words
     (data, dims, rank) in one array for the whole call."""
-    fn = _fast_fns.get(sym)
+    fn = _fast_fns.get(entry)
     if fn is None:
-        fn = _lib.lib()[sym]  # a function object of its own
-        argtypes = [ctypes.c_void_p] * n
-        if kind == "ragged":
-            argtypes.insert(n - len(CONVENTIONS[sym].results), ctypes.c_int32)
-        fn.argtypes = argtypes + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        fn = _lib.lib()[entry]  # a function object of its own
+        fn.argtypes = ([ctypes.c_void_p] * operands + [ctypes.c_int32] * attrs +
+                       [ctypes.c_void_p] * results +
+                       [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p])
         fn.restype = ctypes.c_int
-        _fast_fns[sym] = fn
+        _fast_fns[entry] = fn
     return fn
 
 
-def _make_plan(sym, conv, args, specs, contracting):
+def _make_plan(sym, conv, args, specs, contracting, algorithm):
     plan = _Plan()
     L = _lib.lib()
     plan.dtypes = conv.args
@@ -424,10 +425,12 @@ def _make_plan(sym, conv, args, specs, contracting):
     plan.like = [next((i for i, t in enumerate(args)
                        if t is not None and tuple(t.shape) == s.shape and t.dtype == s.dtype), None)
                  for s in specs]
-    n = len(plan.offsets)
-    plan.attr = contracting if conv.kind == "ragged" else None
-    if plan.attr is not None:
-        plan.offsets.insert(len(args), None)
+    entry = sym
+    plan.attrs = [contracting] if conv.kind == "ragged" else []
+    if algorithm != _lib.DS_DOT_TENSOR_INT8:  # the entry points that take one
+        entry = sym[:-4] + "_algorithm_f64" if sym.endswith("_f64") else sym + "_algorithm"
+        plan.attrs.append(algorithm)
+    plan.offsets[len(args):len(args)] = [None] * len(plan.attrs)
 
     def ref(t):
         b, d = _lib.make_buffer(t.data_ptr(), t.shape)
@@ -438,11 +441,12 @@ def _make_plan(sym, conv, args, specs, contracting):
         plan.workspace = L.ds_linear_recurrence_workspace_size(
             ref(args[0]), _SCAN_TYPES[sym.rsplit("_", 1)[1]])
     elif conv.kind == "ragged":
-        plan.workspace = L.ds_ragged_dot_workspace_size(ref(args[0]), ref(args[-2]), contracting)
+        plan.workspace = L.ds_ragged_dot_algorithm_workspace_size(
+            ref(args[0]), ref(args[-2]), contracting, algorithm)
     else:
-        plan.workspace = L.ds_ragged_dot_contract_workspace_size(ref(args[0]), ref(args[-2]),
-                                                                 ref(args[-1]))
-    plan.fn = _fast_fn(sym, conv.kind, n)
+        plan.workspace = L.ds_ragged_dot_contract_algorithm_workspace_size(
+            ref(args[0]), ref(args[-2]), ref(args[-1]), algorithm)
+    plan.fn = _fast_fn(entry, len(args), len(plan.attrs), len(specs))
     return plan
 
 
@@ -455,10 +459,11 @@ def _invoke_sequence(target_name, sym, conv, specs, args, attrs, device, out):
         if t.device != device:
             raise ValueError(f"{target_name} result {i}: results must be on the operands' device")
     contracting = int(attrs.get("rhs_contracting", 1))
-    key = _plan_key(sym, device.index, contracting, args)
+    algorithm = int(attrs.get("algorithm", _lib.DS_DOT_TENSOR_INT8))
+    key = _plan_key(sym, device.index, contracting, algorithm, args)
     plan = _plans.get(key)
     if plan is None or plan.specs != [(s.shape, s.dtype) for s in specs]:
-        plan = _make_plan(sym, conv, args, specs, contracting)
+        plan = _make_plan(sym, conv, args, specs, contracting, algorithm)
     outs = _run_plan(target_name, plan, args, device.index, out)
     if len(_plans) > 512:
         _plans.clear()
@@ -466,8 +471,8 @@ def _invoke_sequence(target_name, sym, conv, specs, args, attrs, device, out):
     return outs
 
 
-def _plan_key(sym, index, contracting, args):
-    return (sym, index, contracting, *[None if t is None else t.shape for t in args])
+def _plan_key(sym, index, contracting, algorithm, args):
+    return (sym, index, contracting, algorithm, *[None if t is None else t.shape for t in args])
 
 
 def _run_plan(target_name, plan, args, index, out):
@@ -486,8 +491,8 @@ def _run_plan(target_name, plan, args, index, out):
         at += 3
     base = table.buffer_info()[0]
     words = [None if o is None else base + o for o in plan.offsets]
-    if plan.attr is not None:
-        words[len(args)] = plan.attr
+    if plan.attrs:
+        words[len(args):len(args) + len(plan.attrs)] = plan.attrs
     stream = _lib.current_stream_ptr(index)
     ws, wsp = None, None
     if plan.workspace:
@@ -497,7 +502,8 @@ def _run_plan(target_name, plan, args, index, out):
     return out
 
 
-def sequence_call(target_name, args, specs, out=None, rhs_contracting=1):
+def sequence_call(target_name, args, specs, out=None, rhs_contracting=1,
+                  algorithm=_lib.DS_DOT_TENSOR_INT8):
     """ffi_call of a recurrence or grouped product without the per-call set-up:
     the plan of operands of these shapes is looked up, and operands that a
     plan's first call would accept go straight to the entry point.  `specs()`
@@ -507,7 +513,8 @@ def sequence_call(target_name, args, specs, out=None, rhs_contracting=1):
     if isinstance(first, torch.Tensor) and first.is_cuda:
         index = first.get_device()
         try:
-            plan = _plans.get(_plan_key(_registry[target_name], index, rhs_contracting, args))
+            plan = _plans.get(_plan_key(_registry[target_name], index, rhs_contracting, algorithm,
+                                        args))
         except (AttributeError, TypeError):
             plan = None
         if plan is not None and out is None and torch.cuda.current_device() == index:
@@ -519,8 +526,8 @@ def sequence_call(target_name, args, specs, out=None, rhs_contracting=1):
                 outs = _run_plan(target_name, plan, args, index, None)
                 return outs[0] if len(outs) == 1 else tuple(outs)
     results = specs()
-    attrs = {"rhs_contracting": rhs_contracting} \
-        if CONVENTIONS[_registry[target_name]].kind == "ragged" else {}
+    attrs = {k: v for k, v in (("rhs_contracting", rhs_contracting), ("algorithm", algorithm))
+             if k in CONVENTIONS[_registry[target_name]].attrs}
     return ffi_call(target_name, results if len(results) > 1 else results[0])(*args, out=out,
                                                                               **attrs)
 

@@ -329,40 +329,52 @@ def _ragged_shape(lhs, rhs, rhs_contracting):
     return tuple(lhs.shape[:1]) + tuple(rhs.shape[3 - int(rhs_contracting):][:1])
 
 
-def ds_ragged_dot_f64(lhs, rhs, group_sizes, rhs_contracting: int = 1, out=None):
+def ds_ragged_dot_f64(lhs, rhs, group_sizes, rhs_contracting: int = 1, out=None,
+                      algorithm: str = "tensor"):
     """Rows of consecutive groups, each times its group's matrix: f64 lhs
     [M, K], rhs [G, K, N] (rhs_contracting=2: [G, N, K]), int32 group_sizes
     [G] on the device -> [M, N], zeros in rows behind the last group.  The
     gradient of the rows is this product of the result's gradient with the
     same matrices and the other rhs_contracting; that of the matrices is
-    ds_ragged_dot_contract_f64."""
+    ds_ragged_dot_contract_f64.
+
+    algorithm="cuda_core" sums in f64.  "tensor" does so for groups below 128
+    rows (contracted: 256) and where the tensor cores would not be faster; of
+    the rows and matrix columns of the other groups it keeps 46 to 50 bits below
+    the largest value of each, and certifies every output to 2^-24 of it (others
+    are summed again), so that a row with a few values far above the rest loses
+    bits that f64 sums keep."""
     return sequence_call("ds_ragged_dot_f64", (lhs, rhs, group_sizes),
                          lambda: (_sds(_ragged_shape(lhs, rhs, rhs_contracting), F64),), out,
-                         rhs_contracting)
+                         rhs_contracting, _ALGOS[algorithm])
 
 
-def ds_ragged_dot(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes, rhs_contracting: int = 1, out=None):
+def ds_ragged_dot(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes, rhs_contracting: int = 1, out=None,
+                  algorithm: str = "tensor"):
     """ds_ragged_dot_f64 on SoA DS operands -> (hi, lo)."""
     return sequence_call("ds_ragged_dot", (lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes),
                          lambda: (_sds(_ragged_shape(lhs_hi, rhs_hi, rhs_contracting), F32),) * 2,
-                         out, rhs_contracting)
+                         out, rhs_contracting, _ALGOS[algorithm])
 
 
 def _contract_shape(lhs, rhs, group_sizes):
     return tuple(group_sizes.shape[:1]) + tuple(lhs.shape[1:2]) + tuple(rhs.shape[1:2])
 
 
-def ds_ragged_dot_contract_f64(lhs, rhs, group_sizes, out=None):
+def ds_ragged_dot_contract_f64(lhs, rhs, group_sizes, out=None, algorithm: str = "tensor"):
     """out[g] = lhs_g^T rhs_g over the rows of each group: f64 lhs [M, K],
     rhs [M, N], int32 group_sizes [G] -> [G, K, N].  With lhs the rows and
-    rhs the result's gradient: the gradient of ds_ragged_dot_f64's matrices."""
+    rhs the result's gradient: the gradient of ds_ragged_dot_f64's matrices, with
+    its algorithms."""
     return sequence_call("ds_ragged_dot_contract_f64", (lhs, rhs, group_sizes),
-                         lambda: (_sds(_contract_shape(lhs, rhs, group_sizes), F64),), out)
+                         lambda: (_sds(_contract_shape(lhs, rhs, group_sizes), F64),), out,
+                         algorithm=_ALGOS[algorithm])
 
 
-def ds_ragged_dot_contract(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes, out=None):
+def ds_ragged_dot_contract(lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes, out=None,
+                           algorithm: str = "tensor"):
     """ds_ragged_dot_contract_f64 on SoA DS operands -> (hi, lo)."""
     return sequence_call("ds_ragged_dot_contract",
                          (lhs_hi, lhs_lo, rhs_hi, rhs_lo, group_sizes),
                          lambda: (_sds(_contract_shape(lhs_hi, rhs_hi, group_sizes), F32),) * 2,
-                         out)
+                         out, algorithm=_ALGOS[algorithm])

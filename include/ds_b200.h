@@ -65,7 +65,8 @@ enum {
   /* exact integer-residue (Ozaki scheme II) GEMM on the int8 tcgen05 tensor
      cores; the default */
   DS_DOT_TENSOR_INT8 = 0,
-  /* CUDA-core GEMM: exact f32 products (two_prod) summed in DS arithmetic */
+  /* CUDA-core GEMM: exact f32 products (two_prod) summed in DS arithmetic (the
+     products grouped by expert: f64 sums) */
   DS_DOT_CUDA_CORE = 1
 };
 
@@ -485,10 +486,22 @@ DS_API int ds_linear_recurrence_vjp_packed(const ds_buffer* a, const ds_buffer* 
    Sizes are read on the device, so a captured call may be replayed with
    others: a negative size counts as 0, and groups end at row M.  A group with
    no rows does not read its matrix.
-   Operands are f64, or DS pairs as hi / lo tensors of one shape; the result
-   is rounded once from f64 accumulations (CUDA-core and small groups) or
-   from the exact integer products of ds_dot_general's tensor-core path, whose
-   uncertified outputs are summed again in double-length arithmetic.  Row i
+   Operands are f64, or DS pairs as hi / lo tensors of one shape, and the
+   result is rounded once.  Which sums it comes from is the algorithm's choice
+   (the entry points without one take DS_DOT_TENSOR_INT8):
+     DS_DOT_CUDA_CORE: f64 sums, off by at most (K + 20) 2^-53 of the sum of
+     the terms' magnitudes.
+     DS_DOT_TENSOR_INT8: the same for groups below 128 rows (contracted: 256)
+     and for calls that the tensor cores would not speed up.  The other groups
+     take the exact integer products of ds_dot_general's tensor-core path: of
+     each row of lhs and each column of a matrix P bits below the largest
+     magnitude are kept (P = 50 for a contraction of 128, 48 for 2048, 46 for
+     32768, which longer ones are cut into), and an output's error is certified
+     to be at most 2^-24 of it; outputs that are not are summed again in
+     double-length arithmetic.  So where a few values are far larger than the
+     rest of their row or column, outputs that they do not reach have fewer
+     bits than f64 sums would give them.
+   Row i
    depends on the group sizes only through the group it lies in and that
    group's size (a call with more than 2^20 uncertified outputs sums every
    output of its large groups again).  `out` must not overlap operands.
@@ -504,13 +517,25 @@ DS_API int ds_ragged_dot_f64(const ds_buffer* lhs, const ds_buffer* rhs,
                              const ds_buffer* group_sizes, int32_t rhs_contracting,
                              const ds_buffer* out, void* workspace, size_t workspace_bytes,
                              void* stream);
+DS_API size_t ds_ragged_dot_algorithm_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
+                                                     int32_t rhs_contracting, int32_t algorithm);
+DS_API int ds_ragged_dot_algorithm(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
+                                   const ds_buffer* rhs_hi, const ds_buffer* rhs_lo,
+                                   const ds_buffer* group_sizes, int32_t rhs_contracting,
+                                   int32_t algorithm, const ds_buffer* out_hi,
+                                   const ds_buffer* out_lo, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+DS_API int ds_ragged_dot_algorithm_f64(const ds_buffer* lhs, const ds_buffer* rhs,
+                                       const ds_buffer* group_sizes, int32_t rhs_contracting,
+                                       int32_t algorithm, const ds_buffer* out, void* workspace,
+                                       size_t workspace_bytes, void* stream);
 
 /* The groups along the contraction: lhs [M, K], rhs [M, N], group_sizes
    s32[G] -> out [G, K, N], out[g] = lhs_g^T rhs_g over the rows of group g
    (zeros for a group without rows; rows behind the last group take no part).
    With lhs the rows and rhs the gradient of ds_ragged_dot's result this is
-   the gradient of its matrices.  Group sizes, types, overlap and workspace
-   as above. */
+   the gradient of its matrices.  Group sizes, types, algorithms (K the rows of
+   a group), overlap and workspace as above. */
 DS_API size_t ds_ragged_dot_contract_workspace_size(const ds_buffer* lhs, const ds_buffer* rhs,
                                                     const ds_buffer* group_sizes);
 DS_API int ds_ragged_dot_contract(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
@@ -521,6 +546,19 @@ DS_API int ds_ragged_dot_contract(const ds_buffer* lhs_hi, const ds_buffer* lhs_
 DS_API int ds_ragged_dot_contract_f64(const ds_buffer* lhs, const ds_buffer* rhs,
                                       const ds_buffer* group_sizes, const ds_buffer* out,
                                       void* workspace, size_t workspace_bytes, void* stream);
+DS_API size_t ds_ragged_dot_contract_algorithm_workspace_size(const ds_buffer* lhs,
+                                                              const ds_buffer* rhs,
+                                                              const ds_buffer* group_sizes,
+                                                              int32_t algorithm);
+DS_API int ds_ragged_dot_contract_algorithm(const ds_buffer* lhs_hi, const ds_buffer* lhs_lo,
+                                            const ds_buffer* rhs_hi, const ds_buffer* rhs_lo,
+                                            const ds_buffer* group_sizes, int32_t algorithm,
+                                            const ds_buffer* out_hi, const ds_buffer* out_lo,
+                                            void* workspace, size_t workspace_bytes, void* stream);
+DS_API int ds_ragged_dot_contract_algorithm_f64(const ds_buffer* lhs, const ds_buffer* rhs,
+                                                const ds_buffer* group_sizes, int32_t algorithm,
+                                                const ds_buffer* out, void* workspace,
+                                                size_t workspace_bytes, void* stream);
 
 /* ---- diagnostics (no reference counterpart) ------------------------------ */
 

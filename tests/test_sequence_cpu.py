@@ -216,3 +216,34 @@ def test_no_groups_ask_for_no_planes(L):
         assert 0 < q(R(b(8192, 1024)), R(w), contracting) <= 1 << 20
     assert 0 < L.lib().ds_ragged_dot_contract_workspace_size(
         R(b(8192, 1024)), R(b(8192, 1024)), R(b(0))) <= 1 << 20
+
+
+def test_ragged_algorithms(L):
+    """The entry points that take an algorithm refuse what the others do and unknown
+    algorithms; f64 sums need no planes."""
+    b = Bufs(L)
+    lib = L.lib()
+    x, w, s, o = b(8, 4), b(3, 4, 6), b(3), b(8, 6)
+    f = "ds_ragged_dot_algorithm_f64"
+    refused(L, f, (R(x), R(w), R(s), 1, 7, R(o), WS, BIG, None), "unknown algorithm")
+    refused(L, f, (R(x), R(w), R(s), 2, 1, R(o), WS, BIG, None), "contracting dimensions")
+    refused(L, f, (R(x), R(w), R(s), 1, 1, R(x), WS, BIG, None), "output shape")
+    refused(L, f, (R(x), R(w), R(s), 1, 1, R(o), None, 0, None), "workspace")
+    refused(L, "ds_ragged_dot_algorithm",
+            (R(x), R(x), R(w), R(w), R(s), 1, -1, R(o), R(b(8, 6)), WS, BIG, None), "unknown")
+    y, oc = b(8, 6), b(3, 4, 6)
+    f = "ds_ragged_dot_contract_algorithm_f64"
+    refused(L, f, (R(x), R(y), R(s), 2, R(oc), WS, BIG, None), "unknown algorithm")
+    refused(L, f, (R(x), R(y), R(s), 1, R(b(3, 6, 4)), WS, BIG, None), "output shape")
+    refused(L, "ds_ragged_dot_contract_algorithm",
+            (R(x), R(x), R(y), R(y), R(s), 9, R(oc), R(b(3, 4, 6)), WS, BIG, None), "unknown")
+    q = lib.ds_ragged_dot_algorithm_workspace_size
+    big = (R(b(8192, 2048)), R(b(8, 2048, 2048)), 1)
+    assert q(*big, L.DS_DOT_TENSOR_INT8) == lib.ds_ragged_dot_workspace_size(*big) > 1 << 28
+    assert 0 < q(*big, L.DS_DOT_CUDA_CORE) <= 1 << 20
+    assert q(*big, 5) == 0
+    q = lib.ds_ragged_dot_contract_algorithm_workspace_size
+    big = (R(b(8192, 2048)), R(b(8192, 2048)), R(b(8)))
+    assert q(*big, L.DS_DOT_TENSOR_INT8) == lib.ds_ragged_dot_contract_workspace_size(*big) > 1 << 28
+    assert 0 < q(*big, L.DS_DOT_CUDA_CORE) <= 1 << 20
+    assert q(*big, 5) == 0
