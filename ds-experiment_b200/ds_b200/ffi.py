@@ -176,7 +176,7 @@ def _buf(t):
 # host thread) and reused: one thread's calls on one stream run in order, so one
 # buffer serves them all, and a call skips an allocation.  (Two threads that
 # launch on one stream take turns launch by launch, and a call has several.)
-# The buffer starts at 1 MiB and grows
+# They end with their thread.  The buffer starts at 1 MiB and grows
 # to the next power of two a request needs; the one it replaces was
 # allocated on the same stream, so torch's allocator hands its memory out
 # again only to work ordered after the calls that used it.  Larger ones come
@@ -185,6 +185,15 @@ def _buf(t):
 _SMALL_WORKSPACE = 1 << 20
 _CACHED_WORKSPACE_MAX = 64 << 20
 _workspaces: Dict[tuple, torch.Tensor] = {}
+_thread = threading.local()
+
+
+class _ThreadKeys(set):
+    """The keys of a thread's workspaces, held by the thread."""
+
+    def __del__(self):
+        for key in self if _workspaces is not None else ():  # None: the interpreter ends
+            _workspaces.pop(key, None)
 
 
 def _workspace(nbytes: int, device, stream: int = 0) -> torch.Tensor:
@@ -196,6 +205,9 @@ def _workspace(nbytes: int, device, stream: int = 0) -> torch.Tensor:
     if ws is None or ws.numel() < nbytes:
         if ws is None and len(_workspaces) > 64:
             _workspaces.clear()
+        if not hasattr(_thread, "keys"):
+            _thread.keys = _ThreadKeys()
+        _thread.keys.add(key)
         size = max(_SMALL_WORKSPACE, 1 << (nbytes - 1).bit_length())
         ws = _workspaces[key] = torch.empty(size, dtype=torch.uint8, device=device)
     return ws

@@ -247,3 +247,24 @@ def test_ragged_algorithms(L):
     assert q(*big, L.DS_DOT_TENSOR_INT8) == lib.ds_ragged_dot_contract_workspace_size(*big) > 1 << 28
     assert 0 < q(*big, L.DS_DOT_CUDA_CORE) <= 1 << 20
     assert q(*big, 5) == 0
+
+
+def test_workspaces_end_with_their_thread(monkeypatch):
+    import threading
+    import torch
+    from ds_b200 import ffi
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(ffi, "_workspaces", {})
+    here = ffi._workspace(100, torch.device("cpu"), 7)
+
+    def work():
+        for stream in (7, 8):
+            ffi._workspace(100, torch.device("cpu"), stream)
+        assert len(ffi._workspaces) == 3
+
+    for _ in range(3):
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+        assert list(ffi._workspaces) == [(None, 7, threading.get_ident())]
+    assert ffi._workspace(100, torch.device("cpu"), 7) is here
