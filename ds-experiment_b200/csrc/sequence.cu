@@ -38,8 +38,8 @@
 // with every chunk stepped [8, 2048, 1024] of f64 takes 119 us instead of 69,
 // [1, 65536, 250], whose chunks then wait for one another, 2.7 ms instead of 110 us.
 //
-// Measured on one B200 (cold L2, launch included): f64 [8, 2048, 1024] 80 us =
-// 5.0 TB/s, its gradient 129 us = 5.2 TB/s, [1, 65536, 250] 112 us, f32 [4, 4096,
+// Measured on one B200 (cold L2, launch included): f64 [8, 2048, 1024] 76 us =
+// 5.3 TB/s, its gradient 121 us = 5.5 TB/s, [1, 65536, 250] 113 us, f32 [4, 4096,
 // 2048] 90 us.  A plain kernel that reads two arrays of that size and writes a
 // third takes 70 us (5.8 TB/s), whatever the width of its rows.
 #include <mutex>
@@ -726,8 +726,9 @@ scan_chunk_kernel(const __grid_constant__ ChunkArgs<E> p) {
 
 // Steps of one channel per thread, half as many of two channels (f32; f64 and
 // pairs).  Registers hold two (gradient: three) f64 values of each: two blocks per
-// SM with 128 registers.  8 or 12 of f64 instead of 16 were 5 to 15% slower, 20
-// and 24 of f32 4 to 8%, 6 and 8 of the gradient's 10 up to 18%.
+// SM with 128 registers.  12 of f64 instead of 16 take as long for [8, 2048, 1024]
+// and 14% longer for [1, 65536, 250] (76 and 113 us), 8 5% and 40%, 20 of f32 9% for
+// [4, 4096, 2048]; 6 or 8 of the f64 gradient's 10 are within 2% for [8, 2048, 1024].
 constexpr int steps_of(int type, bool gradient) {
   return type == 1 ? (gradient ? 12 : 16) : (gradient ? 10 : 16);
 }
@@ -755,11 +756,11 @@ constexpr int64_t kBlocks = 296;
 // Channels per unit, and who carries the state.  Where tiles of 64, 32 or 16
 // channels keep at least 0.8 of the blocks busy, each block takes whole tiles,
 // chunk by chunk, and nothing is waited for: [8, 2048, 1024] of f64 in 256 tiles
-// of 32 takes 80 us, through the workspace 84, and f32 [4, 4096, 2048] 98 and 104.
+// of 32 takes 76 us, through the workspace 83, and f32 [4, 4096, 2048] 92 and 112.
 // Otherwise the chunks of all tiles are shared out: 64 channels per unit (512
 // contiguous bytes of f64 per step), 16 where the channels are few, so that a
-// unit has more steps and the chain fewer hops ([1, 65536, 250]: 115 us, with 64
-// channels 145), 4 for a handful of channels.  The workspace holds the counter,
+// unit has more steps and the chain fewer hops ([1, 65536, 250]: 113 us, with 64
+// channels 144), 4 for a handful of channels.  The workspace holds the counter,
 // the error word, maps and states; every call sets it to ones.
 Plan plan_of(int64_t B, int64_t T, int64_t D, int steps) {
   Plan g{};

@@ -435,7 +435,8 @@ DS_API int ds_fused_reduce_rows_compile_check(const ds_fused_op* ops, int32_t n_
    finite state stood before.  Where the products of a chunk's coefficients
    leave the f64 range (which no state need do) its channel is stepped through
    as in that loop, at a lower speed; what a product below 2^-1022 leaves of a
-   state up to 2^64 counts as zero to within 2^-994.
+   state up to 2^64 counts as zero to within 2^-994.  A chunk that waits for an
+   earlier one for more than about 2 s goes on with NaN.
    Outputs must not overlap operands.  The workspace
    (ds_linear_recurrence_workspace_size bytes, 256-byte aligned; `type` is
    DS_FUSED_F64, DS_FUSED_F32 or DS_FUSED_PACKED) serves one call at a time. */
