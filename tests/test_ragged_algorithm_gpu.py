@@ -163,3 +163,16 @@ def test_algorithms_take_turns():
             assert torch.equal(outs[0], t) and torch.equal(outs[1], c)
     with pytest.raises(KeyError):
         calls[0](algorithm="f16")
+
+
+def test_ds_tensors_choose():
+    from ds_b200 import ops
+    from ds_b200.dstensor import DSTensor
+    M, K, N, sizes = LARGE[1]
+    x, w, s = on_gpu(M, K, seed=9), on_gpu(len(sizes), K, N, seed=10), sz(sizes)
+    X, W = DSTensor.from_f64(x), DSTensor.from_f64(w)
+    for algorithm in ("tensor", "cuda_core"):
+        want = ops.ds_from_f64(ops.ds_ragged_dot_f64(X.to_f64(), W.to_f64(), s,
+                                                     algorithm=algorithm))
+        assert torch.equal(X.ragged_matmul(W, s, algorithm=algorithm).packed, want)
+    assert torch.equal(X.ragged_matmul(W, s).packed, X.ragged_matmul(W, s, "tensor").packed)
